@@ -561,6 +561,26 @@ int tfc_norm_act_bwd2(const tfc_gate_seg* segs, int32_t n_segs, const float* x, 
                       int64_t n_rows, int32_t d, float eps_squared, int32_t normalize, float* gx, tfc_stream_t stream);
 
 /* ------------------------------------------------------------------------------------------
+ * Element types of the calls below (all tensors of a call have the one type; sums, statistics and moments of the
+ * optimizer are fp32, or fp64 where stated).  Rows and views may start at any multiple of the element size.
+ */
+#define TFC_F32 0
+#define TFC_BF16 1
+#define TFC_F16 2
+
+/* Layer norm over the last axis of x [rows, d]: y = (x - mean) rstd w + b, mean = sum x / d,
+ * rstd = (sum (x - mean)^2 / d + eps)^-1/2 (no counterpart in the reference's two target models).  w, b [d] may be null
+ * (ones / zeros).  mean, rstd [rows] fp32 are what the backward pass needs; both null: not written.
+ * Backward: dx [rows, d], dw [d], db [d], each nullable; the column sums are taken in a fixed order over
+ * tfc_layer_norm_bwd_workspace_floats() floats of workspace (needed for dw or db only).  rows = 0: dw = db = 0. */
+int tfc_layer_norm_fwd(const void* x, const void* w, const void* b, int64_t rows, int64_t d, float eps, int32_t dtype,
+                       void* y, float* mean, float* rstd, tfc_stream_t stream);
+int64_t tfc_layer_norm_bwd_workspace_floats(int64_t rows, int64_t d, int32_t dtype);
+int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float* mean, const float* rstd, int64_t rows,
+                       int64_t d, int32_t dtype, void* dx, void* dw, void* db, float* workspace, int64_t workspace_floats,
+                       tfc_stream_t stream);
+
+/* ------------------------------------------------------------------------------------------
  * Opt-in kernel timing (no counterpart in the reference, whose only timer is the epoch wall
  * clock, eigenn/model/utils.py:4-35).  While enabled, every main kernel launch is bracketed by
  * HIP events on its own stream.  tfc_profile_report() synchronises on those events and writes

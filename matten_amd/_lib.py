@@ -100,6 +100,7 @@ class GateSeg(C.Structure):
 
 
 EPI_NONE, EPI_SSP, EPI_SSP_GRAD = 0, 1, 2
+F32, BF16, F16 = 0, 1, 2
 ACT = {"identity": 0, "ssp": 1, "silu": 2, "tanh": 3, "abs": 4, "sigmoid": 5}
 
 _P = C.c_void_p
@@ -173,6 +174,9 @@ SIGNATURES = {
     "tfc_fctp_rows_numel": (C.c_int64, [_P, _I32, _I32]),
     "tfc_fctp_rows_w": (C.c_int, [_P, _I32, _P, _I32, _I32, _P, _I64, _P, _P]),
     "tfc_fctp_rows_dw": (C.c_int, [_P, _I32, _P, _I32, _I32, _P, _I64, _P, _P]),
+    "tfc_layer_norm_fwd": (C.c_int, [_P, _P, _P, _I64, _I64, _F, _I32, _P, _P, _P, _P]),
+    "tfc_layer_norm_bwd_workspace_floats": (_I64, [_I64, _I64, _I32]),
+    "tfc_layer_norm_bwd": (C.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P]),
     "tfc_gate_fwd_t": (C.c_int, [C.POINTER(GateSeg), _I32, _P, _I64, _I32, _I32, _P, C.POINTER(IrBlock), _I32, _P, _P]),
     "tfc_gate_bwd_t": (C.c_int, [C.POINTER(GateSeg), _I32, _P, _P, _I64, _I32, _I32, _P, C.POINTER(IrBlock), _I32, _P, _P]),
 }

@@ -38,6 +38,7 @@ __all__ = [
     "GateSpec",
     "gate",
     "norm_activation",
+    "layer_norm",
 ]
 
 
@@ -1885,3 +1886,105 @@ def norm_activation(x, spec: GateSpec, eps_squared: float = 0.0, normalize: bool
     """e3nn.nn.NormActivation on [N, d] rows (tfc_norm_act_fwd/bwd); `spec.segs`: one
     (in_off, in_off, mul, 2l+1, -1, act, 1.0) per block."""
     return _NormActFn.apply(_tracked(x), spec, float(eps_squared), bool(normalize))
+
+
+# ------------------------------------------------------------------ scalar head: layer norm
+
+_dtype_codes = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
+
+
+def _floats(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None):
+    """Checks of the operators that take fp32, bf16 and fp16: on a ROCm device, one of the three types, and the type and
+    device of `like`."""
+    if not t.is_cuda:
+        raise RuntimeError(f"matten_amd: `{name}` must live on a ROCm device (no CPU fallback exists); got {t.device}")
+    if t.dtype not in _dtype_codes:
+        raise TypeError(f"matten_amd: `{name}` must be float32, bfloat16 or float16, got {t.dtype}")
+    if like is not None:
+        if t.dtype != like.dtype:
+            raise TypeError(f"matten_amd: `{name}` is {t.dtype}, the input {like.dtype}: one type per call")
+        if t.device != like.device:
+            raise RuntimeError(f"matten_amd: `{name}` is on {t.device}, the input on {like.device}")
+
+
+def _layer_norm_run(x, w, b, eps: float, keep: bool):
+    """(y, stats): rows of a contiguous [rows, d] tensor; `keep`: stats [2, rows] holds the mean and 1 / deviation of every row."""
+    rows, d = x.shape
+    y = torch.empty_like(x)
+    stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
+    with torch.cuda.device(x.device):
+        _lib.check(_lib.lib().tfc_layer_norm_fwd(_ptr(x), _ptr(w), _ptr(b), rows, d, eps, _dtype_codes[x.dtype], _ptr(y), _ptr(stats),
+                                                 _ptr(stats, rows) if keep else None, _stream()))
+    return y, stats
+
+
+class _LayerNormFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w, b, eps: float):
+        y, stats = _layer_norm_run(x, w, b, eps, True)
+        ctx.save_for_backward(x, w, b, stats)
+        ctx.eps = eps
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        x, w, b, stats = ctx.saved_tensors
+        need = ctx.needs_input_grad
+        if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
+            return (*_differentiable_grads(lambda: _layer_norm_composite(x, w, b, ctx.eps), (x, w, b), need, g), None)
+        rows, d = x.shape
+        g = g.contiguous()
+        dx = torch.empty_like(x) if need[0] else None
+        dw = torch.empty_like(w) if need[1] else None
+        db = torch.empty_like(b) if need[2] else None
+        L = _lib.lib()
+        dt = _dtype_codes[x.dtype]
+        with torch.cuda.device(x.device):
+            ws = None
+            if need[1] or need[2]:
+                ws = torch.empty(int(L.tfc_layer_norm_bwd_workspace_floats(rows, d, dt)), dtype=torch.float32, device=x.device)
+            _lib.check(L.tfc_layer_norm_bwd(_ptr(g), _ptr(x), _ptr(w), _ptr(stats), _ptr(stats, rows), rows, d, dt, _ptr(dx), _ptr(dw),
+                                            _ptr(db), _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
+        return dx, dw, db, None
+
+
+def _differentiable_grads(fn, inputs, need, g):
+    """Gradients of fn() with respect to the `inputs` that need one, as a graph of their own (None for the others)."""
+    with torch.enable_grad():
+        grads = iter(torch.autograd.grad(fn(), [t for t, n in zip(inputs, need) if n], g, create_graph=True))
+    return [next(grads) if n else None for _, n in zip(inputs, need)]
+
+
+def _layer_norm_composite(x, w, b, eps: float):
+    v = x.float()
+    v = v - v.mean(-1, keepdim=True)
+    v = v * torch.rsqrt((v * v).mean(-1, keepdim=True) + eps)
+    if w is not None:
+        v = v * w.float()
+    if b is not None:
+        v = v + b.float()
+    return v.to(x.dtype)
+
+
+def layer_norm(x, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5):
+    """y = (x - mean) / sqrt(var + eps) * weight + bias over the last axis (tfc_layer_norm_fwd/bwd); x [..., d], weight and bias
+    [d] or None, all fp32, bf16 or fp16.  Statistics and the sums behind the gradients are fp32 whatever the type; results are
+    the same from run to run.  Differentiable to any order: the first-order backward is the fused kernel, a backward that is
+    itself differentiated (`create_graph=True`) is composed of torch operations."""
+    _floats(x, "x")
+    if x.dim() < 1 or x.shape[-1] < 1:
+        raise ValueError(f"layer_norm: x must have a last axis to normalise, got shape {tuple(x.shape)}")
+    if not 0.0 <= eps < math.inf:
+        raise ValueError(f"layer_norm: eps must be finite and not negative, got {eps}")
+    d = x.shape[-1]
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _floats(t, name, x)
+            if t.shape != (d,):
+                raise ValueError(f"layer_norm: `{name}` must have shape ({d},), got {tuple(t.shape)}")
+    rows, w, b = _tracked(x.reshape(-1, d)), _tracked(weight), _tracked(bias)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+        y = _LayerNormFn.apply(rows, w, b, float(eps))
+    else:
+        y = _layer_norm_run(rows, w, b, float(eps), False)[0]
+    return y.reshape(x.shape)
