@@ -580,6 +580,43 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
                        int64_t d, int32_t dtype, void* dx, void* dw, void* db, float* workspace, int64_t workspace_floats,
                        tfc_stream_t stream);
 
+/* One AdamW step over many parameter tensors of one dtype (the reference's trainer steps torch.optim one tensor at a time,
+ * eigenn/model/model.py:410-426).  With g the gradient, scaled by min(1, max_norm / (norm + 1e-6)) when max_norm > 0, and
+ * t = ++*step of the tensor:
+ *   m = b1 m + (1 - b1) g,  v = b2 v + (1 - b2) g g,
+ *   p = (1 - lr wd) p - lr / (1 - b1^t) m / (sqrt(v) / sqrt(1 - b2^t) + eps)
+ * in fp32 whatever the parameters' type.  state_bits 32: m, v [n] fp32.  state_bits 8: m and v hold e4m3 codes of m and of
+ * sqrt(v), one byte each, n rounded up to whole blocks of 256 (the padding zero, starting at a multiple of 4 bytes), and
+ * m_scale, v_scale one byte e for every block: a code stands for its value times 2^(e - 127).  Codes are rounded up or down at
+ * random, by a hash of (seed, t, index, element).  `index`: which tensor of the optimizer this is.
+ * The global norm: tfc_grad_sumsq leaves tfc_grad_sumsq_partials() doubles (calls for several tables side by side in one
+ * buffer), tfc_adamw_step adds them up, writes the norm to `norm` (nullable) and limits the gradients; without max_norm the
+ * partials are not read.  lr_device (nullable): a device float that takes the place of lr, read when the step runs. */
+typedef struct tfc_adamw_tensor {
+    void* p;
+    const void* g;
+    void* m;
+    void* v;
+    uint8_t* m_scale;
+    uint8_t* v_scale;
+    int32_t* step;
+    int64_t n;
+    int32_t index;
+} tfc_adamw_tensor;
+
+typedef struct tfc_adamw_hyper {
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    const float* lr_device;
+    uint32_t seed;
+} tfc_adamw_hyper;
+
+int64_t tfc_grad_sumsq_partials(const tfc_adamw_tensor* tensors, int32_t n_tensors);
+int tfc_grad_sumsq(const tfc_adamw_tensor* tensors, int32_t n_tensors, int32_t dtype, double* partials, tfc_stream_t stream);
+int64_t tfc_adamw_workspace_bytes(int32_t n_tensors);
+int tfc_adamw_step(const tfc_adamw_tensor* tensors, int32_t n_tensors, int32_t dtype, int32_t state_bits,
+                   const tfc_adamw_hyper* hyper, const double* partials, int64_t n_partials, float* norm, void* workspace,
+                   int64_t workspace_bytes, tfc_stream_t stream);
+
 /* ------------------------------------------------------------------------------------------
  * Opt-in kernel timing (no counterpart in the reference, whose only timer is the epoch wall
  * clock, eigenn/model/utils.py:4-35).  While enabled, every main kernel launch is bracketed by

@@ -99,6 +99,15 @@ class GateSeg(C.Structure):
     ]
 
 
+class AdamwTensor(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "step")] + [("n", C.c_int64), ("index", C.c_int32)]
+
+
+class AdamwHyper(C.Structure):
+    _fields_ = [(n, C.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + [
+        ("lr_device", C.c_void_p), ("seed", C.c_uint32)]
+
+
 EPI_NONE, EPI_SSP, EPI_SSP_GRAD = 0, 1, 2
 F32, BF16, F16 = 0, 1, 2
 ACT = {"identity": 0, "ssp": 1, "silu": 2, "tanh": 3, "abs": 4, "sigmoid": 5}
@@ -177,6 +186,10 @@ SIGNATURES = {
     "tfc_layer_norm_fwd": (C.c_int, [_P, _P, _P, _I64, _I64, _F, _I32, _P, _P, _P, _P]),
     "tfc_layer_norm_bwd_workspace_floats": (_I64, [_I64, _I64, _I32]),
     "tfc_layer_norm_bwd": (C.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P]),
+    "tfc_grad_sumsq_partials": (_I64, [C.POINTER(AdamwTensor), _I32]),
+    "tfc_grad_sumsq": (C.c_int, [C.POINTER(AdamwTensor), _I32, _I32, _P, _P]),
+    "tfc_adamw_workspace_bytes": (_I64, [_I32]),
+    "tfc_adamw_step": (C.c_int, [C.POINTER(AdamwTensor), _I32, _I32, _I32, C.POINTER(AdamwHyper), _P, _I64, _P, _P, _I64, _P]),
     "tfc_gate_fwd_t": (C.c_int, [C.POINTER(GateSeg), _I32, _P, _I64, _I32, _I32, _P, C.POINTER(IrBlock), _I32, _P, _P]),
     "tfc_gate_bwd_t": (C.c_int, [C.POINTER(GateSeg), _I32, _P, _P, _I64, _I32, _I32, _P, C.POINTER(IrBlock), _I32, _P, _P]),
 }

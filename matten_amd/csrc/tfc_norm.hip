@@ -295,9 +295,10 @@ __global__ __launch_bounds__(256) void tfc_layer_norm_long_cols_kernel(const T* 
 }
 
 // 32 columns x 32 walkers; walker k adds the partial rows k, k + 32, ..., the walkers are joined in order.
+// Columns [0, na) go to `a`, the others to `b` (either null: not written).
 template <class T>
 __global__ __launch_bounds__(1024) void tfc_join_columns_kernel(const float* __restrict__ part, long n_part, long stride, long n,
-                                                                T* __restrict__ out) {
+                                                                long na, T* __restrict__ out_a, T* __restrict__ out_b) {
     __shared__ float lds[32][33];
     const int cl = threadIdx.x & 31, k = threadIdx.x >> 5;
     const long c = (long)blockIdx.x * 32 + cl;
@@ -317,15 +318,20 @@ __global__ __launch_bounds__(1024) void tfc_join_columns_kernel(const float* __r
         float t = 0.f;
 #pragma unroll
         for (int i = 0; i < 32; ++i) t += lds[i][cl];
-        out[c] = (T)t;
+        if (c < na) {
+            if (out_a) out_a[c] = (T)t;
+        } else if (out_b) {
+            out_b[c - na] = (T)t;
+        }
     }
 }
 
 template <class T>
-int join_columns(const float* part, int64_t n_part, int64_t stride, int64_t n, void* out, hipStream_t stream) {
+int join_columns(const float* part, int64_t n_part, int64_t na, void* out_a, int64_t nb, void* out_b, hipStream_t stream) {
     TfcProfScope prof("tfc_join_columns", stream);
+    const int64_t n = na + nb;
     hipLaunchKernelGGL(tfc_join_columns_kernel<T>, dim3((unsigned)((n + 31) / 32)), dim3(1024), 0, stream, part, (long)n_part,
-                       (long)stride, (long)n, (T*)out);
+                       (long)n, (long)n, (long)na, (T*)out_a, (T*)out_b);
     TFC_LAUNCH_CHECK("tfc_join_columns");
     return TFC_OK;
 }
@@ -449,8 +455,9 @@ int64_t partial_rows(int64_t rows, int64_t d, int dtype) {
 
 }  // namespace
 
-int tfc_join_columns(const float* part, int64_t n_part, int64_t stride, int64_t n, int dtype, void* out, hipStream_t stream) {
-    return TFC_BY_DTYPE(dtype, join_columns, part, n_part, stride, n, out, stream);
+int tfc_join_columns(const float* part, int64_t n_part, int64_t na, void* out_a, int64_t nb, void* out_b, int dtype,
+                     hipStream_t stream) {
+    return TFC_BY_DTYPE(dtype, join_columns, part, n_part, na, out_a, nb, out_b, stream);
 }
 
 extern "C" int tfc_layer_norm_fwd(const void* x, const void* w, const void* b, int64_t rows, int64_t d, float eps, int32_t dtype,
@@ -478,11 +485,7 @@ extern "C" int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, 
     TFC_REQUIRE(tfc_dtype_ok(dtype), TFC_EINVAL, "tfc_layer_norm_bwd: unknown dtype %d", (int)dtype);
     TFC_REQUIRE(rows >= 0 && d > 0, TFC_EINVAL, "tfc_layer_norm_bwd: bad sizes %lld x %lld", (long long)rows, (long long)d);
     hipStream_t s = (hipStream_t)stream;
-    if (rows == 0) {  // sums over no rows
-        if (dw && tfc_join_columns(nullptr, 0, 0, d, dtype, dw, s)) return TFC_ELAUNCH;
-        if (db && tfc_join_columns(nullptr, 0, 0, d, dtype, db, s)) return TFC_ELAUNCH;
-        return TFC_OK;
-    }
+    if (rows == 0) return dw || db ? tfc_join_columns(nullptr, 0, d, dw, d, db, dtype, s) : TFC_OK;  // sums over no rows
     TFC_REQUIRE(dy && x && mean && rstd, TFC_EINVAL, "tfc_layer_norm_bwd: null pointer");
     if (!dx && !dw && !db) return TFC_OK;
     NormArgs a{};
@@ -498,10 +501,5 @@ extern "C" int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, 
         const int rc = TFC_BY_DTYPE(dtype, layer_norm_bwd, a);
         if (rc) return rc;
     }
-    if (dw) {
-        const int rc = tfc_join_columns(workspace, a.n_part, 2 * d, d, dtype, dw, s);
-        if (rc) return rc;
-    }
-    if (db) return tfc_join_columns(workspace + d, a.n_part, 2 * d, d, dtype, db, s);
-    return TFC_OK;
+    return a.part ? tfc_join_columns(workspace, a.n_part, d, dw, d, db, dtype, s) : TFC_OK;
 }

@@ -71,5 +71,6 @@ __device__ __forceinline__ void tfc_store_f(T* p, long left, const float (&v)[N]
     }
 }
 
-// out[c] = sum over p of part[p * stride + c], in a fixed order (tfc_norm.hip): the join of per-workgroup column sums.
-int tfc_join_columns(const float* part, int64_t n_part, int64_t stride, int64_t n, int dtype, void* out, hipStream_t stream);
+// a[c] = sum over p of part[p][c] for c < na, b[c - na] for the nb columns behind them, in a fixed order (tfc_norm.hip): the join of
+// per-workgroup column sums.  a, b may be null.
+int tfc_join_columns(const float* part, int64_t n_part, int64_t na, void* a, int64_t nb, void* b, int dtype, hipStream_t stream);

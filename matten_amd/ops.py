@@ -8,6 +8,7 @@ SURVEY.md §3.3).  There is no CPU / eager fallback: tensors must live on a ROCm
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes as C
 import functools
 import math
@@ -1890,6 +1891,7 @@ def norm_activation(x, spec: GateSpec, eps_squared: float = 0.0, normalize: bool
 
 # ------------------------------------------------------------------ scalar head: layer norm
 
+_AS_IS = contextlib.nullcontext()
 _dtype_codes = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
 
 
@@ -1907,12 +1909,17 @@ def _floats(t: torch.Tensor, name: str, like: Optional[torch.Tensor] = None):
             raise RuntimeError(f"matten_amd: `{name}` is on {t.device}, the input on {like.device}")
 
 
+def _on(device: torch.device):
+    """The device a launch needs current (nothing to switch on almost every call)."""
+    return _AS_IS if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+
+
 def _layer_norm_run(x, w, b, eps: float, keep: bool):
     """(y, stats): rows of a contiguous [rows, d] tensor; `keep`: stats [2, rows] holds the mean and 1 / deviation of every row."""
     rows, d = x.shape
     y = torch.empty_like(x)
     stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         _lib.check(_lib.lib().tfc_layer_norm_fwd(_ptr(x), _ptr(w), _ptr(b), rows, d, eps, _dtype_codes[x.dtype], _ptr(y), _ptr(stats),
                                                  _ptr(stats, rows) if keep else None, _stream()))
     return y, stats
@@ -1939,7 +1946,7 @@ class _LayerNormFn(torch.autograd.Function):
         db = torch.empty_like(b) if need[2] else None
         L = _lib.lib()
         dt = _dtype_codes[x.dtype]
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             ws = None
             if need[1] or need[2]:
                 ws = torch.empty(int(L.tfc_layer_norm_bwd_workspace_floats(rows, d, dt)), dtype=torch.float32, device=x.device)

@@ -1,0 +1,233 @@
+"""AdamW over all parameter tensors of a model at once (tfc_adamw_step), with moments in 32 or in 8 bits and the gradients
+optionally limited to a largest global norm, in the same launches.
+
+A drop-in for the `class_path: torch.optim.Adam` / `AdamW` of the reference's configs (its trainer steps whatever optimizer the
+yaml names, eigenn/model/model.py:410-426): a `torch.optim.Optimizer` with param groups, schedulers, closures and
+`state_dict`.  Everything a step needs lives on the device - the step counts too - so that a step can be part of a captured
+graph (matten_amd.graphs.GraphedStep)."""
+from __future__ import annotations
+
+import ctypes as C
+import math
+from typing import Iterable, Optional
+
+import torch
+
+from . import _lib, ops
+
+__all__ = ["AdamW"]
+
+BLOCK = 256  # elements that share a scale in the 8-bit moments
+_STATE = {  # state entry -> dtype, by the width of the moments ("step" besides)
+    32: {"exp_avg": torch.float32, "exp_avg_sq": torch.float32},
+    8: {"exp_avg": torch.float8_e4m3fn, "exp_avg_scale": torch.float8_e8m0fnu, "exp_avg_sq_root": torch.float8_e4m3fn,
+        "exp_avg_sq_root_scale": torch.float8_e8m0fnu},
+}
+
+
+class _Table:
+    """The descriptors of the tensors one call steps: everything but the gradients' addresses is set once."""
+
+    def __init__(self, params, states, indexes, bits: int):
+        self.params = params
+        self.at = [p.data_ptr() for p in params]
+        self.keep = states
+        self.rows = (_lib.AdamwTensor * len(params))()
+        names = list(_STATE[bits])
+        for row, p, st, i in zip(self.rows, params, states, indexes):
+            row.p, row.n, row.index, row.step = p.data_ptr(), p.numel(), i, st["step"].data_ptr()
+            if bits == 32:
+                row.m, row.v = (st[k].data_ptr() for k in names)
+            else:
+                row.m, row.m_scale, row.v, row.v_scale = (st[k].data_ptr() for k in names)
+
+
+class AdamW(torch.optim.Optimizer):
+    """With g the gradient and t the tensor's step count:
+
+        m = beta1 m + (1 - beta1) g,    v = beta2 v + (1 - beta2) g^2,
+        p = (1 - lr weight_decay) p - lr / (1 - beta1^t) m / (sqrt(v) / sqrt(1 - beta2^t) + eps)
+
+    in fp32 for fp32, bf16 and fp16 parameters (a 16-bit parameter is rounded to the nearest once, at the end).
+
+    * `state_bits=32`: state entries `exp_avg`, `exp_avg_sq` (fp32).  `state_bits=8`: `exp_avg` and `exp_avg_sq_root` (the root
+      of the second moment) as float8_e4m3fn, flat and padded to whole blocks of 256, each block with a power-of-two scale
+      (`*_scale`, float8_e8m0fnu): a quarter of the state.  They are rounded up or down at random so that they are kept on
+      average; the random bits follow from `seed`, the step and the element, so runs repeat bit for bit.
+    * `max_grad_norm`: all gradients are scaled by min(1, max_grad_norm / (norm + 1e-6)) as they are read (`.grad` itself is
+      left alone).  After a step `grad_norm` holds the norm before scaling (a device scalar; None without `max_grad_norm`).
+      A norm that is not finite reaches the parameters: check `grad_norm` where that can happen.
+    * `lr` is a number or a 0-dim fp32 tensor on the parameters' device, read when the step runs: inside a captured graph a
+      number is fixed, a tensor can be written to between replays.
+
+    Parameters and gradients are contiguous and on a ROCm device (gradients that are not contiguous are copied); a sparse gradient
+    raises.  A parameter without a gradient is skipped and its step count stands.  The first step allocates the state and
+    therefore must not be inside a graph capture."""
+
+    def __init__(self, params: Iterable, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
+                 max_grad_norm: Optional[float] = None, seed: int = 0):
+        if state_bits not in _STATE:
+            raise ValueError(f"AdamW: state_bits must be 32 or 8, got {state_bits}")
+        if max_grad_norm is not None and not 0.0 < float(max_grad_norm) < math.inf:
+            raise ValueError(f"AdamW: max_grad_norm must be positive and finite, got {max_grad_norm}")
+        self.state_bits = int(state_bits)
+        self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
+        self.seed = int(seed) & 0xFFFFFFFF
+        self.grad_norm: Optional[torch.Tensor] = None
+        self._tables = {}
+        super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
+
+    def add_param_group(self, group):
+        super().add_param_group(group)
+        g = self.param_groups[-1]
+        try:
+            self._check_group(g)
+            for p in g["params"]:
+                if p.dtype not in ops._dtype_codes:
+                    raise TypeError(f"AdamW: parameters must be float32, bfloat16 or float16, got {p.dtype}")
+        except Exception:
+            self.param_groups.pop()
+            raise
+
+    @staticmethod
+    def _check_group(g):
+        lr, (b1, b2) = g["lr"], g["betas"]
+        if isinstance(lr, torch.Tensor):
+            if lr.numel() != 1 or lr.dtype != torch.float32:
+                raise ValueError("AdamW: an lr tensor must hold one float32")
+        elif not 0.0 <= lr < math.inf:
+            raise ValueError(f"AdamW: lr must be finite and not negative, got {lr}")
+        if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
+            raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
+        if not 0.0 <= g["eps"] < math.inf or not 0.0 <= g["weight_decay"] < math.inf:
+            raise ValueError(f"AdamW: eps and weight_decay must be finite and not negative, got {g['eps']}, {g['weight_decay']}")
+
+    # ---- state
+    def _new_state(self, p) -> dict:
+        blocks = -(-p.numel() // BLOCK)
+        st = {"step": torch.zeros((), dtype=torch.int32, device=p.device)}
+        for k, dt in _STATE[self.state_bits].items():
+            if self.state_bits == 32:
+                st[k] = torch.zeros_like(p, dtype=dt, memory_format=torch.contiguous_format)
+            else:  # (a scale's exponent is 1 where all its values are zero)
+                n, fill = (blocks, 1) if k.endswith("scale") else (blocks * BLOCK, 0)
+                st[k] = torch.full((n,), fill, dtype=torch.uint8, device=p.device).view(dt)
+        return st
+
+    def load_state_dict(self, state_dict):
+        """Takes copies.  The moments must have this optimizer's width and the parameters' sizes."""
+        names = _STATE[self.state_bits]
+        ids = [i for g in state_dict["param_groups"] for i in g["params"]]
+        params = [p for g in self.param_groups for p in g["params"]]
+        new = {}
+        for i, p in zip(ids, params):
+            saved = state_dict["state"].get(i)
+            if not saved:
+                continue
+            if set(saved) != {"step", *names}:
+                raise ValueError(f"AdamW: state entries {sorted(saved)} are not those of moments in {self.state_bits} bits")
+            st = self._new_state(p)
+            for k, v in saved.items():
+                if k == "step":
+                    st[k].fill_(int(v))
+                    continue
+                if v.numel() != st[k].numel() or v.dtype != st[k].dtype:
+                    raise ValueError(f"AdamW: `{k}` has {v.numel()} x {v.dtype}, expected {st[k].numel()} x {st[k].dtype}")
+                wide = torch.uint8 if self.state_bits == 8 else v.dtype
+                st[k].view(wide).copy_(v.detach().view(wide).reshape(st[k].shape))
+            new[p] = st
+        super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})  # (would cast the moments)
+        self.state.update(new)
+        self._tables = {}
+
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        self._tables = {}
+
+    def __getstate__(self):
+        return {**super().__getstate__(), "state_bits": self.state_bits, "max_grad_norm": self.max_grad_norm, "seed": self.seed,
+                "grad_norm": None}
+
+    # ---- step
+    def _gather(self):
+        """[(group, table, dtype)] of the parameters that have a gradient, one entry for each (group, device, dtype)."""
+        calls, index = [], 0
+        for gi, g in enumerate(self.param_groups):
+            sets = {}
+            for p in g["params"]:
+                if p.grad is not None:
+                    sets.setdefault((p.device, p.dtype), []).append((p, index))
+                index += 1
+            self._check_group(g)  # (schedulers and users write to groups)
+            for (device, dtype), items in sets.items():
+                if isinstance(g["lr"], torch.Tensor) and g["lr"].device != device:
+                    raise RuntimeError(f"AdamW: the lr tensor is on {g['lr'].device}, the parameters on {device}")
+                calls.append((g, device, dtype, self._table(gi, device, dtype, items)))
+        return calls
+
+    def _table(self, gi, device, dtype, items) -> _Table:
+        key = (gi, device, dtype)
+        table = self._tables.get(key)
+        if (table is None or len(table.params) != len(items)
+                or any(p is not q or p.data_ptr() != a for (p, _), q, a in zip(items, table.params, table.at))
+                or any(self.state[p] is not st for (p, _), st in zip(items, table.keep))):
+            if device.type != "cuda":
+                raise RuntimeError(f"matten_amd: parameters must live on a ROCm device (no CPU fallback exists); got {device}")
+            for p, _ in items:
+                if not p.is_contiguous():
+                    raise ValueError("AdamW: parameters must be contiguous")
+                if not self.state[p]:
+                    if torch.cuda.is_current_stream_capturing():
+                        raise RuntimeError("AdamW: the first step allocates the state and cannot be captured; run one step before the capture")
+                    self.state[p].update(self._new_state(p))
+            table = _Table([p for p, _ in items], [self.state[p] for p, _ in items], [i for _, i in items], self.state_bits)
+            self._tables[key] = table
+        return table
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        calls = self._gather()
+        copies = []  # gradients that are not contiguous
+        for _, device, dtype, table in calls:
+            for row, p in zip(table.rows, table.params):
+                g = p.grad
+                if g.dtype != dtype or g.device != device or g.layout != torch.strided or g.shape != p.shape:
+                    raise RuntimeError(f"AdamW: a gradient must be a dense {dtype} tensor of shape {tuple(p.shape)} on {device}; got "
+                                       f"{g.dtype}, {tuple(g.shape)}, {g.layout} on {g.device}")
+                if not g.is_contiguous():
+                    g = g.contiguous()
+                    copies.append(g)
+                row.g = g.data_ptr()
+        L = _lib.lib()
+        partials, n_partials = None, 0
+        self.grad_norm = None
+        if self.max_grad_norm is not None and calls:
+            device = calls[0][1]
+            if any(c[1] != device for c in calls):
+                raise RuntimeError("AdamW: max_grad_norm needs all parameters on one device")
+            counts = [int(L.tfc_grad_sumsq_partials(t.rows, len(t.rows))) for _, _, _, t in calls]
+            n_partials = sum(counts)
+            with ops._on(device):
+                partials = torch.empty(max(n_partials, 1), dtype=torch.float64, device=device)
+                self.grad_norm = torch.empty((), dtype=torch.float32, device=device) if n_partials else torch.zeros((), device=device)
+                at = 0
+                for (_, _, dtype, t), n in zip(calls, counts):
+                    _lib.check(L.tfc_grad_sumsq(t.rows, len(t.rows), ops._dtype_codes[dtype], ops._ptr(partials, at), ops._stream()))
+                    at += n
+        for g, device, dtype, t in calls:
+            h = _lib.AdamwHyper(beta1=g["betas"][0], beta2=g["betas"][1], eps=g["eps"], weight_decay=g["weight_decay"],
+                                max_norm=self.max_grad_norm if n_partials else 0.0, seed=self.seed)
+            if isinstance(g["lr"], torch.Tensor):
+                h.lr_device = g["lr"].data_ptr()
+            else:
+                h.lr = g["lr"]
+            with ops._on(device):
+                ws = torch.empty(int(L.tfc_adamw_workspace_bytes(len(t.rows))), dtype=torch.uint8, device=device)
+                _lib.check(L.tfc_adamw_step(t.rows, len(t.rows), ops._dtype_codes[dtype], self.state_bits, C.byref(h), ops._ptr(partials),
+                                            n_partials, ops._ptr(self.grad_norm), ops._ptr(ws), ws.numel(), ops._stream()))
+            torch.autograd.graph.increment_version(t.params)  # (written behind torch's back: saved tensors and caches see it)
+        return loss
