@@ -580,6 +580,39 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
                        int64_t d, int32_t dtype, void* dx, void* dw, void* db, float* workspace, int64_t workspace_floats,
                        tfc_stream_t stream);
 
+/* Matrix product with its epilogue: c[m, n] = act_cst act(alpha a b + bias) + residual, one dtype throughout, sums in fp32
+ * (fp32 operands as three bf16 pieces each, exactly; an operand that is not finite gives NaN).  The reference's scalar layers
+ * are torch.nn.Linear + activation (eigenn/nn/utils.py); its radial network with a `mlp_activation` other than ssp
+ * (eigenn/nn/utils.py:182,247-252) is a chain of these.
+ *   a [m, k]: a_along_k: element (i, kk) at i lda + kk, else at kk lda + i;
+ *   b [k, n]: b_along_k: element (kk, j) at j ldb + kk, else at kk ldb + j.  (a along its rows with b along k: not built.)
+ *   c: row stride ldc; residual (nullable) [m, n] with row stride ldr; bias (nullable) [n]; z (nullable) [m, n] packed: receives
+ *   alpha a b + bias.  Workspace: tfc_dense_workspace_floats() (0: none).  k = 0: the epilogue of zeros.
+ * tfc_dense_dz: dz = act_cst act'(z) dy (nullable) and db = its column sums (nullable; they need the workspace), all [rows, n]
+ * packed; act identity: z is not read.  The backward pass is that and two more products. */
+#define TFC_ACT_GELU 6 /* x Phi(x) with the normal distribution function Phi (tfc_dense only) */
+typedef struct tfc_dense_desc {
+    int64_t m, n, k;
+    const void* a;
+    int64_t lda;
+    const void* b;
+    int64_t ldb;
+    void* c;
+    int64_t ldc;
+    const void* bias;
+    const void* residual;
+    int64_t ldr;
+    void* z;
+    float alpha, act_cst;
+    int32_t act, dtype, a_along_k, b_along_k;
+} tfc_dense_desc;
+
+int64_t tfc_dense_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype);
+int tfc_dense(const tfc_dense_desc* desc, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
+int64_t tfc_dense_dz_workspace_floats(int64_t rows, int64_t n, int32_t dtype);
+int tfc_dense_dz(const void* dy, const void* z, int64_t rows, int64_t n, int32_t dtype, int32_t act, float act_cst, void* dz,
+                 void* db, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
+
 /* One AdamW step over many parameter tensors of one dtype (the reference's trainer steps torch.optim one tensor at a time,
  * eigenn/model/model.py:410-426).  With g the gradient, scaled by min(1, max_norm / (norm + 1e-6)) when max_norm > 0, and
  * t = ++*step of the tensor:

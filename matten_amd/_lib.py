@@ -99,6 +99,30 @@ class GateSeg(C.Structure):
     ]
 
 
+class DenseDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int64),
+        ("n", C.c_int64),
+        ("k", C.c_int64),
+        ("a", C.c_void_p),
+        ("lda", C.c_int64),
+        ("b", C.c_void_p),
+        ("ldb", C.c_int64),
+        ("c", C.c_void_p),
+        ("ldc", C.c_int64),
+        ("bias", C.c_void_p),
+        ("residual", C.c_void_p),
+        ("ldr", C.c_int64),
+        ("z", C.c_void_p),
+        ("alpha", C.c_float),
+        ("act_cst", C.c_float),
+        ("act", C.c_int32),
+        ("dtype", C.c_int32),
+        ("a_along_k", C.c_int32),
+        ("b_along_k", C.c_int32),
+    ]
+
+
 class AdamwTensor(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "step")] + [("n", C.c_int64), ("index", C.c_int32)]
 
@@ -111,6 +135,8 @@ class AdamwHyper(C.Structure):
 EPI_NONE, EPI_SSP, EPI_SSP_GRAD = 0, 1, 2
 F32, BF16, F16 = 0, 1, 2
 ACT = {"identity": 0, "ssp": 1, "silu": 2, "tanh": 3, "abs": 4, "sigmoid": 5}
+
+DENSE_ACT = {**ACT, "gelu": 6}
 
 _P = C.c_void_p
 _I64 = C.c_int64
@@ -186,6 +212,10 @@ SIGNATURES = {
     "tfc_layer_norm_fwd": (C.c_int, [_P, _P, _P, _I64, _I64, _F, _I32, _P, _P, _P, _P]),
     "tfc_layer_norm_bwd_workspace_floats": (_I64, [_I64, _I64, _I32]),
     "tfc_layer_norm_bwd": (C.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P]),
+    "tfc_dense_workspace_floats": (_I64, [_I64, _I64, _I64, _I32]),
+    "tfc_dense": (C.c_int, [C.POINTER(DenseDesc), _P, _I64, _P]),
+    "tfc_dense_dz_workspace_floats": (_I64, [_I64, _I64, _I32]),
+    "tfc_dense_dz": (C.c_int, [_P, _P, _I64, _I64, _I32, _I32, _F, _P, _P, _P, _I64, _P]),
     "tfc_grad_sumsq_partials": (_I64, [C.POINTER(AdamwTensor), _I32]),
     "tfc_grad_sumsq": (C.c_int, [C.POINTER(AdamwTensor), _I32, _I32, _P, _P]),
     "tfc_adamw_workspace_bytes": (_I64, [_I32]),

@@ -1,0 +1,528 @@
+// Matrix product with its epilogue: C = c act(alpha A B + bias) + residual, for fp32, bf16 and fp16, and the elementwise half of
+// its backward pass (dz = c act'(z) dy with the column sums that are the bias's gradient).  The products of the backward
+// pass are the same kernel without the epilogue: dA = dz B^T, dB = A^T dz.
+//
+// A tile of C belongs to a workgroup of four waves.  Operand tiles go through registers into LDS as rows of 16-bit elements with
+// the contraction index contiguous (row stride padded by 16 bytes: consecutive rows start 16-byte units of different banks), so a
+// lane reads its eight k of a matrix instruction in one access; an operand whose memory runs along the rows instead is
+// transposed on the way, in registers.  The loads of the next step are in flight while this one is multiplied.
+// bf16 and fp16 feed v_mfma_f32_32x32x16 directly.  fp32 is cut into three bf16 pieces, x = h + m + l exactly (8 + 8 + 8
+// significant bits), and the product is the six largest of the nine piece products, the dropped ones below 2^-24 |a b|: 2.67
+// times the rate of the fp32 matrix instruction and no less exact (an infinity has no pieces: it gives NaN).
+// The instruction's rows are the columns of C, so that a lane ends up with four neighbouring columns of a row.
+//
+// Few tiles and a long contraction (a weight's gradient over many rows): the contraction is split, partial tiles go to the
+// workspace and a second kernel adds them in order and applies the epilogue.
+#include "tfc_types.h"
+
+#include <algorithm>
+#include <type_traits>
+
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+
+// ------------------------------------------------------------------------------------------------ activations
+__device__ __forceinline__ float act_eval(int act, float x) {
+    switch (act) {
+        case TFC_ACT_SSP: return (x > 20.f ? x : log1pf(expf(x))) - 0.69314718055994530942f;
+        case TFC_ACT_SILU: return x / (1.f + expf(-x));
+        case TFC_ACT_TANH: return tanhf(x);
+        case TFC_ACT_ABS: return fabsf(x);
+        case TFC_ACT_SIGMOID: return 1.f / (1.f + expf(-x));
+        case TFC_ACT_GELU: return 0.5f * x * erfcf(-0.70710678118654752440f * x);
+        default: return x;
+    }
+}
+
+__device__ __forceinline__ float act_grad(int act, float x) {
+    switch (act) {
+        case TFC_ACT_SSP: return 1.f / (1.f + expf(-x));
+        case TFC_ACT_SILU: {
+            const float s = 1.f / (1.f + expf(-x));
+            return s * (1.f + x * (1.f - s));
+        }
+        case TFC_ACT_TANH: {
+            const float t = tanhf(x);
+            return 1.f - t * t;
+        }
+        case TFC_ACT_ABS: return x > 0.f ? 1.f : (x < 0.f ? -1.f : 0.f);
+        case TFC_ACT_SIGMOID: {
+            const float s = 1.f / (1.f + expf(-x));
+            return s * (1.f - s);
+        }
+        case TFC_ACT_GELU:
+            return 0.5f * erfcf(-0.70710678118654752440f * x) + x * 0.39894228040143267794f * expf(-0.5f * x * x);
+        default: return 1.f;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ operands
+struct Operand {
+    const void* p;
+    long ld;  // elements between rows (k contiguous) / between k (rows contiguous)
+};
+
+template <class T>
+struct Pieces {
+    static constexpr int N = std::is_same<T, float>::value ? 3 : 1;
+    static constexpr int K = std::is_same<T, float>::value ? 32 : 64;  // contraction length of a step
+};
+
+// Eight consecutive k of one row, as fragments of the matrix instruction.
+struct Unit3 {
+    uintx4 h, m, l;
+};
+__device__ __forceinline__ Unit3 split8(const float (&x)[8]) {
+    Unit3 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned u0 = __float_as_uint(x[2 * i]), u1 = __float_as_uint(x[2 * i + 1]);
+        r.h[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // upper halves: cut, not rounded, so that nothing overflows
+        const float a0 = x[2 * i] - __uint_as_float(u0 & 0xffff0000u), a1 = x[2 * i + 1] - __uint_as_float(u1 & 0xffff0000u);
+        const bf16x2 mm = {(__bf16)a0, (__bf16)a1};
+        const unsigned mu = __builtin_bit_cast(unsigned, mm);
+        r.m[i] = mu;
+        const bf16x2 ll = {(__bf16)(a0 - __uint_as_float(mu << 16)), (__bf16)(a1 - __uint_as_float(mu & 0xffff0000u))};
+        r.l[i] = __builtin_bit_cast(unsigned, ll);
+    }
+    return r;
+}
+
+// What a thread has in flight of an operand tile of R rows: UNITS units of eight k.  Along k: unit u is row u / (K/8), eight k
+// from memory.  Along rows: a thread takes RV neighbouring rows x eight k, eight accesses of RV elements.
+template <class T, int R, bool ALONG_K>
+struct Stage {
+    static constexpr int K = Pieces<T>::K, UNITS = R * K / 8 / 256, KU = K / 8, LD = K + 8;
+    static constexpr int RV = UNITS;  // (rows of a thread when the memory runs along them)
+    T v[UNITS][8];
+
+    __device__ __forceinline__ void load(const Operand& o, long r0, long rows, long k0, long kend) {
+        const T* p = (const T*)o.p;
+        const int t = threadIdx.x;
+        if constexpr (ALONG_K) {
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const int u = t + 256 * i;
+                const long r = r0 + u / KU, k = k0 + (u % KU) * 8, left = r < rows ? kend - k : 0;
+                const T* q = p + r * o.ld + k;
+                if (left >= 8) {
+                    const TfcPack<T, 8> w = tfc_load<T, 8>(q);
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i][j] = w.e[j];
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) v[i][j] = j < left ? q[j] : (T)0.f;
+                }
+            }
+        } else {
+            constexpr int TR = R / RV;  // threads along the rows
+            const long r = r0 + (t % TR) * RV, k = k0 + (t / TR) * 8;
+            const long left = rows - r;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const T* q = p + (k + j) * o.ld + r;
+                if (k + j < kend && left >= RV) {
+                    const TfcPack<T, RV> w = tfc_load<T, RV>(q);
+#pragma unroll
+                    for (int i = 0; i < RV; ++i) v[i][j] = w.e[i];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < RV; ++i) v[i][j] = k + j < kend && i < left ? q[i] : (T)0.f;
+                }
+            }
+        }
+    }
+
+    __device__ __forceinline__ void store(uint16_t* lds) const {  // planes of [R][LD]
+        const int t = threadIdx.x;
+#pragma unroll
+        for (int i = 0; i < UNITS; ++i) {
+            int r, ku;
+            if constexpr (ALONG_K) {
+                r = (t + 256 * i) / KU, ku = (t + 256 * i) % KU;
+            } else {
+                constexpr int TR = R / RV;
+                r = (t % TR) * RV + i, ku = t / TR;
+            }
+            uint16_t* q = lds + r * LD + ku * 8;
+            if constexpr (std::is_same<T, float>::value) {
+                const Unit3 s = split8(v[i]);
+                *(uintx4*)q = s.h;
+                *(uintx4*)(q + R * LD) = s.m;
+                *(uintx4*)(q + 2 * R * LD) = s.l;
+            } else {
+                uintx4 w;
+                __builtin_memcpy(&w, v[i], 16);
+                *(uintx4*)q = w;
+            }
+        }
+    }
+};
+
+__device__ __forceinline__ floatx16 mma(tfc_bf16, uintx4 a, uintx4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mma(tfc_f16, uintx4 a, uintx4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+// ------------------------------------------------------------------------------------------------ the product
+struct Args {
+    Operand a, b;
+    long m, n, k;
+    void* c;
+    long ldc;
+    const void *bias, *res;
+    long ldr;
+    void* z;  // [m, n] packed: alpha A B + bias, for the backward pass
+    float alpha, cst;
+    int act;
+    float* part;  // split contraction: [split][m][n]
+    long k_split;
+    int tiles_m, tiles_n;
+};
+
+// Four neighbouring columns of one row of C.
+template <class T>
+__device__ __forceinline__ void epilogue4(const Args& g, long row, long col, float (&v)[4]) {
+    const long left = g.n - col;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= g.alpha;
+    if (g.bias) {
+        float b[4];
+        tfc_load_f<T, 4>((const T*)g.bias + col, left, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += b[j];
+    }
+    if (g.z) tfc_store_f<T, 4>((T*)g.z + row * g.n + col, left, v);
+    if (g.act != TFC_ACT_IDENTITY) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] = act_eval(g.act, v[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] *= g.cst;
+    if (g.res) {
+        float r[4];
+        tfc_load_f<T, 4>((const T*)g.res + row * g.ldr + col, left, r);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) v[j] += r[j];
+    }
+    tfc_store_f<T, 4>((T*)g.c + row * g.ldc + col, left, v);
+}
+
+// BM x BN tile, waves 2 x 2.  SPLIT: this workgroup's part of the contraction to g.part.
+template <class T, bool AK, bool BK, int BM, int BN, bool SPLIT>
+__global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
+    constexpr int P = Pieces<T>::N, K = Pieces<T>::K, LD = K + 8;
+    constexpr int MI = BM / 64, NI = BN / 64;  // 32 x 32 tiles of a wave
+    __shared__ __attribute__((aligned(16))) uint16_t lds[P * (BM + BN) * LD];
+    uint16_t* la = lds;
+    uint16_t* lb = lds + P * BM * LD;
+    const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x);
+    const long m0 = (long)(tile / g.tiles_n) * BM, n0 = (long)(tile % g.tiles_n) * BN;
+    const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
+    const long k1 = SPLIT ? (k0 + g.k_split < g.k ? k0 + g.k_split : g.k) : g.k;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wm = (wave >> 1) * 32 * MI, wn = (wave & 1) * 32 * NI;
+    const int fr = lane & 31, fk = (lane >> 5) * 8;
+    floatx16 acc[MI][NI], low[P == 3 ? MI : 1][P == 3 ? NI : 1];
+#pragma unroll
+    for (int i = 0; i < MI; ++i)
+#pragma unroll
+        for (int j = 0; j < NI; ++j) {
+            acc[i][j] = floatx16(0.f);
+            if constexpr (P == 3) low[i][j] = floatx16(0.f);
+        }
+    Stage<T, BM, AK> sa;
+    Stage<T, BN, BK> sb;
+    sa.load(g.a, m0, g.m, k0, k1);
+    sb.load(g.b, n0, g.n, k0, k1);
+    for (long k = k0; k < k1; k += K) {
+        __syncthreads();  // the step before has been read
+        sa.store(la);
+        sb.store(lb);
+        __syncthreads();
+        if (k + K < k1) {
+            sa.load(g.a, m0, g.m, k + K, k1);
+            sb.load(g.b, n0, g.n, k + K, k1);
+        }
+#pragma unroll
+        for (int kk = 0; kk < K; kk += 16) {
+            uintx4 fa[MI][P], fb[NI][P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+#pragma unroll
+                for (int i = 0; i < MI; ++i) fa[i][p] = *(const uintx4*)(la + (p * BM + wm + 32 * i + fr) * LD + kk + fk);
+#pragma unroll
+                for (int j = 0; j < NI; ++j) fb[j][p] = *(const uintx4*)(lb + (p * BN + wn + 32 * j + fr) * LD + kk + fk);
+            }
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) {
+                    if constexpr (P == 3) {  // the small terms in an accumulator of their own
+                        low[i][j] = mma(tfc_bf16(), fb[j][0], fa[i][2], low[i][j]);
+                        low[i][j] = mma(tfc_bf16(), fb[j][2], fa[i][0], low[i][j]);
+                        low[i][j] = mma(tfc_bf16(), fb[j][1], fa[i][1], low[i][j]);
+                        low[i][j] = mma(tfc_bf16(), fb[j][0], fa[i][1], low[i][j]);
+                        low[i][j] = mma(tfc_bf16(), fb[j][1], fa[i][0], low[i][j]);
+                        acc[i][j] = mma(tfc_bf16(), fb[j][0], fa[i][0], acc[i][j]);
+                    } else {
+                        acc[i][j] = mma(T(), fb[j][0], fa[i][0], acc[i][j]);
+                    }
+                }
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        const long row = m0 + wm + 32 * i + fr;
+        if (row >= g.m) continue;
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const long col = n0 + wn + 32 * j + 8 * q + (lane >> 5) * 4;
+                if (col >= g.n) continue;
+                float v[4];
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    v[e] = acc[i][j][4 * q + e];
+                    if constexpr (P == 3) v[e] += low[i][j][4 * q + e];
+                }
+                if constexpr (SPLIT)
+                    tfc_store_f<float, 4>(g.part + ((long)blockIdx.y * g.m + row) * g.n + col, g.n - col, v);
+                else
+                    epilogue4<T>(g, row, col, v);
+            }
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(256) void tfc_dense_join_kernel(const Args g, int splits) {
+    const long nv = (g.n + 3) / 4, total = g.m * nv, slab = g.m * g.n;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long row = i / nv, col = (i - row * nv) * 4;
+        const float* p = g.part + row * g.n + col;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int s = 0; s < splits; ++s) {
+            float w[4];
+            tfc_load_f<float, 4>(p + s * slab, g.n - col, w);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += w[j];
+        }
+        epilogue4<T>(g, row, col, v);
+    }
+}
+
+// An empty contraction: the epilogue of zeros.
+template <class T>
+__global__ __launch_bounds__(256) void tfc_dense_empty_kernel(const Args g) {
+    const long nv = (g.n + 3) / 4, total = g.m * nv;
+    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
+        const long row = i / nv, col = (i - row * nv) * 4;
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        epilogue4<T>(g, row, col, v);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ backward, elementwise
+// dz = cst act'(z) dy and the column sums of dz: a workgroup walks a slab of rows, cw threads side by side on a chunk of
+// columns, 256 / cw rows at a time; its sums go to one partial row.  z null: act is the identity.
+template <class T>
+__global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, long rows, long n,
+                                                           int act, float cst, int cw, long slab, T* __restrict__ dz,
+                                                           float* __restrict__ part) {
+    constexpr int V = TfcType<T>::V;
+    const int cl = threadIdx.x % cw, rl = threadIdx.x / cw, step = 256 / cw;
+    const long c = ((long)blockIdx.x * cw + cl) * V, left = n - c;
+    const long r0 = (long)blockIdx.y * slab, r1 = r0 + slab < rows ? r0 + slab : rows;
+    float sum[V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) sum[j] = 0.f;
+    if (left > 0) {
+        for (long r = r0 + rl; r < r1; r += step) {
+            float g[V], x[V];
+            tfc_load_f<T, V>(dy + r * n + c, left, g);
+            if (z) {
+                tfc_load_f<T, V>(z + r * n + c, left, x);
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[j] *= act_grad(act, x[j]);
+            }
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                g[j] *= cst;
+                sum[j] += j < left ? g[j] : 0.f;
+            }
+            if (dz) tfc_store_f<T, V>(dz + r * n + c, left, g);
+        }
+    }
+    if (!part) return;
+    __shared__ float lds[256 * V];
+#pragma unroll
+    for (int j = 0; j < V; ++j) lds[(rl * V + j) * cw + cl] = sum[j];
+    __syncthreads();
+    if (rl == 0 && left > 0) {
+        for (int k = 1; k < step; ++k)
+#pragma unroll
+            for (int j = 0; j < V; ++j) sum[j] += lds[(k * V + j) * cw + cl];
+        tfc_store_f<float, V>(part + (long)blockIdx.y * n + c, left, sum);
+    }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+struct Plan {
+    int bm, bn;
+    int64_t tiles_m, tiles_n, splits, k_split;
+};
+
+// Tiles: 128 x 128 where they fill the chip, else smaller ones (twice as many operand bytes through LDS for each product).  The
+// contraction is split until there are two workgroups for every CU, in parts of at least four steps.
+Plan plan(int64_t m, int64_t n, int64_t k, int dtype) {
+    Plan p{};
+    auto tiles = [&](int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
+    p.bm = p.bn = 64;
+    if (n > 64 && m > 64 && tiles(128, 128) >= 256)
+        p.bm = p.bn = 128;
+    else if (m > 64 && tiles(128, 64) >= 256)
+        p.bm = 128;
+    p.tiles_m = (m + p.bm - 1) / p.bm;
+    p.tiles_n = (n + p.bn - 1) / p.bn;
+    const int64_t step = dtype == TFC_F32 ? 32 : 64, steps = (k + step - 1) / step, have = p.tiles_m * p.tiles_n;
+    p.splits = 1;
+    if (have < 256) p.splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / have, steps / 4), 1024));
+    const int64_t each = (steps + p.splits - 1) / p.splits;
+    p.k_split = each * step;
+    p.splits = (steps + each - 1) / each;
+    return p;
+}
+
+template <class T, bool AK, bool BK, int BM, int BN>
+int launch_tile(const Args& g, const Plan& p, hipStream_t s) {
+    const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
+    if (p.splits > 1)
+        hipLaunchKernelGGL((tfc_dense_kernel<T, AK, BK, BM, BN, true>), grid, dim3(256), 0, s, g);
+    else
+        hipLaunchKernelGGL((tfc_dense_kernel<T, AK, BK, BM, BN, false>), grid, dim3(256), 0, s, g);
+    TFC_LAUNCH_CHECK("tfc_dense");
+    return TFC_OK;
+}
+
+template <class T, bool AK, bool BK>
+int launch_layout(const Args& g, const Plan& p, hipStream_t s) {
+    if (p.bn == 128) return launch_tile<T, AK, BK, 128, 128>(g, p, s);
+    if (p.bm == 128) return launch_tile<T, AK, BK, 128, 64>(g, p, s);
+    return launch_tile<T, AK, BK, 64, 64>(g, p, s);
+}
+
+template <class T>
+int dense(Args g, const Plan& p, bool a_k, bool b_k, hipStream_t s) {
+    const long quads = g.m * ((g.n + 3) / 4);
+    const unsigned flat = (unsigned)std::min<long>((quads + 255) / 256, 8192);
+    if (g.k == 0) {
+        hipLaunchKernelGGL(tfc_dense_empty_kernel<T>, dim3(flat), dim3(256), 0, s, g);
+        TFC_LAUNCH_CHECK("tfc_dense_empty");
+        return TFC_OK;
+    }
+    g.tiles_m = (int)p.tiles_m, g.tiles_n = (int)p.tiles_n, g.k_split = p.k_split;
+    const int rc = !a_k ? launch_layout<T, false, false>(g, p, s)
+                   : b_k ? launch_layout<T, true, true>(g, p, s)
+                         : launch_layout<T, true, false>(g, p, s);
+    if (rc || p.splits == 1) return rc;
+    hipLaunchKernelGGL(tfc_dense_join_kernel<T>, dim3(flat), dim3(256), 0, s, g, (int)p.splits);
+    TFC_LAUNCH_CHECK("tfc_dense_join");
+    return TFC_OK;
+}
+
+struct DzPlan {
+    int cw;
+    int64_t chunks, slab, slabs;
+};
+DzPlan dz_plan(int64_t rows, int64_t n, int dtype) {
+    DzPlan p{};
+    const int64_t v = dtype == TFC_F32 ? 4 : 8, nv = (n + v - 1) / v;
+    p.cw = 1;
+    while (p.cw < nv && p.cw < 256) p.cw *= 2;
+    p.chunks = (nv + p.cw - 1) / p.cw;
+    const int64_t step = 256 / p.cw;
+    const int64_t want = std::max<int64_t>(1, 2048 / p.chunks);  // slabs that fill the chip
+    p.slab = std::max<int64_t>(4 * step, (rows + want - 1) / want);
+    p.slabs = (rows + p.slab - 1) / p.slab;
+    return p;
+}
+
+template <class T>
+int dense_dz(const DzPlan& p, const void* dy, const void* z, int64_t rows, int64_t n, int act, float cst, void* dz, float* part,
+             hipStream_t s) {
+    hipLaunchKernelGGL(tfc_dense_dz_kernel<T>, dim3((unsigned)p.chunks, (unsigned)p.slabs), dim3(256), 0, s, (const T*)dy, (const T*)z,
+                       (long)rows, (long)n, act, cst, p.cw, (long)p.slab, (T*)dz, part);
+    TFC_LAUNCH_CHECK("tfc_dense_dz");
+    return TFC_OK;
+}
+
+bool act_ok(int act) {
+    return act == TFC_ACT_IDENTITY || act == TFC_ACT_SSP || act == TFC_ACT_SILU || act == TFC_ACT_TANH || act == TFC_ACT_ABS ||
+           act == TFC_ACT_SIGMOID || act == TFC_ACT_GELU;
+}
+
+}  // namespace
+
+extern "C" int64_t tfc_dense_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype) {
+    if (m <= 0 || n <= 0 || k <= 0 || !tfc_dtype_ok(dtype)) return 0;
+    const Plan p = plan(m, n, k, dtype);
+    return p.splits > 1 ? p.splits * m * n : 0;
+}
+
+extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
+    TFC_REQUIRE(d, TFC_EINVAL, "tfc_dense: null descriptor");
+    TFC_REQUIRE(tfc_dtype_ok(d->dtype), TFC_EINVAL, "tfc_dense: unknown dtype %d", (int)d->dtype);
+    TFC_REQUIRE(act_ok(d->act), TFC_EINVAL, "tfc_dense: unknown activation %d", (int)d->act);
+    TFC_REQUIRE(d->m >= 0 && d->n >= 0 && d->k >= 0, TFC_EINVAL, "tfc_dense: negative size");
+    if (d->m == 0 || d->n == 0) return TFC_OK;
+    TFC_REQUIRE(d->c && (d->k == 0 || (d->a && d->b)), TFC_EINVAL, "tfc_dense: null pointer");
+    TFC_REQUIRE(d->a_along_k || !d->b_along_k, TFC_EUNSUPPORTED,
+                "tfc_dense: an A that runs along its rows needs a B that runs along its columns");
+    TFC_REQUIRE(d->lda >= 0 && d->ldb >= 0 && d->ldc >= d->n && (!d->residual || d->ldr >= 0), TFC_EINVAL, "tfc_dense: bad stride");
+    const Plan p = d->k ? plan(d->m, d->n, d->k, d->dtype) : Plan{64, 64, 1, 1, 1, 0};
+    TFC_REQUIRE(p.tiles_m * p.tiles_n < (int64_t)1 << 31, TFC_EUNSUPPORTED, "tfc_dense: %lld x %lld has too many tiles",
+                (long long)d->m, (long long)d->n);
+    TFC_REQUIRE(p.splits == 1 || (workspace && workspace_floats >= p.splits * d->m * d->n), TFC_EINVAL,
+                "tfc_dense: workspace too small");
+    hipStream_t s = (hipStream_t)stream;
+    TfcProfScope prof("tfc_dense", s);
+    Args g{};
+    g.a = {d->a, (long)d->lda}, g.b = {d->b, (long)d->ldb};
+    g.m = d->m, g.n = d->n, g.k = d->k;
+    g.c = d->c, g.ldc = d->ldc, g.bias = d->bias, g.res = d->residual, g.ldr = d->ldr, g.z = d->z;
+    g.alpha = d->alpha, g.cst = d->act_cst, g.act = d->act, g.part = workspace;
+    return TFC_BY_DTYPE(d->dtype, dense, g, p, d->a_along_k != 0, d->b_along_k != 0, s);
+}
+
+extern "C" int64_t tfc_dense_dz_workspace_floats(int64_t rows, int64_t n, int32_t dtype) {
+    if (rows <= 0 || n <= 0 || !tfc_dtype_ok(dtype)) return 0;
+    return dz_plan(rows, n, dtype).slabs * n;
+}
+
+extern "C" int tfc_dense_dz(const void* dy, const void* z, int64_t rows, int64_t n, int32_t dtype, int32_t act, float act_cst, void* dz,
+                            void* db, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
+    TFC_REQUIRE(tfc_dtype_ok(dtype), TFC_EINVAL, "tfc_dense_dz: unknown dtype %d", (int)dtype);
+    TFC_REQUIRE(act_ok(act), TFC_EINVAL, "tfc_dense_dz: unknown activation %d", (int)act);
+    TFC_REQUIRE(rows >= 0 && n >= 0, TFC_EINVAL, "tfc_dense_dz: negative size");
+    hipStream_t s = (hipStream_t)stream;
+    if (n == 0 || (!dz && !db)) return TFC_OK;
+    if (rows == 0) return db ? tfc_join_columns(nullptr, 0, n, db, 0, nullptr, dtype, s) : TFC_OK;
+    TFC_REQUIRE(dy && (z || act == TFC_ACT_IDENTITY), TFC_EINVAL, "tfc_dense_dz: null pointer");
+    const DzPlan p = dz_plan(rows, n, dtype);
+    TFC_REQUIRE(!db || (workspace && workspace_floats >= p.slabs * n), TFC_EINVAL, "tfc_dense_dz: workspace too small");
+    {
+        TfcProfScope prof("tfc_dense_dz", s);
+        const int rc = TFC_BY_DTYPE(dtype, dense_dz, p, dy, act == TFC_ACT_IDENTITY ? nullptr : z, rows, n, act, act_cst, dz,
+                                    db ? workspace : nullptr, s);
+        if (rc) return rc;
+    }
+    return db ? tfc_join_columns(workspace, p.slabs, n, db, 0, nullptr, dtype, s) : TFC_OK;
+}

@@ -40,6 +40,7 @@ __all__ = [
     "gate",
     "norm_activation",
     "layer_norm",
+    "dense",
 ]
 
 
@@ -1889,7 +1890,7 @@ def norm_activation(x, spec: GateSpec, eps_squared: float = 0.0, normalize: bool
     return _NormActFn.apply(_tracked(x), spec, float(eps_squared), bool(normalize))
 
 
-# ------------------------------------------------------------------ scalar head: layer norm
+# ------------------------------------------------------------------ scalar head: layer norm, dense product with its epilogue
 
 _AS_IS = contextlib.nullcontext()
 _dtype_codes = {torch.float32: _lib.F32, torch.bfloat16: _lib.BF16, torch.float16: _lib.F16}
@@ -1995,3 +1996,158 @@ def layer_norm(x, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Te
     else:
         y = _layer_norm_run(rows, w, b, float(eps), False)[0]
     return y.reshape(x.shape)
+
+
+def _operand(t: torch.Tensor):
+    """(tensor, ld, last axis contiguous?) of a 2-D operand: either axis may be the contiguous one, anything else is packed."""
+    (r, c), (sr, sc) = t.shape, t.stride()
+    if c <= 1 or sc == 1:
+        return t, (sr if r > 1 else max(c, 1)), True
+    if r <= 1 or sr == 1:
+        return t, sc, False
+    return t.contiguous(), c, True
+
+
+def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0, cst: float = 1.0, keep_z: bool = False):
+    """(c, z) of c = cst act(alpha a b + bias) + residual (tfc_dense)."""
+    m, k = a.shape
+    n = b.shape[1]
+    a, lda, a_along_k = _operand(a)
+    b, ldb, along_n = _operand(b)
+    if not a_along_k and not along_n:
+        a, lda, a_along_k = a.contiguous(), max(k, 1), True
+    c = torch.empty(m, n, dtype=a.dtype, device=a.device)
+    z = torch.empty_like(c) if keep_z else None
+    L = _lib.lib()
+    dt = _dtype_codes[a.dtype]
+    d = _lib.DenseDesc(m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, c.data_ptr(), max(n, 1), None if bias is None else bias.data_ptr(),
+                       None if residual is None else residual.data_ptr(), 0 if residual is None else max(n, 1),
+                       None if z is None else z.data_ptr(), alpha, cst, act, dt, a_along_k, not along_n)
+    with _on(a.device):
+        need = int(L.tfc_dense_workspace_floats(m, n, k, dt))
+        ws = torch.empty(need, dtype=torch.float32, device=a.device) if need else None
+        _lib.check(L.tfc_dense(C.byref(d), _ptr(ws), need, _stream()))
+    return c, z
+
+
+def _dense_dz(g, z, act: int, cst: float, need_dz: bool, need_db: bool):
+    """dz = cst act'(z) g and its column sums, either None when not asked for (tfc_dense_dz)."""
+    m, n = g.shape
+    dz = torch.empty_like(g) if need_dz else None
+    db = torch.empty(n, dtype=g.dtype, device=g.device) if need_db else None
+    L = _lib.lib()
+    dt = _dtype_codes[g.dtype]
+    with _on(g.device):
+        need = int(L.tfc_dense_dz_workspace_floats(m, n, dt)) if need_db else 0
+        ws = torch.empty(need, dtype=torch.float32, device=g.device) if need else None
+        _lib.check(L.tfc_dense_dz(_ptr(g), _ptr(z), m, n, dt, act, cst, _ptr(dz), _ptr(db), _ptr(ws), need, _stream()))
+    return dz, db
+
+
+class _DenseFn(torch.autograd.Function):
+    """x [m, k], w [k, n]; the pre-activation is kept in x's type when there is an activation to differentiate."""
+
+    @staticmethod
+    def forward(ctx, x, w, b, r, act: int, alpha: float, cst: float):
+        y, z = _dense_run(x, w, b, r, act, alpha, cst, keep_z=act != 0)
+        ctx.save_for_backward(x, w, b, z)
+        ctx.args = (act, alpha, cst)
+        return y
+
+    @staticmethod
+    def backward(ctx, g):
+        x, w, b, z = ctx.saved_tensors
+        act, alpha, cst = ctx.args
+        need = ctx.needs_input_grad
+        dr = g if need[3] else None
+        if not any(need[:3]):
+            return None, None, None, dr, None, None, None
+        if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
+            return (*_differentiable_grads(lambda: _dense_composite(x, w, b, act, alpha, cst), (x, w, b), need, g), dr, None, None, None)
+        g = g.contiguous()
+        dx = dw = db = None
+        if act == 0:  # the constant goes into the products' own factor
+            dz, scale = g, alpha * cst
+            if need[2]:
+                db = _dense_dz(g, None, 0, cst, False, True)[1]
+        else:
+            scale = alpha
+            dz, db = _dense_dz(g, z, act, cst, need[0] or need[1], need[2])
+        if need[0]:
+            dx = _dense_run(dz, w.t(), alpha=scale)[0]
+        if need[1]:  # in the weight's own order
+            dw = _dense_run(dz.t(), x, alpha=scale)[0].t() if w.stride(1) != 1 and w.stride(0) == 1 else _dense_run(x.t(), dz, alpha=scale)[0]
+        return dx, dw, db, dr, None, None, None
+
+
+class _ProductFn(torch.autograd.Function):
+    """alpha a b, differentiable to any order: its backward is two more such products."""
+
+    @staticmethod
+    def forward(ctx, a, b, alpha: float):
+        ctx.save_for_backward(a, b)
+        ctx.alpha = alpha
+        return _dense_run(a, b, alpha=alpha)[0]
+
+    @staticmethod
+    def backward(ctx, g):
+        a, b = ctx.saved_tensors
+        da = _ProductFn.apply(g, b.t(), ctx.alpha) if ctx.needs_input_grad[0] else None
+        db = _ProductFn.apply(a.t(), g, ctx.alpha) if ctx.needs_input_grad[1] else None
+        return da, db, None
+
+
+def _torch_act(act: int, v):
+    F = torch.nn.functional
+    return {0: lambda t: t, 1: lambda t: F.softplus(t) - math.log(2.0), 2: F.silu, 3: torch.tanh, 4: torch.abs, 5: torch.sigmoid,
+            6: F.gelu}[act](v)
+
+
+def _dense_composite(x, w, b, act: int, alpha: float, cst: float):
+    v = _ProductFn.apply(x, w, alpha).float()
+    if b is not None:
+        v = v + b.float()
+    return (_torch_act(act, v) * cst).to(x.dtype)
+
+
+def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, act: str = "identity",
+          alpha: float = 1.0, act_cst: float = 1.0):
+    """y = act_cst * act(alpha * x @ weight + bias) + residual in one product (tfc_dense); x [..., k], weight [k, n] (this
+    package's order; the transposed view of an [n, k] weight is taken as it lies), bias [n], residual [..., n], all fp32, bf16 or
+    fp16.  `act`: identity, ssp, silu, tanh, abs, sigmoid or gelu.
+
+    Sums are fp32 and the epilogue is applied to them before the one rounding to the result's type.  fp32 operands are cut into
+    three bf16 pieces, which loses nothing, but an operand that is not finite gives NaN.  Results are the same from run to
+    run.  For the backward pass the pre-activation is kept in x's type; the gradient at it is rounded to x's type before the
+    two products that need it, as the matrix instruction takes it.  Differentiable to any order: the first-order backward
+    is fused, a backward that is itself differentiated (`create_graph=True`) goes through torch's activations and this
+    kernel's products."""
+    _floats(x, "x")
+    _floats(weight, "weight", x)
+    if act not in _lib.DENSE_ACT:
+        raise ValueError(f"dense: unknown activation `{act}` (known: {sorted(_lib.DENSE_ACT)})")
+    if weight.dim() != 2 or x.dim() < 1 or x.shape[-1] != weight.shape[0]:
+        raise ValueError(f"dense: x {tuple(x.shape)} and weight {tuple(weight.shape)} do not fit ([..., k] and [k, n])")
+    if not (math.isfinite(alpha) and math.isfinite(act_cst)):
+        raise ValueError(f"dense: alpha and act_cst must be finite, got {alpha}, {act_cst}")
+    k, n = weight.shape
+    shape = (*x.shape[:-1], n)
+    if bias is not None:
+        _floats(bias, "bias", x)
+        if bias.shape != (n,):
+            raise ValueError(f"dense: `bias` must have shape ({n},), got {tuple(bias.shape)}")
+        bias = _tracked(bias)
+    rows = x.reshape(math.prod(x.shape[:-1]), k)
+    if k > 1 and rows.stride(1) != 1:
+        rows = rows.contiguous()
+    if residual is not None:
+        _floats(residual, "residual", x)
+        if residual.shape != shape:
+            raise ValueError(f"dense: `residual` must have shape {shape}, got {tuple(residual.shape)}")
+        residual = _tracked(residual.reshape(rows.shape[0], n))
+    args = _lib.DENSE_ACT[act], float(alpha), float(act_cst)
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+        y = _DenseFn.apply(rows, weight, bias, residual, *args)
+    else:
+        y = _dense_run(rows, weight, bias, residual, *args)[0]
+    return y.reshape(shape)
