@@ -27,23 +27,61 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 
 // ------------------------------------------------------------------------------------------------ activations
+// FAST (16-bit results): exp and 1/x as single instructions, a few 2^-22 of the result off where its half step is 2^-9 or 2^-12.
+template <bool FAST>
+__device__ __forceinline__ float exp_(float x) {
+    return FAST ? __expf(x) : expf(x);
+}
+template <bool FAST>
+__device__ __forceinline__ float inv_(float x) {
+    return FAST ? __builtin_amdgcn_rcpf(x) : 1.f / x;
+}
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_(float x) {
+    return inv_<FAST>(1.f + exp_<FAST>(-x));
+}
+// Half of erfc(|x| / sqrt 2): the normal distribution's tail beyond |x|.  FAST: erfc(z) = t exp(-z^2 + q(t)), t = 1 / (1 + z / 2), with
+// q a Chebyshev fit of degree 9 of log(erfc(z) exp(z^2) / t), off by at most 2.1e-7 (relative, in the tail too).
+template <bool FAST>
+__device__ __forceinline__ float tail_(float x) {
+    const float z = 0.70710678118654752440f * fabsf(x);
+    if (!FAST) return 0.5f * erfcf(z);
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.5f * z);
+    float q = 0.16738100959847832f;
+    q = q * t - 0.8013252602706117f;
+    q = q * t + 1.435545460278193f;
+    q = q * t - 1.0600993927570561f;
+    q = q * t + 0.2137827400077032f;
+    q = q * t - 0.15077300610628097f;
+    q = q * t + 0.0846820952510744f;
+    q = q * t + 0.3765501918286564f;
+    q = q * t + 0.9997568084310646f;
+    q = q * t - 1.265500578284187f;
+    return 0.5f * t * __expf(q - z * z);
+}
+
+template <bool FAST>
 __device__ __forceinline__ float act_eval(int act, float x) {
     switch (act) {
-        case TFC_ACT_SSP: return (x > 20.f ? x : log1pf(expf(x))) - 0.69314718055994530942f;
-        case TFC_ACT_SILU: return x / (1.f + expf(-x));
+        case TFC_ACT_SSP: return fmaxf(x, 0.f) + (FAST ? __logf(1.f + __expf(-fabsf(x))) : log1pf(expf(-fabsf(x)))) - 0.69314718055994530942f;
+        case TFC_ACT_SILU: return x * sigmoid_<FAST>(x);
         case TFC_ACT_TANH: return tanhf(x);
         case TFC_ACT_ABS: return fabsf(x);
-        case TFC_ACT_SIGMOID: return 1.f / (1.f + expf(-x));
-        case TFC_ACT_GELU: return 0.5f * x * erfcf(-0.70710678118654752440f * x);
+        case TFC_ACT_SIGMOID: return sigmoid_<FAST>(x);
+        case TFC_ACT_GELU: {
+            const float h = x * tail_<FAST>(x);
+            return x > 0.f ? x - h : h;
+        }
         default: return x;
     }
 }
 
+template <bool FAST>
 __device__ __forceinline__ float act_grad(int act, float x) {
     switch (act) {
-        case TFC_ACT_SSP: return 1.f / (1.f + expf(-x));
+        case TFC_ACT_SSP: return sigmoid_<FAST>(x);
         case TFC_ACT_SILU: {
-            const float s = 1.f / (1.f + expf(-x));
+            const float s = sigmoid_<FAST>(x);
             return s * (1.f + x * (1.f - s));
         }
         case TFC_ACT_TANH: {
@@ -52,11 +90,13 @@ __device__ __forceinline__ float act_grad(int act, float x) {
         }
         case TFC_ACT_ABS: return x > 0.f ? 1.f : (x < 0.f ? -1.f : 0.f);
         case TFC_ACT_SIGMOID: {
-            const float s = 1.f / (1.f + expf(-x));
+            const float s = sigmoid_<FAST>(x);
             return s * (1.f - s);
         }
-        case TFC_ACT_GELU:
-            return 0.5f * erfcf(-0.70710678118654752440f * x) + x * 0.39894228040143267794f * expf(-0.5f * x * x);
+        case TFC_ACT_GELU: {
+            const float h = tail_<FAST>(x);
+            return (x > 0.f ? 1.f - h : h) + x * 0.39894228040143267794f * exp_<FAST>(-0.5f * x * x);
+        }
         default: return 1.f;
     }
 }
@@ -94,73 +134,85 @@ __device__ __forceinline__ Unit3 split8(const float (&x)[8]) {
 }
 
 // What a thread has in flight of an operand tile of R rows: UNITS units of eight k.  Along k: unit u is row u / (K/8), eight k
-// from memory.  Along rows: a thread takes RV neighbouring rows x eight k, eight accesses of RV elements.
+// from memory.  Along rows: a thread takes RV neighbouring rows x eight k, eight accesses of RV elements, and turns them round
+// on the way to LDS.  A step that lies whole inside the operand is loaded without a comparison (one branch for the workgroup,
+// and nothing touches the values before store(): all accesses are in flight together).
 template <class T, int R, bool ALONG_K>
 struct Stage {
     static constexpr int K = Pieces<T>::K, UNITS = R * K / 8 / 256, KU = K / 8, LD = K + 8;
-    static constexpr int RV = UNITS;  // (rows of a thread when the memory runs along them)
-    T v[UNITS][8];
+    static constexpr int RV = UNITS, TR = R / RV;  // rows of a thread, threads along the rows (memory along the rows)
+    static constexpr int NR = ALONG_K ? UNITS : 8, NE = ALONG_K ? 8 : RV;
+    TfcPack<T, NE> raw[NR];
 
-    __device__ __forceinline__ void load(const Operand& o, long r0, long rows, long k0, long kend) {
-        const T* p = (const T*)o.p;
+    const T* at;    // this thread's first element of step 0
+    long hop, adv;  // elements to the thread's next access / to the next step
+    long r, k;      // its row and k there
+
+    __device__ __forceinline__ void start(const Operand& o, long r0, long k0) {
         const int t = threadIdx.x;
         if constexpr (ALONG_K) {
-#pragma unroll
-            for (int i = 0; i < UNITS; ++i) {
-                const int u = t + 256 * i;
-                const long r = r0 + u / KU, k = k0 + (u % KU) * 8, left = r < rows ? kend - k : 0;
-                const T* q = p + r * o.ld + k;
-                if (left >= 8) {
-                    const TfcPack<T, 8> w = tfc_load<T, 8>(q);
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[i][j] = w.e[j];
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 8; ++j) v[i][j] = j < left ? q[j] : (T)0.f;
-                }
-            }
+            r = r0 + t / KU, k = k0 + (t % KU) * 8;
+            at = (const T*)o.p + r * o.ld + k;
+            hop = (256 / KU) * o.ld, adv = K;
         } else {
-            constexpr int TR = R / RV;  // threads along the rows
-            const long r = r0 + (t % TR) * RV, k = k0 + (t / TR) * 8;
-            const long left = rows - r;
+            r = r0 + (t % TR) * RV, k = k0 + (t / TR) * 8;
+            at = (const T*)o.p + k * o.ld + r;
+            hop = o.ld, adv = K * o.ld;
+        }
+    }
+
+    // `inside`: the whole step of the whole tile lies inside the operand (the same in all threads).
+    __device__ __forceinline__ void load(bool inside, long rows, long kend) {
+        if (inside) {
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const T* q = p + (k + j) * o.ld + r;
-                if (k + j < kend && left >= RV) {
-                    const TfcPack<T, RV> w = tfc_load<T, RV>(q);
+            for (int i = 0; i < NR; ++i) raw[i] = tfc_load<T, NE>(at + i * hop);
+        } else {
 #pragma unroll
-                    for (int i = 0; i < RV; ++i) v[i][j] = w.e[i];
-                } else {
+            for (int i = 0; i < NR; ++i) {
+                const long ri = ALONG_K ? r + i * (256 / KU) : r, ki = ALONG_K ? k : k + i;
 #pragma unroll
-                    for (int i = 0; i < RV; ++i) v[i][j] = k + j < kend && i < left ? q[i] : (T)0.f;
+                for (int j = 0; j < NE; ++j) {
+                    const bool in = ALONG_K ? ri < rows && ki + j < kend : ri + j < rows && ki < kend;
+                    raw[i].e[j] = in ? at[i * hop + j] : (T)0.f;
                 }
             }
         }
+        at += adv;
+        k += K;
     }
 
     __device__ __forceinline__ void store(uint16_t* lds) const {  // planes of [R][LD]
         const int t = threadIdx.x;
 #pragma unroll
         for (int i = 0; i < UNITS; ++i) {
-            int r, ku;
-            if constexpr (ALONG_K) {
-                r = (t + 256 * i) / KU, ku = (t + 256 * i) % KU;
-            } else {
-                constexpr int TR = R / RV;
-                r = (t % TR) * RV + i, ku = t / TR;
-            }
-            uint16_t* q = lds + r * LD + ku * 8;
+            const int row = ALONG_K ? t / KU + i * (256 / KU) : (t % TR) * RV + i, ku = ALONG_K ? t % KU : t / TR;
+            uint16_t* q = lds + row * LD + ku * 8;
             if constexpr (std::is_same<T, float>::value) {
-                const Unit3 s = split8(v[i]);
-                *(uintx4*)q = s.h;
-                *(uintx4*)(q + R * LD) = s.m;
-                *(uintx4*)(q + 2 * R * LD) = s.l;
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) v[j] = ALONG_K ? raw[i % NR].e[j % NE] : raw[j % NR].e[i % NE];
+                const Unit3 u = split8(v);
+                *(uintx4*)q = u.h;
+                *(uintx4*)(q + R * LD) = u.m;
+                *(uintx4*)(q + 2 * R * LD) = u.l;
+            } else if constexpr (ALONG_K) {
+                *(uintx4*)q = __builtin_bit_cast(uintx4, raw[i]);
             } else {
                 uintx4 w;
-                __builtin_memcpy(&w, v[i], 16);
+                const int half = i & 1;  // which half of a word of the rows' accesses
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const uint32_t lo = word(raw[2 * j], i >> 1), hi = word(raw[2 * j + 1], i >> 1);
+                    w[j] = __builtin_amdgcn_perm(hi, lo, half ? 0x07060302u : 0x05040100u);
+                }
                 *(uintx4*)q = w;
             }
         }
+    }
+    static __device__ __forceinline__ uint32_t word(const TfcPack<T, NE>& p, int i) {
+        uint32_t w[sizeof(p) / 4];
+        __builtin_memcpy(w, &p, sizeof(p));
+        return w[i];
     }
 };
 
@@ -170,6 +222,9 @@ __device__ __forceinline__ floatx16 mma(tfc_bf16, uintx4 a, uintx4 b, floatx16 c
 __device__ __forceinline__ floatx16 mma(tfc_f16, uintx4 a, uintx4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
+
+template <class T>
+using Mma = std::conditional_t<std::is_same<T, float>::value, tfc_bf16, T>;  // what the matrix instruction takes
 
 // ------------------------------------------------------------------------------------------------ the product
 struct Args {
@@ -187,32 +242,37 @@ struct Args {
     int tiles_m, tiles_n;
 };
 
-// Four neighbouring columns of one row of C.
-template <class T>
-__device__ __forceinline__ void epilogue4(const Args& g, long row, long col, float (&v)[4]) {
+// N neighbouring columns of one row of C.
+template <class T, int N>
+__device__ __forceinline__ void epilogue(const Args& g, long row, long col, float (&v)[N]) {
     const long left = g.n - col;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] *= g.alpha;
+    for (int j = 0; j < N; ++j) v[j] *= g.alpha;
     if (g.bias) {
-        float b[4];
-        tfc_load_f<T, 4>((const T*)g.bias + col, left, b);
+        float b[N];
+        tfc_load_f<T, N>((const T*)g.bias + col, left, b);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += b[j];
+        for (int j = 0; j < N; ++j) v[j] += b[j];
     }
-    if (g.z) tfc_store_f<T, 4>((T*)g.z + row * g.n + col, left, v);
+    if (g.z) tfc_store_f<T, N>((T*)g.z + row * g.n + col, left, v);
     if (g.act != TFC_ACT_IDENTITY) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] = act_eval(g.act, v[j]);
+        for (int j = 0; j < N; ++j) v[j] = act_eval<sizeof(T) == 2>(g.act, v[j]);
     }
 #pragma unroll
-    for (int j = 0; j < 4; ++j) v[j] *= g.cst;
+    for (int j = 0; j < N; ++j) v[j] *= g.cst;
     if (g.res) {
-        float r[4];
-        tfc_load_f<T, 4>((const T*)g.res + row * g.ldr + col, left, r);
+        float r[N];
+        tfc_load_f<T, N>((const T*)g.res + row * g.ldr + col, left, r);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) v[j] += r[j];
+        for (int j = 0; j < N; ++j) v[j] += r[j];
     }
-    tfc_store_f<T, 4>((T*)g.c + row * g.ldc + col, left, v);
+    tfc_store_f<T, N>((T*)g.c + row * g.ldc + col, left, v);
+}
+
+__device__ __forceinline__ void wave_step() {  // LDS written by the wave's lanes is read by its other lanes
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
 }
 
 // BM x BN tile, waves 2 x 2.  SPLIT: this workgroup's part of the contraction to g.part.
@@ -230,26 +290,27 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int wm = (wave >> 1) * 32 * MI, wn = (wave & 1) * 32 * NI;
     const int fr = lane & 31, fk = (lane >> 5) * 8;
-    floatx16 acc[MI][NI], low[P == 3 ? MI : 1][P == 3 ? NI : 1];
+    floatx16 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
-        for (int j = 0; j < NI; ++j) {
-            acc[i][j] = floatx16(0.f);
-            if constexpr (P == 3) low[i][j] = floatx16(0.f);
-        }
+        for (int j = 0; j < NI; ++j) acc[i][j] = floatx16(0.f);
     Stage<T, BM, AK> sa;
     Stage<T, BN, BK> sb;
-    sa.load(g.a, m0, g.m, k0, k1);
-    sb.load(g.b, n0, g.n, k0, k1);
+    const bool in_a = m0 + BM <= g.m, in_b = n0 + BN <= g.n;
+    sa.start(g.a, m0, k0);
+    sb.start(g.b, n0, k0);
+    sa.load(in_a && k0 + K <= k1, g.m, k1);
+    sb.load(in_b && k0 + K <= k1, g.n, k1);
     for (long k = k0; k < k1; k += K) {
         __syncthreads();  // the step before has been read
         sa.store(la);
         sb.store(lb);
         __syncthreads();
         if (k + K < k1) {
-            sa.load(g.a, m0, g.m, k + K, k1);
-            sb.load(g.b, n0, g.n, k + K, k1);
+            const bool in_k = k + 2 * K <= k1;
+            sa.load(in_a && in_k, g.m, k1);
+            sb.load(in_b && in_k, g.n, k1);
         }
 #pragma unroll
         for (int kk = 0; kk < K; kk += 16) {
@@ -261,62 +322,89 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
 #pragma unroll
                 for (int j = 0; j < NI; ++j) fb[j][p] = *(const uintx4*)(lb + (p * BN + wn + 32 * j + fr) * LD + kk + fk);
             }
+            // (fp32: smallest terms first; the tiles take turns, so that no instruction waits for the one before it)
+            constexpr int TERMS = P == 3 ? 6 : 1, TB[6] = {0, 2, 1, 0, 1, 0}, TA[6] = {2, 0, 1, 1, 0, 0};
 #pragma unroll
-            for (int i = 0; i < MI; ++i)
+            for (int q = 0; q < TERMS; ++q)
 #pragma unroll
-                for (int j = 0; j < NI; ++j) {
-                    if constexpr (P == 3) {  // the small terms in an accumulator of their own
-                        low[i][j] = mma(tfc_bf16(), fb[j][0], fa[i][2], low[i][j]);
-                        low[i][j] = mma(tfc_bf16(), fb[j][2], fa[i][0], low[i][j]);
-                        low[i][j] = mma(tfc_bf16(), fb[j][1], fa[i][1], low[i][j]);
-                        low[i][j] = mma(tfc_bf16(), fb[j][0], fa[i][1], low[i][j]);
-                        low[i][j] = mma(tfc_bf16(), fb[j][1], fa[i][0], low[i][j]);
-                        acc[i][j] = mma(tfc_bf16(), fb[j][0], fa[i][0], acc[i][j]);
-                    } else {
-                        acc[i][j] = mma(T(), fb[j][0], fa[i][0], acc[i][j]);
-                    }
-                }
+                for (int i = 0; i < MI; ++i)
+#pragma unroll
+                    for (int j = 0; j < NI; ++j)
+                        acc[i][j] = mma(Mma<T>(), fb[j][P == 3 ? TB[q] : 0], fa[i][P == 3 ? TA[q] : 0], acc[i][j]);
         }
     }
+    // A lane holds 4 columns of 32 rows apart: 32 rows x 32 NI columns at a time go through the wave's own corner of LDS and come
+    // back as whole 16-byte accesses of neighbouring lanes (128 bytes of a row at least: storing the accumulators where they
+    // lie, 16 bytes of 32 different rows an instruction, made the widest forward product 390 us longer).
+    constexpr int V = SPLIT ? 4 : TfcType<T>::V, WC = 32 * NI, LW = WC + 4;
+    constexpr int LPR = WC / V, RPP = 64 / LPR;  // lanes of a row, rows of a pass
+    static_assert(4 * 32 * LW * 4 <= (int)sizeof(lds), "the waves' corners");
+    float* corner = (float*)lds + wave * 32 * LW;
+    __syncthreads();
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
-        const long row = m0 + wm + 32 * i + fr;
-        if (row >= g.m) continue;
+        wave_step();
 #pragma unroll
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                const long col = n0 + wn + 32 * j + 8 * q + (lane >> 5) * 4;
-                if (col >= g.n) continue;
-                float v[4];
+                TfcPack<float, 4> v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    v[e] = acc[i][j][4 * q + e];
-                    if constexpr (P == 3) v[e] += low[i][j][4 * q + e];
-                }
-                if constexpr (SPLIT)
-                    tfc_store_f<float, 4>(g.part + ((long)blockIdx.y * g.m + row) * g.n + col, g.n - col, v);
-                else
-                    epilogue4<T>(g, row, col, v);
+                for (int e = 0; e < 4; ++e) v.e[e] = acc[i][j][4 * q + e];
+                *(TfcPack<float, 4>*)__builtin_assume_aligned(corner + fr * LW + 32 * j + 8 * q + (lane >> 5) * 4, 16) = v;
             }
+        wave_step();
+#pragma unroll
+        for (int p = 0; p < 32 / RPP; ++p) {
+            const int rl = p * RPP + lane / LPR, cl = (lane % LPR) * V;
+            const long row = m0 + wm + 32 * i + rl, col = n0 + wn + cl;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const TfcPack<float, 4> w = *(const TfcPack<float, 4>*)__builtin_assume_aligned(corner + rl * LW + cl + e, 16);
+#pragma unroll
+                for (int f = 0; f < 4; ++f) v[e + f] = w.e[f];
+            }
+            if (row >= g.m || col >= g.n) continue;
+            if constexpr (SPLIT)
+                tfc_store_f<float, V>(g.part + ((long)blockIdx.y * g.m + row) * g.n + col, g.n - col, v);
+            else
+                epilogue<T, V>(g, row, col, v);
+        }
     }
 }
 
-template <class T>
+// 256 / W quads of columns x W walkers: walker w adds the parts w, w + W, ..., the walkers are joined in order.
+template <class T, int W>
 __global__ __launch_bounds__(256) void tfc_dense_join_kernel(const Args g, int splits) {
+    constexpr int Q = 256 / W;
+    __shared__ float lds[W > 1 ? W : 1][Q][4];
     const long nv = (g.n + 3) / 4, total = g.m * nv, slab = g.m * g.n;
-    for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
-        const long row = i / nv, col = (i - row * nv) * 4;
+    const int ql = threadIdx.x % Q, w = threadIdx.x / Q;
+    const long i = (long)blockIdx.x * Q + ql;
+    const long row = i / nv, col = (i - row * nv) * 4;
+    float v[4] = {0.f, 0.f, 0.f, 0.f};
+    if (i < total) {
         const float* p = g.part + row * g.n + col;
-        float v[4] = {0.f, 0.f, 0.f, 0.f};
-        for (int s = 0; s < splits; ++s) {
-            float w[4];
-            tfc_load_f<float, 4>(p + s * slab, g.n - col, w);
+#pragma unroll 4
+        for (int s = w; s < splits; s += W) {
+            float x[4];
+            tfc_load_f<float, 4>(p + s * slab, g.n - col, x);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] += w[j];
+            for (int j = 0; j < 4; ++j) v[j] += x[j];
         }
-        epilogue4<T>(g, row, col, v);
     }
+    if constexpr (W > 1) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lds[w][ql][j] = v[j];
+        __syncthreads();
+        if (w > 0) return;
+#pragma unroll
+        for (int k = 1; k < W; ++k)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] += lds[k][ql][j];
+    }
+    if (i < total) epilogue<T, 4>(g, row, col, v);
 }
 
 // An empty contraction: the epilogue of zeros.
@@ -326,7 +414,7 @@ __global__ __launch_bounds__(256) void tfc_dense_empty_kernel(const Args g) {
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long row = i / nv, col = (i - row * nv) * 4;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        epilogue4<T>(g, row, col, v);
+        epilogue<T, 4>(g, row, col, v);
     }
 }
 
@@ -351,7 +439,7 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
             if (z) {
                 tfc_load_f<T, V>(z + r * n + c, left, x);
 #pragma unroll
-                for (int j = 0; j < V; ++j) g[j] *= act_grad(act, x[j]);
+                for (int j = 0; j < V; ++j) g[j] *= act_grad<sizeof(T) == 2>(act, x[j]);
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -380,24 +468,32 @@ struct Plan {
     int64_t tiles_m, tiles_n, splits, k_split;
 };
 
-// Tiles: 128 x 128 where they fill the chip, else smaller ones (twice as many operand bytes through LDS for each product).  The
-// contraction is split until there are two workgroups for every CU, in parts of at least four steps.
+// Tiles: 128 x 128, or narrower ones for a narrow C (64 x 64 moves twice as many operand bytes through LDS for each product).  Where
+// the tiles alone do not put three workgroups (fp32: two, by LDS) on every CU the contraction is split, in parts of at least eight
+// steps; and where the partial tiles would not stay in the caches (over 16 MB) in parts long enough that writing and adding them
+// up takes less than half the time of the products: 1024 of k for 16 bits, 192 for fp32, whose products cost six times as much.
 Plan plan(int64_t m, int64_t n, int64_t k, int dtype) {
     Plan p{};
-    auto tiles = [&](int bm, int bn) { return ((m + bm - 1) / bm) * ((n + bn - 1) / bn); };
-    p.bm = p.bn = 64;
-    if (n > 64 && m > 64 && tiles(128, 128) >= 256)
-        p.bm = p.bn = 128;
-    else if (m > 64 && tiles(128, 64) >= 256)
-        p.bm = 128;
-    p.tiles_m = (m + p.bm - 1) / p.bm;
-    p.tiles_n = (n + p.bn - 1) / p.bn;
-    const int64_t step = dtype == TFC_F32 ? 32 : 64, steps = (k + step - 1) / step, have = p.tiles_m * p.tiles_n;
-    p.splits = 1;
-    if (have < 256) p.splits = std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(512 / have, steps / 4), 1024));
-    const int64_t each = (steps + p.splits - 1) / p.splits;
-    p.k_split = each * step;
-    p.splits = (steps + each - 1) / each;
+    const bool wide = dtype == TFC_F32;
+    const int64_t step = wide ? 32 : 64, steps = (k + step - 1) / step, want = wide ? 512 : 768;
+    auto take = [&](int bm, int bn) {
+        p.bm = bm, p.bn = bn;
+        p.tiles_m = (m + bm - 1) / bm;
+        p.tiles_n = (n + bn - 1) / bn;
+        const int64_t have = p.tiles_m * p.tiles_n;
+        p.splits = 1;
+        if (have < want) {
+            p.splits = std::max<int64_t>(1, std::min<int64_t>((want + have / 2) / have, steps / 8));
+            if (p.splits * m * n * 4 > (16 << 20)) p.splits = std::max<int64_t>(1, std::min<int64_t>(p.splits, k / (wide ? 192 : 1024)));
+        }
+        const int64_t each = (steps + p.splits - 1) / p.splits;
+        p.k_split = each * step;
+        p.splits = steps ? (steps + each - 1) / each : 1;
+        return have * p.splits >= 256;
+    };
+    if (m > 64 && n > 64 && take(128, 128)) return p;
+    if (m > 64 && take(128, 64)) return p;
+    take(64, 64);
     return p;
 }
 
@@ -433,7 +529,10 @@ int dense(Args g, const Plan& p, bool a_k, bool b_k, hipStream_t s) {
                    : b_k ? launch_layout<T, true, true>(g, p, s)
                          : launch_layout<T, true, false>(g, p, s);
     if (rc || p.splits == 1) return rc;
-    hipLaunchKernelGGL(tfc_dense_join_kernel<T>, dim3(flat), dim3(256), 0, s, g, (int)p.splits);
+    if (p.splits >= 32)  // (many parts: few columns, or they would fill the chip; walkers side by side keep the accesses in flight)
+        hipLaunchKernelGGL((tfc_dense_join_kernel<T, 16>), dim3((unsigned)((quads + 15) / 16)), dim3(256), 0, s, g, (int)p.splits);
+    else
+        hipLaunchKernelGGL((tfc_dense_join_kernel<T, 1>), dim3((unsigned)((quads + 255) / 256)), dim3(256), 0, s, g, (int)p.splits);
     TFC_LAUNCH_CHECK("tfc_dense_join");
     return TFC_OK;
 }
