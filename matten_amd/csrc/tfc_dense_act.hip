@@ -354,7 +354,7 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
                 *(TfcPack<float, 4>*)__builtin_assume_aligned(corner + fr * LW + 32 * j + 8 * q + (lane >> 5) * 4, 16) = v;
             }
         wave_step();
-#pragma unroll
+#pragma unroll 2  // (more, and the loop around it is not unrolled: the accumulators would be indexed in memory)
         for (int p = 0; p < 32 / RPP; ++p) {
             const int rl = p * RPP + lane / LPR, cl = (lane % LPR) * V;
             const long row = m0 + wm + 32 * i + rl, col = n0 + wn + cl;
