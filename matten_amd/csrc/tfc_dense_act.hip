@@ -275,6 +275,50 @@ __device__ __forceinline__ void wave_step() {  // LDS written by the wave's lane
     __builtin_amdgcn_wave_barrier();
 }
 
+constexpr int corner_floats(int ni) { return 32 * (32 * ni + 4); }
+
+// A wave's 32 MI x 32 NI part of C, first element (m0, n0).  A lane holds 4 columns of 32 rows apart: 32 rows x 32 NI columns at a time
+// go through the wave's own corner of LDS and come back as whole 16-byte accesses of neighbouring lanes (128 bytes of a row at
+// least: storing the accumulators where they lie, 16 bytes of 32 different rows an instruction, took 255 us longer in the
+// product of 16384 x 1024 x 4096).
+template <class T, int MI, int NI, bool SPLIT>
+__device__ __forceinline__ void write_out(const Args& g, const floatx16 (&acc)[MI][NI], float* corner, long m0, long n0) {
+    constexpr int V = SPLIT ? 4 : TfcType<T>::V, WC = 32 * NI, LW = WC + 4;
+    constexpr int LPR = WC / V, RPP = 64 / LPR;  // lanes of a row, rows of a pass
+    const int lane = threadIdx.x & 63, fr = lane & 31;
+#pragma unroll
+    for (int i = 0; i < MI; ++i) {
+        wave_step();
+#pragma unroll
+        for (int j = 0; j < NI; ++j)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                TfcPack<float, 4> v;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) v.e[e] = acc[i][j][4 * q + e];
+                *(TfcPack<float, 4>*)__builtin_assume_aligned(corner + fr * LW + 32 * j + 8 * q + (lane >> 5) * 4, 16) = v;
+            }
+        wave_step();
+#pragma unroll 2  // (more, and the loop around it is not unrolled: the accumulators would be indexed in memory)
+        for (int p = 0; p < 32 / RPP; ++p) {
+            const int rl = p * RPP + lane / LPR, cl = (lane % LPR) * V;
+            const long row = m0 + 32 * i + rl, col = n0 + cl;
+            float v[V];
+#pragma unroll
+            for (int e = 0; e < V; e += 4) {
+                const TfcPack<float, 4> w = *(const TfcPack<float, 4>*)__builtin_assume_aligned(corner + rl * LW + cl + e, 16);
+#pragma unroll
+                for (int f = 0; f < 4; ++f) v[e + f] = w.e[f];
+            }
+            if (row >= g.m || col >= g.n) continue;
+            if constexpr (SPLIT)
+                tfc_store_f<float, V>(g.part + ((long)blockIdx.y * g.m + row) * g.n + col, g.n - col, v);
+            else
+                epilogue<T, V>(g, row, col, v);
+        }
+    }
+}
+
 // BM x BN tile, waves 2 x 2.  SPLIT: this workgroup's part of the contraction to g.part.
 template <class T, bool AK, bool BK, int BM, int BN, bool SPLIT>
 __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
@@ -333,45 +377,129 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
                         acc[i][j] = mma(Mma<T>(), fb[j][P == 3 ? TB[q] : 0], fa[i][P == 3 ? TA[q] : 0], acc[i][j]);
         }
     }
-    // A lane holds 4 columns of 32 rows apart: 32 rows x 32 NI columns at a time go through the wave's own corner of LDS and come
-    // back as whole 16-byte accesses of neighbouring lanes (128 bytes of a row at least: storing the accumulators where they
-    // lie, 16 bytes of 32 different rows an instruction, made the widest forward product 390 us longer).
-    constexpr int V = SPLIT ? 4 : TfcType<T>::V, WC = 32 * NI, LW = WC + 4;
-    constexpr int LPR = WC / V, RPP = 64 / LPR;  // lanes of a row, rows of a pass
-    static_assert(4 * 32 * LW * 4 <= (int)sizeof(lds), "the waves' corners");
-    float* corner = (float*)lds + wave * 32 * LW;
+    static_assert(4 * corner_floats(NI) * 4 <= (int)sizeof(lds), "the waves' corners");
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < MI; ++i) {
-        wave_step();
-#pragma unroll
-        for (int j = 0; j < NI; ++j)
-#pragma unroll
-            for (int q = 0; q < 4; ++q) {
-                TfcPack<float, 4> v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v.e[e] = acc[i][j][4 * q + e];
-                *(TfcPack<float, 4>*)__builtin_assume_aligned(corner + fr * LW + 32 * j + 8 * q + (lane >> 5) * 4, 16) = v;
-            }
-        wave_step();
-#pragma unroll 2  // (more, and the loop around it is not unrolled: the accumulators would be indexed in memory)
-        for (int p = 0; p < 32 / RPP; ++p) {
-            const int rl = p * RPP + lane / LPR, cl = (lane % LPR) * V;
-            const long row = m0 + wm + 32 * i + rl, col = n0 + wn + cl;
-            float v[V];
-#pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                const TfcPack<float, 4> w = *(const TfcPack<float, 4>*)__builtin_assume_aligned(corner + rl * LW + cl + e, 16);
-#pragma unroll
-                for (int f = 0; f < 4; ++f) v[e + f] = w.e[f];
-            }
-            if (row >= g.m || col >= g.n) continue;
-            if constexpr (SPLIT)
-                tfc_store_f<float, V>(g.part + ((long)blockIdx.y * g.m + row) * g.n + col, g.n - col, v);
-            else
-                epilogue<T, V>(g, row, col, v);
+    write_out<T, MI, NI, SPLIT>(g, acc, (float*)lds + wave * corner_floats(NI), m0 + wm, n0 + wn);
+}
+
+// ------------------------------------------------------------------------------------------------ large 16-bit products
+// 256 x 256 tile of eight waves (2 x 4, 128 x 64 each: a wave multiplies eight 32 x 32 tiles for six operand reads), two LDS
+// images, one barrier a step of 64: the next step's operands are loaded into registers at the top of a step and written to the other
+// image near its end.  Operands lie in LDS as they do in memory; one that runs along the rows is [k][row], row stride padded by
+// 64 bytes, and is turned by the transposing LDS read: of 16 lanes, lane 4 j + i gives 4 rows of k = j and gets 4 k of its row.
+constexpr int BIG = 256, BIG_K = 64, BIG_LK = BIG_K + 8, BIG_LR = BIG + 32;
+constexpr int BIG_IMAGE = BIG * BIG_LK;  // (= BIG_K * BIG_LR: both orders take the same space)
+static_assert(BIG * BIG_LK == BIG_K * BIG_LR, "");
+
+template <class T, bool ALONG_K>
+struct BigStage {
+    TfcPack<T, 8> raw[4];
+    const T* at;
+    long hop, adv, r, k;
+
+    __device__ __forceinline__ void start(const Operand& o, long r0, long k0) {
+        const int t = threadIdx.x;
+        if constexpr (ALONG_K) {
+            r = r0 + t / 8, k = k0 + (t % 8) * 8;
+            at = (const T*)o.p + r * o.ld + k;
+            hop = 64 * o.ld, adv = BIG_K;
+        } else {
+            r = r0 + (t % 32) * 8, k = k0 + t / 32;
+            at = (const T*)o.p + k * o.ld + r;
+            hop = 16 * o.ld, adv = BIG_K * o.ld;
         }
     }
+    __device__ __forceinline__ void load(bool inside, long rows, long kend) {
+        if (inside) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) raw[i] = tfc_load<T, 8>(at + i * hop);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const bool in = ALONG_K ? r + 64 * i < rows && k + j < kend : r + j < rows && k + 16 * i < kend;
+                    raw[i].e[j] = in ? at[i * hop + j] : (T)0.f;
+                }
+        }
+        at += adv;
+        k += BIG_K;
+    }
+    __device__ __forceinline__ void store(uint16_t* lds) const {
+        const int t = threadIdx.x;
+        uint16_t* q = ALONG_K ? lds + (t / 8) * BIG_LK + (t % 8) * 8 : lds + (t / 32) * BIG_LR + (t % 32) * 8;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) *(uintx4*)(q + i * (ALONG_K ? 64 * BIG_LK : 16 * BIG_LR)) = __builtin_bit_cast(uintx4, raw[i]);
+    }
+};
+
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+// Fragment of 32 rows from row r0 on and 16 k from kk on.
+template <bool ALONG_K>
+__device__ __forceinline__ uintx4 big_fragment(const uint16_t* lds, int r0, int kk) {
+    const int lane = threadIdx.x & 63;
+    if constexpr (ALONG_K) return *(const uintx4*)(lds + (r0 + (lane & 31)) * BIG_LK + kk + (lane >> 5) * 8);
+    const uint16_t* q = lds + (kk + (lane >> 5) * 8 + ((lane & 15) >> 2)) * BIG_LR + r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+    typedef __attribute__((address_space(3))) shortx4* Lds;
+    const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 4 * BIG_LR));
+    struct {
+        shortx4 a, b;
+    } both = {lo, hi};
+    return __builtin_bit_cast(uintx4, both);
+}
+
+template <class T, bool AK, bool BK, bool SPLIT>
+__global__ __launch_bounds__(512) void tfc_dense_big_kernel(const Args g) {
+    __shared__ __attribute__((aligned(16))) uint16_t lds[4 * BIG_IMAGE];
+    const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x);
+    const long m0 = (long)(tile / g.tiles_n) * BIG, n0 = (long)(tile % g.tiles_n) * BIG;
+    const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
+    const long k1 = SPLIT ? (k0 + g.k_split < g.k ? k0 + g.k_split : g.k) : g.k;
+    const int wave = threadIdx.x >> 6, wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+    floatx16 acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = floatx16(0.f);
+    BigStage<T, AK> sa;
+    BigStage<T, BK> sb;
+    const bool in_a = m0 + BIG <= g.m, in_b = n0 + BIG <= g.n;
+    sa.start(g.a, m0, k0);
+    sb.start(g.b, n0, k0);
+    sa.load(in_a && k0 + BIG_K <= k1, g.m, k1);
+    sb.load(in_b && k0 + BIG_K <= k1, g.n, k1);
+    sa.store(lds);
+    sb.store(lds + BIG_IMAGE);
+    __syncthreads();
+    int image = 0;
+    for (long k = k0; k < k1; k += BIG_K, image ^= 1) {
+        const uint16_t *la = lds + image * 2 * BIG_IMAGE, *lb = la + BIG_IMAGE;
+        const bool more = k + BIG_K < k1;
+        if (more) {
+            const bool in_k = k + 2 * BIG_K <= k1;
+            sa.load(in_a && in_k, g.m, k1);
+            sb.load(in_b && in_k, g.n, k1);
+        }
+#pragma unroll
+        for (int kk = 0; kk < BIG_K; kk += 16) {
+            uintx4 fa[4], fb[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fa[i] = big_fragment<AK>(la, wm + 32 * i, kk);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) fb[j] = big_fragment<BK>(lb, wn + 32 * j, kk);
+            if (kk == BIG_K - 16 && more) {
+                sa.store(lds + (image ^ 1) * 2 * BIG_IMAGE);
+                sb.store(lds + (image ^ 1) * 2 * BIG_IMAGE + BIG_IMAGE);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = mma(T(), fb[j], fa[i], acc[i][j]);
+        }
+        __syncthreads();  // the other image is whole, this one has been read
+    }
+    write_out<T, 4, 2, SPLIT>(g, acc, (float*)lds + wave * corner_floats(2), m0 + wm, n0 + wn);
 }
 
 // 256 / W quads of columns x W walkers: walker w adds the parts w, w + W, ..., the walkers are joined in order.
@@ -464,7 +592,7 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
 
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
-    int bm, bn;
+    int bm, bn;  // (256 x 256: tfc_dense_big_kernel)
     int64_t tiles_m, tiles_n, splits, k_split;
 };
 
@@ -476,7 +604,7 @@ Plan plan(int64_t m, int64_t n, int64_t k, int dtype) {
     Plan p{};
     const bool wide = dtype == TFC_F32;
     const int64_t step = wide ? 32 : 64, steps = (k + step - 1) / step, want = wide ? 512 : 768;
-    auto take = [&](int bm, int bn) {
+    auto take = [&](int bm, int bn, int64_t want) {
         p.bm = bm, p.bn = bn;
         p.tiles_m = (m + bm - 1) / bm;
         p.tiles_n = (n + bn - 1) / bn;
@@ -491,9 +619,10 @@ Plan plan(int64_t m, int64_t n, int64_t k, int dtype) {
         p.splits = steps ? (steps + each - 1) / each : 1;
         return have * p.splits >= 256;
     };
-    if (m > 64 && n > 64 && take(128, 128)) return p;
-    if (m > 64 && take(128, 64)) return p;
-    take(64, 64);
+    if (!wide && m >= 256 && n >= 256 && take(256, 256, 256)) return p;
+    if (m > 64 && n > 64 && take(128, 128, want)) return p;
+    if (m > 64 && take(128, 64, want)) return p;
+    take(64, 64, want);
     return p;
 }
 
@@ -510,6 +639,17 @@ int launch_tile(const Args& g, const Plan& p, hipStream_t s) {
 
 template <class T, bool AK, bool BK>
 int launch_layout(const Args& g, const Plan& p, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (p.bn == 256) {
+            const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
+            if (p.splits > 1)
+                hipLaunchKernelGGL((tfc_dense_big_kernel<T, AK, BK, true>), grid, dim3(512), 0, s, g);
+            else
+                hipLaunchKernelGGL((tfc_dense_big_kernel<T, AK, BK, false>), grid, dim3(512), 0, s, g);
+            TFC_LAUNCH_CHECK("tfc_dense_big");
+            return TFC_OK;
+        }
+    }
     if (p.bn == 128) return launch_tile<T, AK, BK, 128, 128>(g, p, s);
     if (p.bm == 128) return launch_tile<T, AK, BK, 128, 64>(g, p, s);
     return launch_tile<T, AK, BK, 64, 64>(g, p, s);

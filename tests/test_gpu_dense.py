@@ -122,7 +122,7 @@ def test_activations(device, dt, act):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("m,k,n", [(4000, 200, 1100), (5000, 64, 64), (40000, 33, 70), (2048, 700, 2048)])
+@pytest.mark.parametrize("m,k,n", [(4000, 200, 1100), (5000, 64, 64), (40000, 33, 70), (2048, 700, 2048), (4100, 300, 4109)])
 def test_large(device, dt, m, k, n):
     """Every tile, one and many parts of the contraction (the weight's gradient sums over m)."""
     _check(*_inputs(m, k, n, dt, m + n, device), "silu", 1 / math.sqrt(k))
