@@ -133,52 +133,57 @@ __device__ __forceinline__ Unit3 split8(const float (&x)[8]) {
     return r;
 }
 
+// The comparisons of a step at an edge are made when it comes: kept from step to step they would cost the registers that a second
+// workgroup on the CU needs.
+__device__ __forceinline__ void hide(int& t) { asm volatile("" : "+v"(t)); }
+
 // What a thread has in flight of an operand tile of R rows: UNITS units of eight k.  Along k: unit u is row u / (K/8), eight k
 // from memory.  Along rows: a thread takes RV neighbouring rows x eight k, eight accesses of RV elements, and turns them round
-// on the way to LDS.  A step that lies whole inside the operand is loaded without a comparison (one branch for the workgroup,
-// and nothing touches the values before store(): all accesses are in flight together).
+// on the way to LDS.  A step is loaded without a comparison, from an address that is the workgroup's plus a 32-bit offset that is the
+// thread's for good (nothing touches the values before store(): all accesses are in flight together), wherever its accesses
+// stay inside the operand's memory: rows behind the last one are the last one again (their products are not stored), and an
+// access that begins in the last rows may run into the next k's.  The others (the tail of the contraction; along the rows, the
+// edge tile's last step) go element by element.
 template <class T, int R, bool ALONG_K>
 struct Stage {
     static constexpr int K = Pieces<T>::K, UNITS = R * K / 8 / 256, KU = K / 8, LD = K + 8;
     static constexpr int RV = UNITS, TR = R / RV;  // rows of a thread, threads along the rows (memory along the rows)
     static constexpr int NR = ALONG_K ? UNITS : 8, NE = ALONG_K ? 8 : RV;
     TfcPack<T, NE> raw[NR];
+    uint32_t off[NR];  // bytes from the tile's first element of this step
+    const char* base;
+    long adv;  // bytes to the next step
 
-    const T* at;    // this thread's first element of step 0
-    long hop, adv;  // elements to the thread's next access / to the next step
-    long r, k;      // its row and k there
-
-    __device__ __forceinline__ void start(const Operand& o, long r0, long k0) {
-        const int t = threadIdx.x;
-        if constexpr (ALONG_K) {
-            r = r0 + t / KU, k = k0 + (t % KU) * 8;
-            at = (const T*)o.p + r * o.ld + k;
-            hop = (256 / KU) * o.ld, adv = K;
-        } else {
-            r = r0 + (t % TR) * RV, k = k0 + (t / TR) * 8;
-            at = (const T*)o.p + k * o.ld + r;
-            hop = o.ld, adv = K * o.ld;
-        }
+    __device__ __forceinline__ void start(const Operand& o, long r0, long rows, long k0) {
+        const int t = threadIdx.x, last = (int)(rows < R ? rows : R) - 1;
+#pragma unroll
+        for (int i = 0; i < NR; ++i)
+            off[i] = (uint32_t)sizeof(T) * (ALONG_K ? (uint32_t)min(t / KU + i * (256 / KU), last) * (uint32_t)o.ld + (t % KU) * 8
+                                                    : (uint32_t)((t / TR) * 8 + i) * (uint32_t)o.ld + min((t % TR) * RV, last));
+        base = (const char*)o.p + sizeof(T) * (ALONG_K ? r0 * o.ld + k0 : k0 * o.ld + r0);
+        adv = sizeof(T) * (ALONG_K ? K : K * o.ld);
     }
 
-    // `inside`: the whole step of the whole tile lies inside the operand (the same in all threads).
-    __device__ __forceinline__ void load(bool inside, long rows, long kend) {
-        if (inside) {
+    // rows, k: how many of each there are from the tile's first on (FULL: a whole tile and a whole step).
+    template <bool FULL>
+    __device__ __forceinline__ void load(long rows, long k) {
+        int t = threadIdx.x;
+        if (!FULL) hide(t);
 #pragma unroll
-            for (int i = 0; i < NR; ++i) raw[i] = tfc_load<T, NE>(at + i * hop);
-        } else {
-#pragma unroll
-            for (int i = 0; i < NR; ++i) {
-                const long ri = ALONG_K ? r + i * (256 / KU) : r, ki = ALONG_K ? k : k + i;
+        for (int i = 0; i < NR; ++i) {
+            const T* q = (const T*)(base + off[i]);
+            if constexpr (FULL) {
+                raw[i] = tfc_load<T, NE>(q);
+            } else {
+                const int ri = ALONG_K ? t / KU + i * (256 / KU) : (t % TR) * RV, ki = ALONG_K ? (t % KU) * 8 : (t / TR) * 8 + i;
 #pragma unroll
                 for (int j = 0; j < NE; ++j) {
-                    const bool in = ALONG_K ? ri < rows && ki + j < kend : ri + j < rows && ki < kend;
-                    raw[i].e[j] = in ? at[i * hop + j] : (T)0.f;
+                    const bool in = ALONG_K ? ri < rows && ki + j < k : ri + j < rows && ki < k;
+                    raw[i].e[j] = in ? q[j] : (T)0.f;
                 }
             }
         }
-        at += adv;
-        k += K;
+        base += adv;
     }
 
     __device__ __forceinline__ void store(uint16_t* lds) const {  // planes of [R][LD]
@@ -227,6 +232,15 @@ template <class T>
 using Mma = std::conditional_t<std::is_same<T, float>::value, tfc_bf16, T>;  // what the matrix instruction takes
 
 // ------------------------------------------------------------------------------------------------ the product
+// How much of a contraction of k elements from k0 to k1 goes in whole steps without comparisons.  An operand along the rows whose tile
+// is not full must have eight elements between k and must not be at its last k: its accesses then end inside its memory.
+__device__ __forceinline__ long plain_part(long k0, long k1, long k, long step, bool full_a, long lda, bool full_b, long ldb) {
+    long n = (k1 - k0) / step * step;
+    if ((!full_a && lda < 8) || (!full_b && ldb < 8)) return 0;
+    if ((!full_a || !full_b) && k0 + n == k) n -= step;
+    return n < 0 ? 0 : n;
+}
+
 struct Args {
     Operand a, b;
     long m, n, k;
@@ -341,21 +355,17 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
         for (int j = 0; j < NI; ++j) acc[i][j] = floatx16(0.f);
     Stage<T, BM, AK> sa;
     Stage<T, BN, BK> sb;
-    const bool in_a = m0 + BM <= g.m, in_b = n0 + BN <= g.n;
-    sa.start(g.a, m0, k0);
-    sb.start(g.b, n0, k0);
-    sa.load(in_a && k0 + K <= k1, g.m, k1);
-    sb.load(in_b && k0 + K <= k1, g.n, k1);
-    for (long k = k0; k < k1; k += K) {
+    const long ra = g.m - m0, rb = g.n - n0;
+    sa.start(g.a, m0, ra, k0);
+    sb.start(g.b, n0, rb, k0);
+    // One step: its operands to LDS, then (MORE) the loads of the next one and the products.
+    auto step = [&](auto more, long left) {
         __syncthreads();  // the step before has been read
         sa.store(la);
         sb.store(lb);
         __syncthreads();
-        if (k + K < k1) {
-            const bool in_k = k + 2 * K <= k1;
-            sa.load(in_a && in_k, g.m, k1);
-            sb.load(in_b && in_k, g.n, k1);
-        }
+        if constexpr (more == 1) sa.template load<true>(ra, left), sb.template load<true>(rb, left);
+        if constexpr (more == 2) sa.template load<false>(ra, left), sb.template load<false>(rb, left);
 #pragma unroll
         for (int kk = 0; kk < K; kk += 16) {
             uintx4 fa[MI][P], fb[NI][P];
@@ -376,7 +386,17 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
                     for (int j = 0; j < NI; ++j)
                         acc[i][j] = mma(Mma<T>(), fb[j][P == 3 ? TB[q] : 0], fa[i][P == 3 ? TA[q] : 0], acc[i][j]);
         }
-    }
+    };
+    long left = k1 - k0;  // of the contraction, from the step in hand on
+    long plain = plain_part(k0, k1, g.k, K, AK || ra >= BM, g.a.ld, BK || rb >= BN, g.b.ld);
+    if (plain > 0)
+        sa.template load<true>(ra, left), sb.template load<true>(rb, left);
+    else
+        sa.template load<false>(ra, left), sb.template load<false>(rb, left);
+    for (; plain > K; plain -= K, left -= K) step(std::integral_constant<int, 1>(), left - K);
+#pragma unroll 1
+    for (; left > K; left -= K) step(std::integral_constant<int, 2>(), left - K);
+    step(std::integral_constant<int, 0>(), 0);
     static_assert(4 * corner_floats(NI) * 4 <= (int)sizeof(lds), "the waves' corners");
     __syncthreads();
     write_out<T, MI, NI, SPLIT>(g, acc, (float*)lds + wave * corner_floats(NI), m0 + wm, n0 + wn);
@@ -392,38 +412,40 @@ constexpr int BIG_IMAGE = BIG * BIG_LK;  // (= BIG_K * BIG_LR: both orders take 
 static_assert(BIG * BIG_LK == BIG_K * BIG_LR, "");
 
 template <class T, bool ALONG_K>
-struct BigStage {
+struct BigStage {  // (as Stage, in memory's own order)
     TfcPack<T, 8> raw[4];
-    const T* at;
-    long hop, adv, r, k;
+    uint32_t off[4];
+    const char* base;
+    long adv;
 
-    __device__ __forceinline__ void start(const Operand& o, long r0, long k0) {
-        const int t = threadIdx.x;
-        if constexpr (ALONG_K) {
-            r = r0 + t / 8, k = k0 + (t % 8) * 8;
-            at = (const T*)o.p + r * o.ld + k;
-            hop = 64 * o.ld, adv = BIG_K;
-        } else {
-            r = r0 + (t % 32) * 8, k = k0 + t / 32;
-            at = (const T*)o.p + k * o.ld + r;
-            hop = 16 * o.ld, adv = BIG_K * o.ld;
-        }
+    __device__ __forceinline__ void start(const Operand& o, long r0, long rows, long k0) {
+        const int t = threadIdx.x, last = (int)(rows < BIG ? rows : BIG) - 1;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            off[i] = 2u * (ALONG_K ? (uint32_t)min(t / 8 + 64 * i, last) * (uint32_t)o.ld + (t % 8) * 8
+                                   : (uint32_t)(t / 32 + 16 * i) * (uint32_t)o.ld + min((t % 32) * 8, last));
+        base = (const char*)o.p + 2 * (ALONG_K ? r0 * o.ld + k0 : k0 * o.ld + r0);
+        adv = 2 * (ALONG_K ? BIG_K : BIG_K * o.ld);
     }
-    __device__ __forceinline__ void load(bool inside, long rows, long kend) {
-        if (inside) {
+    template <bool FULL>
+    __device__ __forceinline__ void load(long rows, long k) {
+        int t = threadIdx.x;
+        if (!FULL) hide(t);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) raw[i] = tfc_load<T, 8>(at + i * hop);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < 4; ++i) {
+            const T* q = (const T*)(base + off[i]);
+            if constexpr (FULL) {
+                raw[i] = tfc_load<T, 8>(q);
+            } else {
+                const int ri = ALONG_K ? t / 8 + 64 * i : (t % 32) * 8, ki = ALONG_K ? (t % 8) * 8 : t / 32 + 16 * i;
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
-                    const bool in = ALONG_K ? r + 64 * i < rows && k + j < kend : r + j < rows && k + 16 * i < kend;
-                    raw[i].e[j] = in ? at[i * hop + j] : (T)0.f;
+                    const bool in = ALONG_K ? ri < rows && ki + j < k : ri + j < rows && ki < k;
+                    raw[i].e[j] = in ? q[j] : (T)0.f;
                 }
+            }
         }
-        at += adv;
-        k += BIG_K;
+        base += adv;
     }
     __device__ __forceinline__ void store(uint16_t* lds) const {
         const int t = threadIdx.x;
@@ -464,23 +486,14 @@ __global__ __launch_bounds__(512) void tfc_dense_big_kernel(const Args g) {
         for (int j = 0; j < 2; ++j) acc[i][j] = floatx16(0.f);
     BigStage<T, AK> sa;
     BigStage<T, BK> sb;
-    const bool in_a = m0 + BIG <= g.m, in_b = n0 + BIG <= g.n;
-    sa.start(g.a, m0, k0);
-    sb.start(g.b, n0, k0);
-    sa.load(in_a && k0 + BIG_K <= k1, g.m, k1);
-    sb.load(in_b && k0 + BIG_K <= k1, g.n, k1);
-    sa.store(lds);
-    sb.store(lds + BIG_IMAGE);
-    __syncthreads();
+    const long ra = g.m - m0, rb = g.n - n0;
+    sa.start(g.a, m0, ra, k0);
+    sb.start(g.b, n0, rb, k0);
     int image = 0;
-    for (long k = k0; k < k1; k += BIG_K, image ^= 1) {
+    auto step = [&](auto more, long left) {
         const uint16_t *la = lds + image * 2 * BIG_IMAGE, *lb = la + BIG_IMAGE;
-        const bool more = k + BIG_K < k1;
-        if (more) {
-            const bool in_k = k + 2 * BIG_K <= k1;
-            sa.load(in_a && in_k, g.m, k1);
-            sb.load(in_b && in_k, g.n, k1);
-        }
+        if constexpr (more == 1) sa.template load<true>(ra, left), sb.template load<true>(rb, left);
+        if constexpr (more == 2) sa.template load<false>(ra, left), sb.template load<false>(rb, left);
 #pragma unroll
         for (int kk = 0; kk < BIG_K; kk += 16) {
             uintx4 fa[4], fb[2];
@@ -488,7 +501,7 @@ __global__ __launch_bounds__(512) void tfc_dense_big_kernel(const Args g) {
             for (int i = 0; i < 4; ++i) fa[i] = big_fragment<AK>(la, wm + 32 * i, kk);
 #pragma unroll
             for (int j = 0; j < 2; ++j) fb[j] = big_fragment<BK>(lb, wn + 32 * j, kk);
-            if (kk == BIG_K - 16 && more) {
+            if (more && kk == BIG_K - 16) {
                 sa.store(lds + (image ^ 1) * 2 * BIG_IMAGE);
                 sb.store(lds + (image ^ 1) * 2 * BIG_IMAGE + BIG_IMAGE);
             }
@@ -497,8 +510,22 @@ __global__ __launch_bounds__(512) void tfc_dense_big_kernel(const Args g) {
 #pragma unroll
                 for (int j = 0; j < 2; ++j) acc[i][j] = mma(T(), fb[j], fa[i], acc[i][j]);
         }
+        image ^= 1;
         __syncthreads();  // the other image is whole, this one has been read
-    }
+    };
+    long left = k1 - k0;
+    long plain = plain_part(k0, k1, g.k, BIG_K, AK || ra >= BIG, g.a.ld, BK || rb >= BIG, g.b.ld);
+    if (plain > 0)
+        sa.template load<true>(ra, left), sb.template load<true>(rb, left);
+    else
+        sa.template load<false>(ra, left), sb.template load<false>(rb, left);
+    sa.store(lds);
+    sb.store(lds + BIG_IMAGE);
+    __syncthreads();
+    for (; plain > BIG_K; plain -= BIG_K, left -= BIG_K) step(std::integral_constant<int, 1>(), left - BIG_K);
+#pragma unroll 1
+    for (; left > BIG_K; left -= BIG_K) step(std::integral_constant<int, 2>(), left - BIG_K);
+    step(std::integral_constant<int, 0>(), 0);
     write_out<T, 4, 2, SPLIT>(g, acc, (float*)lds + wave * corner_floats(2), m0 + wm, n0 + wn);
 }
 
@@ -727,6 +754,8 @@ extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t work
                 "tfc_dense: an A that runs along its rows needs a B that runs along its columns");
     TFC_REQUIRE(d->lda >= 0 && d->ldb >= 0 && d->ldc >= d->n && (!d->residual || d->ldr >= 0), TFC_EINVAL, "tfc_dense: bad stride");
     const Plan p = d->k ? plan(d->m, d->n, d->k, d->dtype) : Plan{64, 64, 1, 1, 1, 0};
+    // (a thread's offset in a tile has 32 bits: 256 rows, or a step of 64, of the longest row)
+    TFC_REQUIRE(d->lda < 1 << 22 && d->ldb < 1 << 22, TFC_EUNSUPPORTED, "tfc_dense: operand rows of 2^22 elements or more");
     TFC_REQUIRE(p.tiles_m * p.tiles_n < (int64_t)1 << 31, TFC_EUNSUPPORTED, "tfc_dense: %lld x %lld has too many tiles",
                 (long long)d->m, (long long)d->n);
     TFC_REQUIRE(p.splits == 1 || (workspace && workspace_floats >= p.splits * d->m * d->n), TFC_EINVAL,

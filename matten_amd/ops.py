@@ -2002,7 +2002,7 @@ def _operand(t: torch.Tensor):
     """(tensor, ld, last axis contiguous?) of a 2-D operand: either axis may be the contiguous one, anything else is packed."""
     (r, c), (sr, sc) = t.shape, t.stride()
     if c <= 1 or sc == 1:
-        return t, (sr if r > 1 else max(c, 1)), True
+        return t, (sr if r > 1 else 0), True  # (one row: nothing strides)
     if r <= 1 or sr == 1:
         return t, sc, False
     return t.contiguous(), c, True

@@ -202,7 +202,7 @@ def test_values_that_are_not_finite(device):
             assert not torch.isfinite(y[33]).any()
             keep = [i for i in range(70) if i != 33]
             assert torch.equal(y[keep], ref[keep])
-        buf = torch.full((80, 64), float("nan"), dtype=dt, device=device)  # what lies around the operands is not read
+        buf = torch.full((80, 64), float("nan"), dtype=dt, device=device)  # what lies around the operands does not matter
         buf[:70, :45] = x
         assert torch.equal(ops.dense(buf[:70, :45], w, b, r), ref)
         big = torch.full((70, 45), torch.finfo(dt).max, dtype=dt, device=device)
