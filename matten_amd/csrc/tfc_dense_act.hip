@@ -25,6 +25,7 @@ typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
 
 // ------------------------------------------------------------------------------------------------ activations
 // FAST (16-bit results): exp and 1/x as single instructions, a few 2^-22 of the result off where its half step is 2^-9 or 2^-12.
@@ -137,87 +138,101 @@ __device__ __forceinline__ Unit3 split8(const float (&x)[8]) {
 // workgroup on the CU needs.
 __device__ __forceinline__ void hide(int& t) { asm volatile("" : "+v"(t)); }
 
-// What a thread has in flight of an operand tile of R rows: UNITS units of eight k.  Along k: unit u is row u / (K/8), eight k
-// from memory.  Along rows: a thread takes RV neighbouring rows x eight k, eight accesses of RV elements, and turns them round
-// on the way to LDS.  A step is loaded without a comparison, from an address that is the workgroup's plus a 32-bit offset that is the
-// thread's for good (nothing touches the values before store(): all accesses are in flight together), wherever its accesses
-// stay inside the operand's memory: rows behind the last one are the last one again (their products are not stored), and an
-// access that begins in the last rows may run into the next k's.  The others (the tail of the contraction; along the rows, the
-// edge tile's last step) go element by element.
+// What a thread has in flight of an operand tile of R rows and a step of K, and its way to LDS.
+//  along k: units of eight k of a row; LDS [row][K + 8].
+//  along the rows, 16 bits: units of eight rows of a k; LDS [k][R + 32], turned by the transposing LDS read (fragment()).  The padding
+//    puts the four k that such a read takes side by side into different quarters of the banks.
+//  along the rows, fp32: the pieces are formed on the way to LDS, so the turning is done there too: a thread takes RV neighbouring
+//    rows x eight k and writes units of eight k; LDS [row][K + 8].
+// A step is loaded without a comparison, from an address that is the workgroup's plus a 32-bit offset that is the thread's for
+// good (nothing touches the values before store(): all accesses are in flight together), wherever its accesses stay inside
+// the operand's memory: rows behind the last one are the last one again (their products are not stored), and an access that
+// begins in the last rows may run into the next k's.  The others (the tail of the contraction; along the rows, the edge
+// tile's last step) go element by element.
 template <class T, int R, bool ALONG_K>
 struct Stage {
-    static constexpr int K = Pieces<T>::K, UNITS = R * K / 8 / 256, KU = K / 8, LD = K + 8;
-    static constexpr int RV = UNITS, TR = R / RV;  // rows of a thread, threads along the rows (memory along the rows)
-    static constexpr int NR = ALONG_K ? UNITS : 8, NE = ALONG_K ? 8 : RV;
+    static constexpr bool F32 = std::is_same<T, float>::value, TURN = !ALONG_K && F32, TR_READ = !ALONG_K && !F32;
+    static constexpr int P = Pieces<T>::N, K = Pieces<T>::K, UNITS = R * K / 8 / 256;
+    static constexpr int LD = TR_READ ? R + 32 : K + 8;                  // 16-bit elements of an LDS row
+    static constexpr int IMAGE = TR_READ ? K * LD : P * R * LD;          // and of the operand's whole image
+    static constexpr int RV = TURN ? UNITS : 8;                          // rows of an access along the rows
+    static constexpr int NR = TURN ? 8 : UNITS, NE = TURN ? RV : 8;      // accesses, elements of one
+    static constexpr int SIDE = ALONG_K ? K / 8 : R / RV, HOP = 256 / SIDE;  // threads side by side; rows (or k) between accesses
     TfcPack<T, NE> raw[NR];
     uint32_t off[NR];  // bytes from the tile's first element of this step
     const char* base;
     long adv;  // bytes to the next step
 
+    // Row and k, in the tile and step, of access i of thread t.
+    static __device__ __forceinline__ int row_of(int t, int i) { return ALONG_K ? t / SIDE + i * HOP : (t % SIDE) * RV; }
+    static __device__ __forceinline__ int k_of(int t, int i) {
+        return ALONG_K ? (t % SIDE) * 8 : TURN ? (t / SIDE) * 8 + i : t / SIDE + i * HOP;
+    }
+
     __device__ __forceinline__ void start(const Operand& o, long r0, long rows, long k0) {
         const int t = threadIdx.x, last = (int)(rows < R ? rows : R) - 1;
 #pragma unroll
-        for (int i = 0; i < NR; ++i)
-            off[i] = (uint32_t)sizeof(T) * (ALONG_K ? (uint32_t)min(t / KU + i * (256 / KU), last) * (uint32_t)o.ld + (t % KU) * 8
-                                                    : (uint32_t)((t / TR) * 8 + i) * (uint32_t)o.ld + min((t % TR) * RV, last));
+        for (int i = 0; i < NR; ++i) {
+            const uint32_t r = (uint32_t)min(row_of(t, i), last), k = (uint32_t)k_of(t, i), ld = (uint32_t)o.ld;
+            off[i] = (uint32_t)sizeof(T) * (ALONG_K ? r * ld + k : k * ld + r);
+        }
         base = (const char*)o.p + sizeof(T) * (ALONG_K ? r0 * o.ld + k0 : k0 * o.ld + r0);
         adv = sizeof(T) * (ALONG_K ? K : K * o.ld);
     }
 
-    // rows, k: how many of each there are from the tile's first on (FULL: a whole tile and a whole step).
-    template <bool FULL>
+    // rows, k: how many of each there are from the tile's first on (PLAIN: accesses that need no comparison).
+    template <bool PLAIN>
     __device__ __forceinline__ void load(long rows, long k) {
         int t = threadIdx.x;
-        if (!FULL) hide(t);
+        if (!PLAIN) hide(t);
 #pragma unroll
         for (int i = 0; i < NR; ++i) {
             const T* q = (const T*)(base + off[i]);
-            if constexpr (FULL) {
+            if constexpr (PLAIN) {
                 raw[i] = tfc_load<T, NE>(q);
             } else {
-                const int ri = ALONG_K ? t / KU + i * (256 / KU) : (t % TR) * RV, ki = ALONG_K ? (t % KU) * 8 : (t / TR) * 8 + i;
+                const int r = row_of(t, i), kk = k_of(t, i);
 #pragma unroll
-                for (int j = 0; j < NE; ++j) {
-                    const bool in = ALONG_K ? ri < rows && ki + j < k : ri + j < rows && ki < k;
-                    raw[i].e[j] = in ? q[j] : (T)0.f;
-                }
+                for (int j = 0; j < NE; ++j) raw[i].e[j] = (ALONG_K ? r < rows && kk + j < k : r + j < rows && kk < k) ? q[j] : (T)0.f;
             }
         }
         base += adv;
     }
 
-    __device__ __forceinline__ void store(uint16_t* lds) const {  // planes of [R][LD]
+    __device__ __forceinline__ void store(uint16_t* lds) const {
         const int t = threadIdx.x;
+        if constexpr (!F32) {
 #pragma unroll
-        for (int i = 0; i < UNITS; ++i) {
-            const int row = ALONG_K ? t / KU + i * (256 / KU) : (t % TR) * RV + i, ku = ALONG_K ? t % KU : t / TR;
-            uint16_t* q = lds + row * LD + ku * 8;
-            if constexpr (std::is_same<T, float>::value) {
+            for (int i = 0; i < NR; ++i)
+                *(uintx4*)(lds + (ALONG_K ? row_of(t, i) * LD + k_of(t, i) : k_of(t, i) * LD + row_of(t, i))) = __builtin_bit_cast(uintx4, raw[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < UNITS; ++i) {
+                const int row = TURN ? row_of(t, 0) + i : row_of(t, i), k = k_of(t, 0);
                 float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = ALONG_K ? raw[i % NR].e[j % NE] : raw[j % NR].e[i % NE];
+                for (int j = 0; j < 8; ++j) v[j] = TURN ? raw[j % NR].e[i % NE] : raw[i % NR].e[j % NE];
                 const Unit3 u = split8(v);
+                uint16_t* q = lds + row * LD + k;
                 *(uintx4*)q = u.h;
                 *(uintx4*)(q + R * LD) = u.m;
                 *(uintx4*)(q + 2 * R * LD) = u.l;
-            } else if constexpr (ALONG_K) {
-                *(uintx4*)q = __builtin_bit_cast(uintx4, raw[i]);
-            } else {
-                uintx4 w;
-                const int half = i & 1;  // which half of a word of the rows' accesses
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const uint32_t lo = word(raw[2 * j], i >> 1), hi = word(raw[2 * j + 1], i >> 1);
-                    w[j] = __builtin_amdgcn_perm(hi, lo, half ? 0x07060302u : 0x05040100u);
-                }
-                *(uintx4*)q = w;
             }
         }
     }
-    static __device__ __forceinline__ uint32_t word(const TfcPack<T, NE>& p, int i) {
-        uint32_t w[sizeof(p) / 4];
-        __builtin_memcpy(w, &p, sizeof(p));
-        return w[i];
+
+    // Piece p of 32 rows from r0 on and 16 k from kk on, as the matrix instruction takes it: lane l has row l % 32, eight k from
+    // 8 (l / 32) on.  The transposing read gives, in each group of 16 lanes, lane i the column i of four rows of LDS of 16
+    // elements each, whose quarters the lanes 4 j .. 4 j + 3 address.
+    static __device__ __forceinline__ uintx4 fragment(const uint16_t* lds, int p, int r0, int kk) {
+        const int lane = threadIdx.x & 63;
+        if constexpr (!TR_READ) return *(const uintx4*)(lds + (p * R + r0 + (lane & 31)) * LD + kk + (lane >> 5) * 8);
+        const uint16_t* q = lds + (kk + (lane >> 5) * 8 + ((lane & 15) >> 2)) * LD + r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        typedef __attribute__((address_space(3))) shortx4* Lds;
+        struct {
+            shortx4 a, b;
+        } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q)), __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 4 * LD))};
+        return __builtin_bit_cast(uintx4, both);
     }
 };
 
@@ -335,26 +350,28 @@ __device__ __forceinline__ void write_out(const Args& g, const floatx16 (&acc)[M
 
 // BM x BN tile, waves 2 x 2.  SPLIT: this workgroup's part of the contraction to g.part.
 template <class T, bool AK, bool BK, int BM, int BN, bool SPLIT>
-__global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
-    constexpr int P = Pieces<T>::N, K = Pieces<T>::K, LD = K + 8;
+__global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
+    using A = Stage<T, BM, AK>;
+    using B = Stage<T, BN, BK>;
+    constexpr int P = Pieces<T>::N, K = Pieces<T>::K;
     constexpr int MI = BM / 64, NI = BN / 64;  // 32 x 32 tiles of a wave
-    __shared__ __attribute__((aligned(16))) uint16_t lds[P * (BM + BN) * LD];
+    constexpr int LDS = A::IMAGE + B::IMAGE > 8 * corner_floats(NI) ? A::IMAGE + B::IMAGE : 8 * corner_floats(NI);
+    __shared__ __attribute__((aligned(16))) uint16_t lds[LDS];
     uint16_t* la = lds;
-    uint16_t* lb = lds + P * BM * LD;
+    uint16_t* lb = lds + A::IMAGE;
     const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x);
     const long m0 = (long)(tile / g.tiles_n) * BM, n0 = (long)(tile % g.tiles_n) * BN;
     const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
     const long k1 = SPLIT ? (k0 + g.k_split < g.k ? k0 + g.k_split : g.k) : g.k;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int wave = threadIdx.x >> 6;
     const int wm = (wave >> 1) * 32 * MI, wn = (wave & 1) * 32 * NI;
-    const int fr = lane & 31, fk = (lane >> 5) * 8;
     floatx16 acc[MI][NI];
 #pragma unroll
     for (int i = 0; i < MI; ++i)
 #pragma unroll
         for (int j = 0; j < NI; ++j) acc[i][j] = floatx16(0.f);
-    Stage<T, BM, AK> sa;
-    Stage<T, BN, BK> sb;
+    A sa;
+    B sb;
     const long ra = g.m - m0, rb = g.n - n0;
     sa.start(g.a, m0, ra, k0);
     sb.start(g.b, n0, rb, k0);
@@ -372,9 +389,9 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
 #pragma unroll
             for (int p = 0; p < P; ++p) {
 #pragma unroll
-                for (int i = 0; i < MI; ++i) fa[i][p] = *(const uintx4*)(la + (p * BM + wm + 32 * i + fr) * LD + kk + fk);
+                for (int i = 0; i < MI; ++i) fa[i][p] = A::fragment(la, p, wm + 32 * i, kk);
 #pragma unroll
-                for (int j = 0; j < NI; ++j) fb[j][p] = *(const uintx4*)(lb + (p * BN + wn + 32 * j + fr) * LD + kk + fk);
+                for (int j = 0; j < NI; ++j) fb[j][p] = B::fragment(lb, p, wn + 32 * j, kk);
             }
             // (fp32: smallest terms first; the tiles take turns, so that no instruction waits for the one before it)
             constexpr int TERMS = P == 3 ? 6 : 1, TB[6] = {0, 2, 1, 0, 1, 0}, TA[6] = {2, 0, 1, 1, 0, 0};
@@ -397,136 +414,8 @@ __global__ __launch_bounds__(256) void tfc_dense_kernel(const Args g) {
 #pragma unroll 1
     for (; left > K; left -= K) step(std::integral_constant<int, 2>(), left - K);
     step(std::integral_constant<int, 0>(), 0);
-    static_assert(4 * corner_floats(NI) * 4 <= (int)sizeof(lds), "the waves' corners");
     __syncthreads();
     write_out<T, MI, NI, SPLIT>(g, acc, (float*)lds + wave * corner_floats(NI), m0 + wm, n0 + wn);
-}
-
-// ------------------------------------------------------------------------------------------------ large 16-bit products
-// 256 x 256 tile of eight waves (2 x 4, 128 x 64 each: a wave multiplies eight 32 x 32 tiles for six operand reads), two LDS
-// images, one barrier a step of 64: the next step's operands are loaded into registers at the top of a step and written to the other
-// image near its end.  Operands lie in LDS as they do in memory; one that runs along the rows is [k][row], row stride padded by
-// 64 bytes, and is turned by the transposing LDS read: of 16 lanes, lane 4 j + i gives 4 rows of k = j and gets 4 k of its row.
-constexpr int BIG = 256, BIG_K = 64, BIG_LK = BIG_K + 8, BIG_LR = BIG + 32;
-constexpr int BIG_IMAGE = BIG * BIG_LK;  // (= BIG_K * BIG_LR: both orders take the same space)
-static_assert(BIG * BIG_LK == BIG_K * BIG_LR, "");
-
-template <class T, bool ALONG_K>
-struct BigStage {  // (as Stage, in memory's own order)
-    TfcPack<T, 8> raw[4];
-    uint32_t off[4];
-    const char* base;
-    long adv;
-
-    __device__ __forceinline__ void start(const Operand& o, long r0, long rows, long k0) {
-        const int t = threadIdx.x, last = (int)(rows < BIG ? rows : BIG) - 1;
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-            off[i] = 2u * (ALONG_K ? (uint32_t)min(t / 8 + 64 * i, last) * (uint32_t)o.ld + (t % 8) * 8
-                                   : (uint32_t)(t / 32 + 16 * i) * (uint32_t)o.ld + min((t % 32) * 8, last));
-        base = (const char*)o.p + 2 * (ALONG_K ? r0 * o.ld + k0 : k0 * o.ld + r0);
-        adv = 2 * (ALONG_K ? BIG_K : BIG_K * o.ld);
-    }
-    template <bool FULL>
-    __device__ __forceinline__ void load(long rows, long k) {
-        int t = threadIdx.x;
-        if (!FULL) hide(t);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const T* q = (const T*)(base + off[i]);
-            if constexpr (FULL) {
-                raw[i] = tfc_load<T, 8>(q);
-            } else {
-                const int ri = ALONG_K ? t / 8 + 64 * i : (t % 32) * 8, ki = ALONG_K ? (t % 8) * 8 : t / 32 + 16 * i;
-#pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const bool in = ALONG_K ? ri < rows && ki + j < k : ri + j < rows && ki < k;
-                    raw[i].e[j] = in ? q[j] : (T)0.f;
-                }
-            }
-        }
-        base += adv;
-    }
-    __device__ __forceinline__ void store(uint16_t* lds) const {
-        const int t = threadIdx.x;
-        uint16_t* q = ALONG_K ? lds + (t / 8) * BIG_LK + (t % 8) * 8 : lds + (t / 32) * BIG_LR + (t % 32) * 8;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) *(uintx4*)(q + i * (ALONG_K ? 64 * BIG_LK : 16 * BIG_LR)) = __builtin_bit_cast(uintx4, raw[i]);
-    }
-};
-
-typedef short shortx4 __attribute__((ext_vector_type(4)));
-
-// Fragment of 32 rows from row r0 on and 16 k from kk on.
-template <bool ALONG_K>
-__device__ __forceinline__ uintx4 big_fragment(const uint16_t* lds, int r0, int kk) {
-    const int lane = threadIdx.x & 63;
-    if constexpr (ALONG_K) return *(const uintx4*)(lds + (r0 + (lane & 31)) * BIG_LK + kk + (lane >> 5) * 8);
-    const uint16_t* q = lds + (kk + (lane >> 5) * 8 + ((lane & 15) >> 2)) * BIG_LR + r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
-    typedef __attribute__((address_space(3))) shortx4* Lds;
-    const shortx4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q)), hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 4 * BIG_LR));
-    struct {
-        shortx4 a, b;
-    } both = {lo, hi};
-    return __builtin_bit_cast(uintx4, both);
-}
-
-template <class T, bool AK, bool BK, bool SPLIT>
-__global__ __launch_bounds__(512) void tfc_dense_big_kernel(const Args g) {
-    __shared__ __attribute__((aligned(16))) uint16_t lds[4 * BIG_IMAGE];
-    const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x);
-    const long m0 = (long)(tile / g.tiles_n) * BIG, n0 = (long)(tile % g.tiles_n) * BIG;
-    const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
-    const long k1 = SPLIT ? (k0 + g.k_split < g.k ? k0 + g.k_split : g.k) : g.k;
-    const int wave = threadIdx.x >> 6, wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
-    floatx16 acc[4][2];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) acc[i][j] = floatx16(0.f);
-    BigStage<T, AK> sa;
-    BigStage<T, BK> sb;
-    const long ra = g.m - m0, rb = g.n - n0;
-    sa.start(g.a, m0, ra, k0);
-    sb.start(g.b, n0, rb, k0);
-    int image = 0;
-    auto step = [&](auto more, long left) {
-        const uint16_t *la = lds + image * 2 * BIG_IMAGE, *lb = la + BIG_IMAGE;
-        if constexpr (more == 1) sa.template load<true>(ra, left), sb.template load<true>(rb, left);
-        if constexpr (more == 2) sa.template load<false>(ra, left), sb.template load<false>(rb, left);
-#pragma unroll
-        for (int kk = 0; kk < BIG_K; kk += 16) {
-            uintx4 fa[4], fb[2];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) fa[i] = big_fragment<AK>(la, wm + 32 * i, kk);
-#pragma unroll
-            for (int j = 0; j < 2; ++j) fb[j] = big_fragment<BK>(lb, wn + 32 * j, kk);
-            if (more && kk == BIG_K - 16) {
-                sa.store(lds + (image ^ 1) * 2 * BIG_IMAGE);
-                sb.store(lds + (image ^ 1) * 2 * BIG_IMAGE + BIG_IMAGE);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mma(T(), fb[j], fa[i], acc[i][j]);
-        }
-        image ^= 1;
-        __syncthreads();  // the other image is whole, this one has been read
-    };
-    long left = k1 - k0;
-    long plain = plain_part(k0, k1, g.k, BIG_K, AK || ra >= BIG, g.a.ld, BK || rb >= BIG, g.b.ld);
-    if (plain > 0)
-        sa.template load<true>(ra, left), sb.template load<true>(rb, left);
-    else
-        sa.template load<false>(ra, left), sb.template load<false>(rb, left);
-    sa.store(lds);
-    sb.store(lds + BIG_IMAGE);
-    __syncthreads();
-    for (; plain > BIG_K; plain -= BIG_K, left -= BIG_K) step(std::integral_constant<int, 1>(), left - BIG_K);
-#pragma unroll 1
-    for (; left > BIG_K; left -= BIG_K) step(std::integral_constant<int, 2>(), left - BIG_K);
-    step(std::integral_constant<int, 0>(), 0);
-    write_out<T, 4, 2, SPLIT>(g, acc, (float*)lds + wave * corner_floats(2), m0 + wm, n0 + wn);
 }
 
 // 256 / W quads of columns x W walkers: walker w adds the parts w, w + W, ..., the walkers are joined in order.
@@ -619,7 +508,7 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
 
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
-    int bm, bn;  // (256 x 256: tfc_dense_big_kernel)
+    int bm, bn;
     int64_t tiles_m, tiles_n, splits, k_split;
 };
 
@@ -646,7 +535,7 @@ Plan plan(int64_t m, int64_t n, int64_t k, int dtype) {
         p.splits = steps ? (steps + each - 1) / each : 1;
         return have * p.splits >= 256;
     };
-    if (!wide && m >= 256 && n >= 256 && take(256, 256, 256)) return p;
+    if (!wide && m >= 256 && n >= 128 && take(256, 128, 512) && p.tiles_m * p.tiles_n * p.splits >= 512) return p;
     if (m > 64 && n > 64 && take(128, 128, want)) return p;
     if (m > 64 && take(128, 64, want)) return p;
     take(64, 64, want);
@@ -666,17 +555,8 @@ int launch_tile(const Args& g, const Plan& p, hipStream_t s) {
 
 template <class T, bool AK, bool BK>
 int launch_layout(const Args& g, const Plan& p, hipStream_t s) {
-    if constexpr (sizeof(T) == 2) {
-        if (p.bn == 256) {
-            const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
-            if (p.splits > 1)
-                hipLaunchKernelGGL((tfc_dense_big_kernel<T, AK, BK, true>), grid, dim3(512), 0, s, g);
-            else
-                hipLaunchKernelGGL((tfc_dense_big_kernel<T, AK, BK, false>), grid, dim3(512), 0, s, g);
-            TFC_LAUNCH_CHECK("tfc_dense_big");
-            return TFC_OK;
-        }
-    }
+    if constexpr (sizeof(T) == 2)
+        if (p.bm == 256) return launch_tile<T, AK, BK, 256, 128>(g, p, s);
     if (p.bn == 128) return launch_tile<T, AK, BK, 128, 128>(g, p, s);
     if (p.bm == 128) return launch_tile<T, AK, BK, 128, 64>(g, p, s);
     return launch_tile<T, AK, BK, 64, 64>(g, p, s);
