@@ -21,7 +21,8 @@
 namespace {
 
 typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef unsigned uintx4 __attribute__((ext_vector_type(4)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef tfc_u32x4 uintx4;
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -75,6 +76,26 @@ __device__ __forceinline__ float act_eval(int act, float x) {
         }
         default: return x;
     }
+}
+
+// The same on an array: one branch for all of it, so that its elements' chains run side by side.
+template <bool FAST, int N>
+__device__ __forceinline__ void act_apply(int act, float (&v)[N]) {
+#define TFC_ACT_CASE(A)                                              \
+    case A: {                                                        \
+        _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = act_eval<FAST>(A, v[j]); \
+        break;                                                       \
+    }
+    switch (act) {
+        TFC_ACT_CASE(TFC_ACT_SSP)
+        TFC_ACT_CASE(TFC_ACT_SILU)
+        TFC_ACT_CASE(TFC_ACT_TANH)
+        TFC_ACT_CASE(TFC_ACT_ABS)
+        TFC_ACT_CASE(TFC_ACT_SIGMOID)
+        TFC_ACT_CASE(TFC_ACT_GELU)
+        default: break;
+    }
+#undef TFC_ACT_CASE
 }
 
 template <bool FAST>
@@ -158,7 +179,7 @@ struct Stage {
     static constexpr int RV = TURN ? UNITS : 8;                          // rows of an access along the rows
     static constexpr int NR = TURN ? 8 : UNITS, NE = TURN ? RV : 8;      // accesses, elements of one
     static constexpr int SIDE = ALONG_K ? K / 8 : R / RV, HOP = 256 / SIDE;  // threads side by side; rows (or k) between accesses
-    TfcPack<T, NE> raw[NR];
+    TfcRaw<T, NE> raw[NR];
     uint32_t off[NR];  // bytes from the tile's first element of this step
     const char* base;
     long adv;  // bytes to the next step
@@ -192,8 +213,10 @@ struct Stage {
                 raw[i] = tfc_load<T, NE>(q);
             } else {
                 const int r = row_of(t, i), kk = k_of(t, i);
+                T e[NE];
 #pragma unroll
-                for (int j = 0; j < NE; ++j) raw[i].e[j] = (ALONG_K ? r < rows && kk + j < k : r + j < rows && kk < k) ? q[j] : (T)0.f;
+                for (int j = 0; j < NE; ++j) e[j] = (ALONG_K ? r < rows && kk + j < k : r + j < rows && kk < k) ? q[j] : (T)0.f;
+                __builtin_memcpy(&raw[i], e, sizeof(e));
             }
         }
         base += adv;
@@ -204,14 +227,17 @@ struct Stage {
         if constexpr (!F32) {
 #pragma unroll
             for (int i = 0; i < NR; ++i)
-                *(uintx4*)(lds + (ALONG_K ? row_of(t, i) * LD + k_of(t, i) : k_of(t, i) * LD + row_of(t, i))) = __builtin_bit_cast(uintx4, raw[i]);
+                *(uintx4*)(lds + (ALONG_K ? row_of(t, i) * LD + k_of(t, i) : k_of(t, i) * LD + row_of(t, i))) = raw[i];
         } else {
+            float f[NR][NE];
+#pragma unroll
+            for (int i = 0; i < NR; ++i) tfc_unpack<T, NE>(raw[i], f[i]);
 #pragma unroll
             for (int i = 0; i < UNITS; ++i) {
                 const int row = TURN ? row_of(t, 0) + i : row_of(t, i), k = k_of(t, 0);
                 float v[8];
 #pragma unroll
-                for (int j = 0; j < 8; ++j) v[j] = TURN ? raw[j % NR].e[i % NE] : raw[i % NR].e[j % NE];
+                for (int j = 0; j < 8; ++j) v[j] = TURN ? f[j % NR][i % NE] : f[i % NR][j % NE];
                 const Unit3 u = split8(v);
                 uint16_t* q = lds + row * LD + k;
                 *(uintx4*)q = u.h;
@@ -271,32 +297,52 @@ struct Args {
     int tiles_m, tiles_n;
 };
 
-// N neighbouring columns of one row of C.
+// N neighbouring columns of one row of C, all inside; `res`: their residual where there is one.
 template <class T, int N>
-__device__ __forceinline__ void epilogue(const Args& g, long row, long col, float (&v)[N]) {
-    const long left = g.n - col;
+__device__ __forceinline__ void epilogue(const Args& g, long row, long col, float (&v)[N], TfcRaw<T, N> res) {
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] *= g.alpha;
     if (g.bias) {
         float b[N];
-        tfc_load_f<T, N>((const T*)g.bias + col, left, b);
+        tfc_unpack<T, N>(tfc_load<T, N>((const T*)g.bias + col), b);
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] += b[j];
     }
-    if (g.z) tfc_store_f<T, N>((T*)g.z + row * g.n + col, left, v);
-    if (g.act != TFC_ACT_IDENTITY) {
-#pragma unroll
-        for (int j = 0; j < N; ++j) v[j] = act_eval<sizeof(T) == 2>(g.act, v[j]);
-    }
+    if (g.z) tfc_store<T, N>((T*)g.z + row * g.n + col, tfc_pack<T, N>(v));
+    act_apply<sizeof(T) == 2>(g.act, v);
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] *= g.cst;
     if (g.res) {
         float r[N];
-        tfc_load_f<T, N>((const T*)g.res + row * g.ldr + col, left, r);
+        tfc_unpack<T, N>(res, r);
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] += r[j];
     }
-    tfc_store_f<T, N>((T*)g.c + row * g.ldc + col, left, v);
+    tfc_store<T, N>((T*)g.c + row * g.ldc + col, tfc_pack<T, N>(v));
+}
+
+template <class T, int N>
+__device__ __forceinline__ TfcRaw<T, N> residual(const Args& g, long row, long col) {
+    TfcRaw<T, N> r = {};
+    if (g.res) r = tfc_load<T, N>((const T*)g.res + row * g.ldr + col);
+    return r;
+}
+
+// Columns [col, col + N) of a row as far as there are any: whole, or one by one.
+template <class T, int N>
+__device__ __forceinline__ void epilogue_left(const Args& g, long row, long col, const float (&v)[N]) {
+    if (g.n - col >= N) {
+        float w[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) w[j] = v[j];
+        epilogue<T, N>(g, row, col, w, residual<T, N>(g, row, col));
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            float w[1] = {v[j]};
+            if (col + j < g.n) epilogue<T, 1>(g, row, col + j, w, residual<T, 1>(g, row, col + j));
+        }
+    }
 }
 
 __device__ __forceinline__ void wave_step() {  // LDS written by the wave's lanes is read by its other lanes
@@ -309,12 +355,26 @@ constexpr int corner_floats(int ni) { return 32 * (32 * ni + 4); }
 // A wave's 32 MI x 32 NI part of C, first element (m0, n0).  A lane holds 4 columns of 32 rows apart: 32 rows x 32 NI columns at a time
 // go through the wave's own corner of LDS and come back as whole 16-byte accesses of neighbouring lanes (128 bytes of a row at
 // least: storing the accumulators where they lie, 16 bytes of 32 different rows an instruction, took 255 us longer in the
-// product of 16384 x 1024 x 4096).
+// product of 16384 x 1024 x 4096).  The residual of the next 32 rows is asked for before this one's results are stored: a wait
+// for a load is a wait for every access before it, stores too.
 template <class T, int MI, int NI, bool SPLIT>
 __device__ __forceinline__ void write_out(const Args& g, const floatx16 (&acc)[MI][NI], float* corner, long m0, long n0) {
     constexpr int V = SPLIT ? 4 : TfcType<T>::V, WC = 32 * NI, LW = WC + 4;
-    constexpr int LPR = WC / V, RPP = 64 / LPR;  // lanes of a row, rows of a pass
-    const int lane = threadIdx.x & 63, fr = lane & 31;
+    constexpr int LPR = WC / V, RPP = 64 / LPR, PASSES = 32 / RPP;  // lanes of a row, rows of a pass
+    constexpr int TOGETHER = PASSES < 4 ? PASSES : 4;               // passes whose residuals are in flight together
+    const int lane = threadIdx.x & 63, fr = lane & 31, cl = (lane % LPR) * V;
+    const long col = n0 + cl;
+    const bool whole = g.n - n0 >= WC && g.m - m0 >= 32 * MI;  // (the same in all lanes)
+    TfcRaw<T, V> next[TOGETHER];
+    auto ask = [&](int i, int p0) {
+        if constexpr (!SPLIT) {
+            if (whole) {
+#pragma unroll
+                for (int p = 0; p < TOGETHER; ++p) next[p] = residual<T, V>(g, m0 + 32 * i + (p0 + p) * RPP + lane / LPR, col);
+            }
+        }
+    };
+    ask(0, 0);
 #pragma unroll
     for (int i = 0; i < MI; ++i) {
         wave_step();
@@ -322,28 +382,50 @@ __device__ __forceinline__ void write_out(const Args& g, const floatx16 (&acc)[M
         for (int j = 0; j < NI; ++j)
 #pragma unroll
             for (int q = 0; q < 4; ++q) {
-                TfcPack<float, 4> v;
+                floatx4 v;
 #pragma unroll
-                for (int e = 0; e < 4; ++e) v.e[e] = acc[i][j][4 * q + e];
-                *(TfcPack<float, 4>*)__builtin_assume_aligned(corner + fr * LW + 32 * j + 8 * q + (lane >> 5) * 4, 16) = v;
+                for (int e = 0; e < 4; ++e) v[e] = acc[i][j][4 * q + e];
+                *(floatx4*)(corner + fr * LW + 32 * j + 8 * q + (lane >> 5) * 4) = v;
             }
         wave_step();
-#pragma unroll 2  // (more, and the loop around it is not unrolled: the accumulators would be indexed in memory)
-        for (int p = 0; p < 32 / RPP; ++p) {
-            const int rl = p * RPP + lane / LPR, cl = (lane % LPR) * V;
-            const long row = m0 + 32 * i + rl, col = n0 + cl;
-            float v[V];
-#pragma unroll
-            for (int e = 0; e < V; e += 4) {
-                const TfcPack<float, 4> w = *(const TfcPack<float, 4>*)__builtin_assume_aligned(corner + rl * LW + cl + e, 16);
-#pragma unroll
-                for (int f = 0; f < 4; ++f) v[e + f] = w.e[f];
+        if (!whole) {  // an edge: element by element, straight from LDS
+#pragma unroll 1
+            for (int at = lane; at < 32 * WC; at += 64) {
+                const long row = m0 + 32 * i + at / WC, c = n0 + at % WC;
+                float v[1] = {corner[at / WC * LW + at % WC]};
+                if (row >= g.m || c >= g.n) continue;
+                if constexpr (SPLIT)
+                    g.part[((long)blockIdx.y * g.m + row) * g.n + c] = v[0];
+                else
+                    epilogue<T, 1>(g, row, c, v, residual<T, 1>(g, row, c));
             }
-            if (row >= g.m || col >= g.n) continue;
-            if constexpr (SPLIT)
-                tfc_store_f<float, V>(g.part + ((long)blockIdx.y * g.m + row) * g.n + col, g.n - col, v);
-            else
-                epilogue<T, V>(g, row, col, v);
+            continue;
+        }
+#pragma unroll
+        for (int p0 = 0; p0 < PASSES; p0 += TOGETHER) {
+            TfcRaw<T, V> res[TOGETHER];
+#pragma unroll
+            for (int p = 0; p < TOGETHER; ++p) res[p] = next[p];
+            if (p0 + TOGETHER < PASSES)
+                ask(i, p0 + TOGETHER);
+            else if (i + 1 < MI)
+                ask(i + 1, 0);
+#pragma unroll
+            for (int p = 0; p < TOGETHER; ++p) {
+                const int rl = (p0 + p) * RPP + lane / LPR;
+                const long row = m0 + 32 * i + rl;
+                float v[V];
+#pragma unroll
+                for (int e = 0; e < V; e += 4) {
+                    const floatx4 w = *(const floatx4*)(corner + rl * LW + cl + e);
+#pragma unroll
+                    for (int f = 0; f < 4; ++f) v[e + f] = w[f];
+                }
+                if constexpr (SPLIT)
+                    tfc_store<float, V>(g.part + ((long)blockIdx.y * g.m + row) * g.n + col, tfc_pack<float, V>(v));
+                else
+                    epilogue<T, V>(g, row, col, v, res[p]);
+            }
         }
     }
 }
@@ -359,8 +441,12 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
     __shared__ __attribute__((aligned(16))) uint16_t lds[LDS];
     uint16_t* la = lds;
     uint16_t* lb = lds + A::IMAGE;
-    const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x);
-    const long m0 = (long)(tile / g.tiles_n) * BM, n0 = (long)(tile % g.tiles_n) * BN;
+    // Neighbouring workgroups of an XCD share its L2: they take tiles in columns of GROUP (64 tiles in flight read 8 + 8 operand panels
+    // instead of 2 + 32 when they go along the rows of a wide C: its product 204 -> 196 us).
+    constexpr unsigned GROUP = 8;
+    const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x), strip = GROUP * (unsigned)g.tiles_n;
+    const unsigned top = tile / strip * GROUP, in = tile % strip, high = min(GROUP, (unsigned)g.tiles_m - top);
+    const long m0 = (long)(top + in % high) * BM, n0 = (long)(in / high) * BN;
     const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
     const long k1 = SPLIT ? (k0 + g.k_split < g.k ? k0 + g.k_split : g.k) : g.k;
     const int wave = threadIdx.x >> 6;
@@ -448,7 +534,7 @@ __global__ __launch_bounds__(256) void tfc_dense_join_kernel(const Args g, int s
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] += lds[k][ql][j];
     }
-    if (i < total) epilogue<T, 4>(g, row, col, v);
+    if (i < total) epilogue_left<T, 4>(g, row, col, v);
 }
 
 // An empty contraction: the epilogue of zeros.
@@ -458,7 +544,7 @@ __global__ __launch_bounds__(256) void tfc_dense_empty_kernel(const Args g) {
     for (long i = (long)blockIdx.x * 256 + threadIdx.x; i < total; i += (long)gridDim.x * 256) {
         const long row = i / nv, col = (i - row * nv) * 4;
         float v[4] = {0.f, 0.f, 0.f, 0.f};
-        epilogue<T, 4>(g, row, col, v);
+        epilogue_left<T, 4>(g, row, col, v);
     }
 }
 

@@ -29,41 +29,84 @@ inline bool tfc_dtype_ok(int dtype) { return dtype == TFC_F32 || dtype == TFC_BF
     ((dtype) == TFC_F32 ? F<float>(__VA_ARGS__) : (dtype) == TFC_BF16 ? F<tfc_bf16>(__VA_ARGS__) : F<tfc_f16>(__VA_ARGS__))
 
 // N elements at a pointer that is aligned to ONE element only: rows of odd width and views into flat buffers start anywhere,
-// and global memory takes 8- and 16-byte accesses at any address.
-template <class T, int N>
-struct TfcPack {
-    T e[N];
+// and global memory takes 8- and 16-byte accesses at any address.  They are held as whole words until they are used: an access
+// whose elements are named apart is taken apart by the compiler too, into narrower ones with a wait in every branch.
+typedef unsigned tfc_u32x4 __attribute__((ext_vector_type(4)));
+typedef unsigned tfc_u32x2 __attribute__((ext_vector_type(2)));
+template <int BYTES>
+struct TfcWords;
+template <>
+struct TfcWords<32> {
+    typedef unsigned type __attribute__((ext_vector_type(8)));
+};
+template <>
+struct TfcWords<16> {
+    typedef tfc_u32x4 type;
+};
+template <>
+struct TfcWords<8> {
+    typedef tfc_u32x2 type;
+};
+template <>
+struct TfcWords<4> {
+    typedef uint32_t type;
+};
+template <>
+struct TfcWords<2> {
+    typedef uint16_t type;
 };
 template <class T, int N>
-__device__ __forceinline__ TfcPack<T, N> tfc_load(const T* p) {
-    TfcPack<T, N> r;
+using TfcRaw = typename TfcWords<N * (int)sizeof(T)>::type;
+
+template <class T, int N>
+__device__ __forceinline__ TfcRaw<T, N> tfc_load(const T* p) {
+    TfcRaw<T, N> r;
     __builtin_memcpy(&r, p, sizeof(r));
     return r;
 }
 template <class T, int N>
-__device__ __forceinline__ void tfc_store(T* p, const TfcPack<T, N>& v) {
+__device__ __forceinline__ void tfc_store(T* p, TfcRaw<T, N> v) {
     __builtin_memcpy(p, &v, sizeof(v));
 }
+template <class T, int N>
+__device__ __forceinline__ void tfc_unpack(TfcRaw<T, N> r, float (&v)[N]) {
+    T e[N];
+    __builtin_memcpy(e, &r, sizeof(r));
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = (float)e[i];
+}
+template <class T, int N>
+__device__ __forceinline__ TfcRaw<T, N> tfc_pack(const float (&v)[N]) {
+    T e[N];
+#pragma unroll
+    for (int i = 0; i < N; ++i) e[i] = (T)v[i];
+    TfcRaw<T, N> r;
+    __builtin_memcpy(&r, e, sizeof(r));
+    return r;
+}
 
-// N elements as floats, those at or behind `left` as zeros / not written (left >= N: one access).
+// The same with `left` elements up to the end of the row: those at or behind it are zeros / not written.
+template <class T, int N>
+__device__ __forceinline__ TfcRaw<T, N> tfc_load_left(const T* p, long left) {
+    TfcRaw<T, N> r = {};
+    if (left >= N) {
+        r = tfc_load<T, N>(p);
+    } else if (left > 0) {
+        T e[N];
+#pragma unroll
+        for (int i = 0; i < N; ++i) e[i] = i < left ? p[i] : (T)0.f;
+        __builtin_memcpy(&r, e, sizeof(r));
+    }
+    return r;
+}
 template <class T, int N>
 __device__ __forceinline__ void tfc_load_f(const T* p, long left, float (&v)[N]) {
-    if (left >= N) {
-        const TfcPack<T, N> r = tfc_load<T, N>(p);
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = (float)r.e[i];
-    } else {
-#pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = i < left ? (float)p[i] : 0.f;
-    }
+    tfc_unpack<T, N>(tfc_load_left<T, N>(p, left), v);
 }
 template <class T, int N>
 __device__ __forceinline__ void tfc_store_f(T* p, long left, const float (&v)[N]) {
     if (left >= N) {
-        TfcPack<T, N> r;
-#pragma unroll
-        for (int i = 0; i < N; ++i) r.e[i] = (T)v[i];
-        tfc_store<T, N>(p, r);
+        tfc_store<T, N>(p, tfc_pack<T, N>(v));
     } else {
 #pragma unroll
         for (int i = 0; i < N; ++i)
