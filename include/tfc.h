@@ -588,8 +588,11 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
  *   b [k, n]: b_along_k: element (kk, j) at j ldb + kk, else at kk ldb + j.  (a along its rows with b along k: not built.)
  *   c: row stride ldc; residual (nullable) [m, n] with row stride ldr; bias (nullable) [n]; z (nullable) [m, n] packed: receives
  *   alpha a b + bias.  Workspace: tfc_dense_workspace_floats() (0: none).  k = 0: the epilogue of zeros.
- * tfc_dense_dz: dz = act_cst act'(z) dy (nullable) and db = its column sums (nullable; they need the workspace), all [rows, n]
- * packed; act identity: z is not read.  The backward pass is that and two more products. */
+ * Operand rows are shorter than 2^22 elements.
+ * tfc_dense_bwd: from dy [m, n] packed, with dz = act_cst act'(alpha x w + bias) dy:  dx = alpha dz w^T [m, k] packed,
+ *   dw = alpha x^T dz, packed in the order of w ([k, n], or [n, k] where w_along_k), db = the column sums of dz [n]; each nullable.
+ *   x [m, k] with row stride ldx.  z is what the forward call left, wanted where tfc_dense_keeps_z() says so (layers of at
+ *   most 64 x 64 form it again, from x, w and bias: one kernel, bound by reading x and dy once). */
 #define TFC_ACT_GELU 6 /* x Phi(x) with the normal distribution function Phi (tfc_dense only) */
 typedef struct tfc_dense_desc {
     int64_t m, n, k;
@@ -609,9 +612,25 @@ typedef struct tfc_dense_desc {
 
 int64_t tfc_dense_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype);
 int tfc_dense(const tfc_dense_desc* desc, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
-int64_t tfc_dense_dz_workspace_floats(int64_t rows, int64_t n, int32_t dtype);
-int tfc_dense_dz(const void* dy, const void* z, int64_t rows, int64_t n, int32_t dtype, int32_t act, float act_cst, void* dz,
-                 void* db, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
+typedef struct tfc_dense_bwd_desc {
+    int64_t m, n, k;
+    const void* x;
+    int64_t ldx;
+    const void* w;
+    int64_t ldw;
+    const void* bias;
+    const void* z;
+    const void* dy;
+    void* dx;
+    void* dw;
+    void* db;
+    float alpha, act_cst;
+    int32_t act, dtype, w_along_k;
+} tfc_dense_bwd_desc;
+
+int tfc_dense_keeps_z(int64_t n, int64_t k, int32_t act);
+int64_t tfc_dense_bwd_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act);
+int tfc_dense_bwd(const tfc_dense_bwd_desc* desc, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
 
 /* One AdamW step over many parameter tensors of one dtype (the reference's trainer steps torch.optim one tensor at a time,
  * eigenn/model/model.py:410-426).  With g the gradient, scaled by min(1, max_norm / (norm + 1e-6)) when max_norm > 0, and

@@ -123,6 +123,29 @@ class DenseDesc(C.Structure):
     ]
 
 
+class DenseBwdDesc(C.Structure):
+    _fields_ = [
+        ("m", C.c_int64),
+        ("n", C.c_int64),
+        ("k", C.c_int64),
+        ("x", C.c_void_p),
+        ("ldx", C.c_int64),
+        ("w", C.c_void_p),
+        ("ldw", C.c_int64),
+        ("bias", C.c_void_p),
+        ("z", C.c_void_p),
+        ("dy", C.c_void_p),
+        ("dx", C.c_void_p),
+        ("dw", C.c_void_p),
+        ("db", C.c_void_p),
+        ("alpha", C.c_float),
+        ("act_cst", C.c_float),
+        ("act", C.c_int32),
+        ("dtype", C.c_int32),
+        ("w_along_k", C.c_int32),
+    ]
+
+
 class AdamwTensor(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("p", "g", "m", "v", "m_scale", "v_scale", "step")] + [("n", C.c_int64), ("index", C.c_int32)]
 
@@ -214,8 +237,9 @@ SIGNATURES = {
     "tfc_layer_norm_bwd": (C.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P]),
     "tfc_dense_workspace_floats": (_I64, [_I64, _I64, _I64, _I32]),
     "tfc_dense": (C.c_int, [C.POINTER(DenseDesc), _P, _I64, _P]),
-    "tfc_dense_dz_workspace_floats": (_I64, [_I64, _I64, _I32]),
-    "tfc_dense_dz": (C.c_int, [_P, _P, _I64, _I64, _I32, _I32, _F, _P, _P, _P, _I64, _P]),
+    "tfc_dense_keeps_z": (C.c_int, [_I64, _I64, _I32]),
+    "tfc_dense_bwd_workspace_floats": (_I64, [_I64, _I64, _I64, _I32, _I32]),
+    "tfc_dense_bwd": (C.c_int, [C.POINTER(DenseBwdDesc), _P, _I64, _P]),
     "tfc_grad_sumsq_partials": (_I64, [C.POINTER(AdamwTensor), _I32]),
     "tfc_grad_sumsq": (C.c_int, [C.POINTER(AdamwTensor), _I32, _I32, _P, _P]),
     "tfc_adamw_workspace_bytes": (_I64, [_I32]),

@@ -1,0 +1,184 @@
+// What the dense products share (tfc_dense_act.hip, tfc_dense_narrow.hip): activations, the cut of fp32 into bf16 pieces, the matrix
+// instructions.
+#pragma once
+
+#include <type_traits>
+
+#include "tfc_types.h"
+
+namespace {
+
+typedef float floatx16 __attribute__((ext_vector_type(16)));
+typedef float floatx4 __attribute__((ext_vector_type(4)));
+typedef tfc_u32x4 uintx4;
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef short shortx4 __attribute__((ext_vector_type(4)));
+
+// FAST (16-bit results): exp and 1/x as single instructions, a few 2^-22 of the result off where its half step is 2^-9 or 2^-12.
+template <bool FAST>
+__device__ __forceinline__ float exp_(float x) {
+    return FAST ? __expf(x) : expf(x);
+}
+template <bool FAST>
+__device__ __forceinline__ float inv_(float x) {
+    return FAST ? __builtin_amdgcn_rcpf(x) : 1.f / x;
+}
+template <bool FAST>
+__device__ __forceinline__ float sigmoid_(float x) {
+    return inv_<FAST>(1.f + exp_<FAST>(-x));
+}
+// Half of erfc(|x| / sqrt 2): the normal distribution's tail beyond |x|.  FAST: erfc(z) = t exp(-z^2 + q(t)), t = 1 / (1 + z / 2), with
+// q a Chebyshev fit of degree 9 of log(erfc(z) exp(z^2) / t), off by at most 2.1e-7 (relative, in the tail too).
+template <bool FAST>
+__device__ __forceinline__ float tail_(float x) {
+    const float z = 0.70710678118654752440f * fabsf(x);
+    if (!FAST) return 0.5f * erfcf(z);
+    const float t = __builtin_amdgcn_rcpf(1.f + 0.5f * z);
+    float q = 0.16738100959847832f;
+    q = q * t - 0.8013252602706117f;
+    q = q * t + 1.435545460278193f;
+    q = q * t - 1.0600993927570561f;
+    q = q * t + 0.2137827400077032f;
+    q = q * t - 0.15077300610628097f;
+    q = q * t + 0.0846820952510744f;
+    q = q * t + 0.3765501918286564f;
+    q = q * t + 0.9997568084310646f;
+    q = q * t - 1.265500578284187f;
+    return 0.5f * t * __expf(q - z * z);
+}
+
+template <bool FAST>
+__device__ __forceinline__ float act_eval(int act, float x) {
+    switch (act) {
+        // (the log of 1 .. 2 to 2^-23 absolute, which is what is left of it beside ln 2)
+        case TFC_ACT_SSP: return fmaxf(x, 0.f) + __logf(1.f + exp_<FAST>(-fabsf(x))) - 0.69314718055994530942f;
+        case TFC_ACT_SILU: return x * sigmoid_<FAST>(x);
+        case TFC_ACT_TANH: return tanhf(x);
+        case TFC_ACT_ABS: return fabsf(x);
+        case TFC_ACT_SIGMOID: return sigmoid_<FAST>(x);
+        case TFC_ACT_GELU: {
+            const float h = x * tail_<FAST>(x);
+            return x > 0.f ? x - h : h;
+        }
+        default: return x;
+    }
+}
+
+// The same on an array: one branch for all of it, so that its elements' chains run side by side.
+template <bool FAST, int N>
+__device__ __forceinline__ void act_apply(int act, float (&v)[N]) {
+#define TFC_ACT_CASE(A)                                              \
+    case A: {                                                        \
+        _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = act_eval<FAST>(A, v[j]); \
+        break;                                                       \
+    }
+    switch (act) {
+        TFC_ACT_CASE(TFC_ACT_SSP)
+        TFC_ACT_CASE(TFC_ACT_SILU)
+        TFC_ACT_CASE(TFC_ACT_TANH)
+        TFC_ACT_CASE(TFC_ACT_ABS)
+        TFC_ACT_CASE(TFC_ACT_SIGMOID)
+        TFC_ACT_CASE(TFC_ACT_GELU)
+        default: break;
+    }
+#undef TFC_ACT_CASE
+}
+
+template <bool FAST>
+__device__ __forceinline__ float act_grad(int act, float x) {
+    switch (act) {
+        case TFC_ACT_SSP: return sigmoid_<FAST>(x);
+        case TFC_ACT_SILU: {
+            const float s = sigmoid_<FAST>(x);
+            return s * (1.f + x * (1.f - s));
+        }
+        case TFC_ACT_TANH: {
+            const float t = tanhf(x);
+            return 1.f - t * t;
+        }
+        case TFC_ACT_ABS: return x > 0.f ? 1.f : (x < 0.f ? -1.f : 0.f);
+        case TFC_ACT_SIGMOID: {
+            const float s = sigmoid_<FAST>(x);
+            return s * (1.f - s);
+        }
+        case TFC_ACT_GELU: {
+            const float h = tail_<FAST>(x);
+            return (x > 0.f ? 1.f - h : h) + x * 0.39894228040143267794f * exp_<FAST>(-0.5f * x * x);
+        }
+        default: return 1.f;
+    }
+}
+
+template <bool FAST, int N>
+__device__ __forceinline__ void act_grad_apply(int act, float (&v)[N]) {
+#define TFC_ACT_CASE(A)                                              \
+    case A: {                                                        \
+        _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = act_grad<FAST>(A, v[j]); \
+        break;                                                       \
+    }
+    switch (act) {
+        TFC_ACT_CASE(TFC_ACT_SSP)
+        TFC_ACT_CASE(TFC_ACT_SILU)
+        TFC_ACT_CASE(TFC_ACT_TANH)
+        TFC_ACT_CASE(TFC_ACT_ABS)
+        TFC_ACT_CASE(TFC_ACT_SIGMOID)
+        TFC_ACT_CASE(TFC_ACT_GELU)
+        default:
+            _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = 1.f;
+    }
+#undef TFC_ACT_CASE
+}
+
+template <class T>
+struct Pieces {
+    static constexpr int N = std::is_same<T, float>::value ? 3 : 1;
+    static constexpr int K = std::is_same<T, float>::value ? 32 : 64;  // contraction length of a step
+};
+
+// Eight consecutive k of one row, as fragments of the matrix instruction.
+struct Unit3 {
+    uintx4 h, m, l;
+};
+__device__ __forceinline__ Unit3 split8(const float (&x)[8]) {
+    Unit3 r;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const unsigned u0 = __float_as_uint(x[2 * i]), u1 = __float_as_uint(x[2 * i + 1]);
+        r.h[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // upper halves: cut, not rounded, so that nothing overflows
+        const float a0 = x[2 * i] - __uint_as_float(u0 & 0xffff0000u), a1 = x[2 * i + 1] - __uint_as_float(u1 & 0xffff0000u);
+        const bf16x2 mm = {(__bf16)a0, (__bf16)a1};
+        const unsigned mu = __builtin_bit_cast(unsigned, mm);
+        r.m[i] = mu;
+        const bf16x2 ll = {(__bf16)(a0 - __uint_as_float(mu << 16)), (__bf16)(a1 - __uint_as_float(mu & 0xffff0000u))};
+        r.l[i] = __builtin_bit_cast(unsigned, ll);
+    }
+    return r;
+}
+
+__device__ __forceinline__ floatx16 mma(tfc_bf16, uintx4 a, uintx4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+__device__ __forceinline__ floatx16 mma(tfc_f16, uintx4 a, uintx4 b, floatx16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+
+template <class T>
+using Mma = std::conditional_t<std::is_same<T, float>::value, tfc_bf16, T>;  // what the matrix instruction takes
+
+__device__ __forceinline__ void wave_step() {  // LDS written by the wave's lanes is read by its other lanes
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+// Six of the nine piece products, smallest first: pieces of one operand and of the other.
+constexpr int TFC_TERM_B[6] = {0, 2, 1, 0, 1, 0}, TFC_TERM_A[6] = {2, 0, 1, 1, 0, 0};
+
+}  // namespace
+
+// tfc_dense_narrow.hip: the backward pass of a layer of at most 64 x 64 in one kernel.
+constexpr int TFC_NARROW = 64;
+inline bool tfc_dense_is_narrow(int64_t n, int64_t k) { return n <= TFC_NARROW && k <= TFC_NARROW && n > 0 && k > 0; }
+int64_t tfc_dense_narrow_partials(int64_t m);
+int tfc_dense_narrow_bwd(const tfc_dense_bwd_desc* d, float* part, hipStream_t stream);

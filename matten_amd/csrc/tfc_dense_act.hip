@@ -13,147 +13,17 @@
 //
 // Few tiles and a long contraction (a weight's gradient over many rows): the contraction is split, partial tiles go to the
 // workspace and a second kernel adds them in order and applies the epilogue.
-#include "tfc_types.h"
+#include "tfc_dense_act.h"
 
 #include <algorithm>
-#include <type_traits>
 
 namespace {
-
-typedef float floatx16 __attribute__((ext_vector_type(16)));
-typedef float floatx4 __attribute__((ext_vector_type(4)));
-typedef tfc_u32x4 uintx4;
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-typedef short shortx4 __attribute__((ext_vector_type(4)));
-
-// ------------------------------------------------------------------------------------------------ activations
-// FAST (16-bit results): exp and 1/x as single instructions, a few 2^-22 of the result off where its half step is 2^-9 or 2^-12.
-template <bool FAST>
-__device__ __forceinline__ float exp_(float x) {
-    return FAST ? __expf(x) : expf(x);
-}
-template <bool FAST>
-__device__ __forceinline__ float inv_(float x) {
-    return FAST ? __builtin_amdgcn_rcpf(x) : 1.f / x;
-}
-template <bool FAST>
-__device__ __forceinline__ float sigmoid_(float x) {
-    return inv_<FAST>(1.f + exp_<FAST>(-x));
-}
-// Half of erfc(|x| / sqrt 2): the normal distribution's tail beyond |x|.  FAST: erfc(z) = t exp(-z^2 + q(t)), t = 1 / (1 + z / 2), with
-// q a Chebyshev fit of degree 9 of log(erfc(z) exp(z^2) / t), off by at most 2.1e-7 (relative, in the tail too).
-template <bool FAST>
-__device__ __forceinline__ float tail_(float x) {
-    const float z = 0.70710678118654752440f * fabsf(x);
-    if (!FAST) return 0.5f * erfcf(z);
-    const float t = __builtin_amdgcn_rcpf(1.f + 0.5f * z);
-    float q = 0.16738100959847832f;
-    q = q * t - 0.8013252602706117f;
-    q = q * t + 1.435545460278193f;
-    q = q * t - 1.0600993927570561f;
-    q = q * t + 0.2137827400077032f;
-    q = q * t - 0.15077300610628097f;
-    q = q * t + 0.0846820952510744f;
-    q = q * t + 0.3765501918286564f;
-    q = q * t + 0.9997568084310646f;
-    q = q * t - 1.265500578284187f;
-    return 0.5f * t * __expf(q - z * z);
-}
-
-template <bool FAST>
-__device__ __forceinline__ float act_eval(int act, float x) {
-    switch (act) {
-        case TFC_ACT_SSP: return fmaxf(x, 0.f) + (FAST ? __logf(1.f + __expf(-fabsf(x))) : log1pf(expf(-fabsf(x)))) - 0.69314718055994530942f;
-        case TFC_ACT_SILU: return x * sigmoid_<FAST>(x);
-        case TFC_ACT_TANH: return tanhf(x);
-        case TFC_ACT_ABS: return fabsf(x);
-        case TFC_ACT_SIGMOID: return sigmoid_<FAST>(x);
-        case TFC_ACT_GELU: {
-            const float h = x * tail_<FAST>(x);
-            return x > 0.f ? x - h : h;
-        }
-        default: return x;
-    }
-}
-
-// The same on an array: one branch for all of it, so that its elements' chains run side by side.
-template <bool FAST, int N>
-__device__ __forceinline__ void act_apply(int act, float (&v)[N]) {
-#define TFC_ACT_CASE(A)                                              \
-    case A: {                                                        \
-        _Pragma("unroll") for (int j = 0; j < N; ++j) v[j] = act_eval<FAST>(A, v[j]); \
-        break;                                                       \
-    }
-    switch (act) {
-        TFC_ACT_CASE(TFC_ACT_SSP)
-        TFC_ACT_CASE(TFC_ACT_SILU)
-        TFC_ACT_CASE(TFC_ACT_TANH)
-        TFC_ACT_CASE(TFC_ACT_ABS)
-        TFC_ACT_CASE(TFC_ACT_SIGMOID)
-        TFC_ACT_CASE(TFC_ACT_GELU)
-        default: break;
-    }
-#undef TFC_ACT_CASE
-}
-
-template <bool FAST>
-__device__ __forceinline__ float act_grad(int act, float x) {
-    switch (act) {
-        case TFC_ACT_SSP: return sigmoid_<FAST>(x);
-        case TFC_ACT_SILU: {
-            const float s = sigmoid_<FAST>(x);
-            return s * (1.f + x * (1.f - s));
-        }
-        case TFC_ACT_TANH: {
-            const float t = tanhf(x);
-            return 1.f - t * t;
-        }
-        case TFC_ACT_ABS: return x > 0.f ? 1.f : (x < 0.f ? -1.f : 0.f);
-        case TFC_ACT_SIGMOID: {
-            const float s = sigmoid_<FAST>(x);
-            return s * (1.f - s);
-        }
-        case TFC_ACT_GELU: {
-            const float h = tail_<FAST>(x);
-            return (x > 0.f ? 1.f - h : h) + x * 0.39894228040143267794f * exp_<FAST>(-0.5f * x * x);
-        }
-        default: return 1.f;
-    }
-}
 
 // ------------------------------------------------------------------------------------------------ operands
 struct Operand {
     const void* p;
     long ld;  // elements between rows (k contiguous) / between k (rows contiguous)
 };
-
-template <class T>
-struct Pieces {
-    static constexpr int N = std::is_same<T, float>::value ? 3 : 1;
-    static constexpr int K = std::is_same<T, float>::value ? 32 : 64;  // contraction length of a step
-};
-
-// Eight consecutive k of one row, as fragments of the matrix instruction.
-struct Unit3 {
-    uintx4 h, m, l;
-};
-__device__ __forceinline__ Unit3 split8(const float (&x)[8]) {
-    Unit3 r;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const unsigned u0 = __float_as_uint(x[2 * i]), u1 = __float_as_uint(x[2 * i + 1]);
-        r.h[i] = __builtin_amdgcn_perm(u1, u0, 0x07060302u);  // upper halves: cut, not rounded, so that nothing overflows
-        const float a0 = x[2 * i] - __uint_as_float(u0 & 0xffff0000u), a1 = x[2 * i + 1] - __uint_as_float(u1 & 0xffff0000u);
-        const bf16x2 mm = {(__bf16)a0, (__bf16)a1};
-        const unsigned mu = __builtin_bit_cast(unsigned, mm);
-        r.m[i] = mu;
-        const bf16x2 ll = {(__bf16)(a0 - __uint_as_float(mu << 16)), (__bf16)(a1 - __uint_as_float(mu & 0xffff0000u))};
-        r.l[i] = __builtin_bit_cast(unsigned, ll);
-    }
-    return r;
-}
 
 // The comparisons of a step at an edge are made when it comes: kept from step to step they would cost the registers that a second
 // workgroup on the CU needs.
@@ -262,16 +132,6 @@ struct Stage {
     }
 };
 
-__device__ __forceinline__ floatx16 mma(tfc_bf16, uintx4 a, uintx4 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
-}
-__device__ __forceinline__ floatx16 mma(tfc_f16, uintx4 a, uintx4 b, floatx16 c) {
-    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
-}
-
-template <class T>
-using Mma = std::conditional_t<std::is_same<T, float>::value, tfc_bf16, T>;  // what the matrix instruction takes
-
 // ------------------------------------------------------------------------------------------------ the product
 // How much of a contraction of k elements from k0 to k1 goes in whole steps without comparisons.  An operand along the rows whose tile
 // is not full must have eight elements between k and must not be at its last k: its accesses then end inside its memory.
@@ -343,11 +203,6 @@ __device__ __forceinline__ void epilogue_left(const Args& g, long row, long col,
             if (col + j < g.n) epilogue<T, 1>(g, row, col + j, w, residual<T, 1>(g, row, col + j));
         }
     }
-}
-
-__device__ __forceinline__ void wave_step() {  // LDS written by the wave's lanes is read by its other lanes
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
-    __builtin_amdgcn_wave_barrier();
 }
 
 constexpr int corner_floats(int ni) { return 32 * (32 * ni + 4); }
@@ -480,14 +335,14 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
                 for (int j = 0; j < NI; ++j) fb[j][p] = B::fragment(lb, p, wn + 32 * j, kk);
             }
             // (fp32: smallest terms first; the tiles take turns, so that no instruction waits for the one before it)
-            constexpr int TERMS = P == 3 ? 6 : 1, TB[6] = {0, 2, 1, 0, 1, 0}, TA[6] = {2, 0, 1, 1, 0, 0};
+            constexpr int TERMS = P == 3 ? 6 : 1;
 #pragma unroll
             for (int q = 0; q < TERMS; ++q)
 #pragma unroll
                 for (int i = 0; i < MI; ++i)
 #pragma unroll
                     for (int j = 0; j < NI; ++j)
-                        acc[i][j] = mma(Mma<T>(), fb[j][P == 3 ? TB[q] : 0], fa[i][P == 3 ? TA[q] : 0], acc[i][j]);
+                        acc[i][j] = mma(Mma<T>(), fb[j][P == 3 ? TFC_TERM_B[q] : 0], fa[i][P == 3 ? TFC_TERM_A[q] : 0], acc[i][j]);
         }
     };
     long left = k1 - k0;  // of the contraction, from the step in hand on
@@ -568,8 +423,9 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
             tfc_load_f<T, V>(dy + r * n + c, left, g);
             if (z) {
                 tfc_load_f<T, V>(z + r * n + c, left, x);
+                act_grad_apply<sizeof(T) == 2>(act, x);
 #pragma unroll
-                for (int j = 0; j < V; ++j) g[j] *= act_grad<sizeof(T) == 2>(act, x[j]);
+                for (int j = 0; j < V; ++j) g[j] *= x[j];
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
@@ -736,27 +592,87 @@ extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t work
     return TFC_BY_DTYPE(d->dtype, dense, g, p, d->a_along_k != 0, d->b_along_k != 0, s);
 }
 
-extern "C" int64_t tfc_dense_dz_workspace_floats(int64_t rows, int64_t n, int32_t dtype) {
-    if (rows <= 0 || n <= 0 || !tfc_dtype_ok(dtype)) return 0;
-    return dz_plan(rows, n, dtype).slabs * n;
-}
-
-extern "C" int tfc_dense_dz(const void* dy, const void* z, int64_t rows, int64_t n, int32_t dtype, int32_t act, float act_cst, void* dz,
-                            void* db, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
-    TFC_REQUIRE(tfc_dtype_ok(dtype), TFC_EINVAL, "tfc_dense_dz: unknown dtype %d", (int)dtype);
-    TFC_REQUIRE(act_ok(act), TFC_EINVAL, "tfc_dense_dz: unknown activation %d", (int)act);
-    TFC_REQUIRE(rows >= 0 && n >= 0, TFC_EINVAL, "tfc_dense_dz: negative size");
-    hipStream_t s = (hipStream_t)stream;
-    if (n == 0 || (!dz && !db)) return TFC_OK;
+static int dense_dz_pass(const void* dy, const void* z, int64_t rows, int64_t n, int dtype, int act, float cst, void* dz, void* db,
+                         float* part, hipStream_t s) {
     if (rows == 0) return db ? tfc_join_columns(nullptr, 0, n, db, 0, nullptr, dtype, s) : TFC_OK;
-    TFC_REQUIRE(dy && (z || act == TFC_ACT_IDENTITY), TFC_EINVAL, "tfc_dense_dz: null pointer");
     const DzPlan p = dz_plan(rows, n, dtype);
-    TFC_REQUIRE(!db || (workspace && workspace_floats >= p.slabs * n), TFC_EINVAL, "tfc_dense_dz: workspace too small");
     {
         TfcProfScope prof("tfc_dense_dz", s);
-        const int rc = TFC_BY_DTYPE(dtype, dense_dz, p, dy, act == TFC_ACT_IDENTITY ? nullptr : z, rows, n, act, act_cst, dz,
-                                    db ? workspace : nullptr, s);
+        const int rc = TFC_BY_DTYPE(dtype, dense_dz, p, dy, act == TFC_ACT_IDENTITY ? nullptr : z, rows, n, act, cst, dz,
+                                    db ? part : nullptr, s);
         if (rc) return rc;
     }
-    return db ? tfc_join_columns(workspace, p.slabs, n, db, 0, nullptr, dtype, s) : TFC_OK;
+    return db ? tfc_join_columns(part, p.slabs, n, db, 0, nullptr, dtype, s) : TFC_OK;
+}
+
+extern "C" int tfc_dense_keeps_z(int64_t n, int64_t k, int32_t act) { return act != TFC_ACT_IDENTITY && !tfc_dense_is_narrow(n, k); }
+
+// The general backward pass's workspace: [dz | what one of its parts needs at a time], in floats.
+struct BwdSpace {
+    int64_t dz, rest;
+};
+static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int dtype, int act) {
+    BwdSpace w{};
+    if (act != TFC_ACT_IDENTITY) w.dz = (m * n * (int64_t)tfc_dtype_size(dtype) + 15) / 16 * 4;
+    w.rest = std::max(m > 0 && n > 0 ? dz_plan(m, n, dtype).slabs * n : 0,
+                      std::max(tfc_dense_workspace_floats(m, k, n, dtype),
+                               std::max(tfc_dense_workspace_floats(k, n, m, dtype), tfc_dense_workspace_floats(n, k, m, dtype))));
+    return w;
+}
+
+extern "C" int64_t tfc_dense_bwd_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act) {
+    if (m < 0 || n < 0 || k < 0 || !tfc_dtype_ok(dtype)) return 0;
+    if (m > 0 && tfc_dense_is_narrow(n, k)) return tfc_dense_narrow_partials(m) * (k * n + n);
+    const BwdSpace w = bwd_space(m, n, k, dtype, act);
+    return w.dz + w.rest;
+}
+
+extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
+    TFC_REQUIRE(d, TFC_EINVAL, "tfc_dense_bwd: null descriptor");
+    TFC_REQUIRE(tfc_dtype_ok(d->dtype), TFC_EINVAL, "tfc_dense_bwd: unknown dtype %d", (int)d->dtype);
+    TFC_REQUIRE(act_ok(d->act), TFC_EINVAL, "tfc_dense_bwd: unknown activation %d", (int)d->act);
+    TFC_REQUIRE(d->m >= 0 && d->n >= 0 && d->k >= 0, TFC_EINVAL, "tfc_dense_bwd: negative size");
+    TFC_REQUIRE(d->ldx >= 0 && d->ldw >= 0, TFC_EINVAL, "tfc_dense_bwd: bad stride");
+    if (!d->dx && !d->dw && !d->db) return TFC_OK;
+    const int64_t m = d->m, n = d->n, k = d->k;
+    TFC_REQUIRE(m == 0 || n == 0 || (d->dy && (k == 0 || (d->x && d->w))), TFC_EINVAL, "tfc_dense_bwd: null pointer");
+    TFC_REQUIRE(m == 0 || n == 0 || d->z || !tfc_dense_keeps_z(n, k, d->act), TFC_EINVAL, "tfc_dense_bwd: activation %d needs z",
+                (int)d->act);
+    TFC_REQUIRE(workspace_floats >= tfc_dense_bwd_workspace_floats(m, n, k, d->dtype, d->act) && (workspace || workspace_floats == 0),
+                TFC_EINVAL, "tfc_dense_bwd: workspace too small");
+    hipStream_t s = (hipStream_t)stream;
+    if (m > 0 && tfc_dense_is_narrow(n, k)) return tfc_dense_narrow_bwd(d, workspace, s);
+    const BwdSpace space = bwd_space(m, n, k, d->dtype, d->act);
+    const bool plain = d->act == TFC_ACT_IDENTITY;  // its constant goes into the products' own factor
+    const void* dz = plain ? d->dy : (const void*)workspace;
+    float* rest = workspace + space.dz;
+    if (n > 0 && ((!plain && (d->dx || d->dw)) || d->db)) {
+        const int rc = dense_dz_pass(d->dy, d->z, m, n, d->dtype, d->act, d->act_cst, plain || !(d->dx || d->dw) ? nullptr : workspace,
+                                     d->db, rest, s);
+        if (rc) return rc;
+    }
+    tfc_dense_desc g{};
+    g.alpha = plain ? d->alpha * d->act_cst : d->alpha;
+    g.act_cst = 1.f, g.act = TFC_ACT_IDENTITY, g.dtype = d->dtype;
+    if (d->dx) {  // dz W^T
+        g.m = m, g.n = k, g.k = n;
+        g.a = dz, g.lda = n, g.a_along_k = 1;
+        g.b = d->w, g.ldb = d->ldw, g.b_along_k = !d->w_along_k;
+        g.c = d->dx, g.ldc = k;
+        const int rc = tfc_dense(&g, rest, space.rest, stream);
+        if (rc) return rc;
+    }
+    if (d->dw) {  // x^T dz, or its transpose, in the weight's own order
+        g.k = m, g.a_along_k = g.b_along_k = 0;
+        if (d->w_along_k) {
+            g.m = n, g.n = k;
+            g.a = dz, g.lda = n, g.b = d->x, g.ldb = d->ldx;
+        } else {
+            g.m = k, g.n = n;
+            g.a = d->x, g.lda = d->ldx, g.b = dz, g.ldb = n;
+        }
+        g.c = d->dw, g.ldc = g.n;
+        return tfc_dense(&g, rest, space.rest, stream);
+    }
+    return TFC_OK;
 }

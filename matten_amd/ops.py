@@ -2030,26 +2030,34 @@ def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0,
     return c, z
 
 
-def _dense_dz(g, z, act: int, cst: float, need_dz: bool, need_db: bool):
-    """dz = cst act'(z) g and its column sums, either None when not asked for (tfc_dense_dz)."""
-    m, n = g.shape
-    dz = torch.empty_like(g) if need_dz else None
-    db = torch.empty(n, dtype=g.dtype, device=g.device) if need_db else None
+def _dense_bwd_run(g, x, w, b, z, act: int, alpha: float, cst: float, need):
+    """(dx, dw, db) of a contiguous incoming gradient, None where not needed (tfc_dense_bwd); dw in the weight's own order."""
+    m, k = x.shape
+    n = w.shape[1]
+    x, ldx, _ = _operand(x)
+    w, ldw, along_n = _operand(w)
+    new = functools.partial(torch.empty, dtype=g.dtype, device=g.device)
+    dx = new(m, k) if need[0] else None
+    dw = (new(k, n) if along_n else new(n, k)) if need[1] else None
+    db = new(n) if need[2] else None
+    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     L = _lib.lib()
     dt = _dtype_codes[g.dtype]
+    d = _lib.DenseBwdDesc(m, n, k, x.data_ptr(), ldx, w.data_ptr(), ldw, at(b), at(z), g.data_ptr(), at(dx), at(dw), at(db), alpha, cst,
+                          act, dt, not along_n)
     with _on(g.device):
-        need = int(L.tfc_dense_dz_workspace_floats(m, n, dt)) if need_db else 0
-        ws = torch.empty(need, dtype=torch.float32, device=g.device) if need else None
-        _lib.check(L.tfc_dense_dz(_ptr(g), _ptr(z), m, n, dt, act, cst, _ptr(dz), _ptr(db), _ptr(ws), need, _stream()))
-    return dz, db
+        floats = int(L.tfc_dense_bwd_workspace_floats(m, n, k, dt, act))
+        ws = torch.empty(floats, dtype=torch.float32, device=g.device) if floats else None
+        _lib.check(L.tfc_dense_bwd(C.byref(d), _ptr(ws), floats, _stream()))
+    return dx, (dw if along_n or dw is None else dw.t()), db
 
 
 class _DenseFn(torch.autograd.Function):
-    """x [m, k], w [k, n]; the pre-activation is kept in x's type when there is an activation to differentiate."""
+    """x [m, k], w [k, n]; the pre-activation is kept, in x's type, where the backward kernels want it."""
 
     @staticmethod
     def forward(ctx, x, w, b, r, act: int, alpha: float, cst: float):
-        y, z = _dense_run(x, w, b, r, act, alpha, cst, keep_z=act != 0)
+        y, z = _dense_run(x, w, b, r, act, alpha, cst, keep_z=bool(_lib.lib().tfc_dense_keeps_z(w.shape[1], w.shape[0], act)))
         ctx.save_for_backward(x, w, b, z)
         ctx.args = (act, alpha, cst)
         return y
@@ -2057,27 +2065,13 @@ class _DenseFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, g):
         x, w, b, z = ctx.saved_tensors
-        act, alpha, cst = ctx.args
         need = ctx.needs_input_grad
         dr = g if need[3] else None
         if not any(need[:3]):
             return None, None, None, dr, None, None, None
         if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
-            return (*_differentiable_grads(lambda: _dense_composite(x, w, b, act, alpha, cst), (x, w, b), need, g), dr, None, None, None)
-        g = g.contiguous()
-        dx = dw = db = None
-        if act == 0:  # the constant goes into the products' own factor
-            dz, scale = g, alpha * cst
-            if need[2]:
-                db = _dense_dz(g, None, 0, cst, False, True)[1]
-        else:
-            scale = alpha
-            dz, db = _dense_dz(g, z, act, cst, need[0] or need[1], need[2])
-        if need[0]:
-            dx = _dense_run(dz, w.t(), alpha=scale)[0]
-        if need[1]:  # in the weight's own order
-            dw = _dense_run(dz.t(), x, alpha=scale)[0].t() if w.stride(1) != 1 and w.stride(0) == 1 else _dense_run(x.t(), dz, alpha=scale)[0]
-        return dx, dw, db, dr, None, None, None
+            return (*_differentiable_grads(lambda: _dense_composite(x, w, b, *ctx.args), (x, w, b), need, g), dr, None, None, None)
+        return (*_dense_bwd_run(g.contiguous(), x, w, b, z, *ctx.args, need), dr, None, None, None)
 
 
 class _ProductFn(torch.autograd.Function):
@@ -2118,8 +2112,8 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
 
     Sums are fp32 and the epilogue is applied to them before the one rounding to the result's type.  fp32 operands are cut into
     three bf16 pieces, which loses nothing, but an operand that is not finite gives NaN.  Results are the same from run to
-    run.  For the backward pass the pre-activation is kept in x's type; the gradient at it is rounded to x's type before the
-    two products that need it, as the matrix instruction takes it.  Differentiable to any order: the first-order backward
+    run.  For the backward pass the pre-activation is kept in x's type (layers of at most 64 x 64 form it again); the gradient
+    at it is rounded to x's type before the two products that need it, as the matrix instruction takes it.  Differentiable to any order: the first-order backward
     is fused, a backward that is itself differentiated (`create_graph=True`) goes through torch's activations and this
     kernel's products."""
     _floats(x, "x")

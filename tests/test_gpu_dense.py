@@ -1,4 +1,4 @@
-"""-m gpu: ops.dense (tfc_dense, tfc_dense_dz) against the formula in 64 bits.
+"""-m gpu: ops.dense (tfc_dense, tfc_dense_bwd) against the formula in 64 bits.
 
 Tolerances are bounds on the kernels' own roundings, u = 2^-24 and h half a step of the tensors' type.  A sum of k products in
 fp32: fp32 operands lose at most 2^-24 |a b| of a product (the dropped pieces: three below 2^-24 each, 3 u), and every matrix
@@ -122,7 +122,7 @@ def test_activations(device, dt, act):
 
 
 @pytest.mark.parametrize("dt", TYPES)
-@pytest.mark.parametrize("m,k,n", [(4000, 200, 1100), (5000, 64, 64), (40000, 33, 70), (2048, 700, 2048), (4100, 300, 4109)])
+@pytest.mark.parametrize("m,k,n", [(4000, 200, 1100), (5000, 64, 64), (40000, 33, 70), (2048, 700, 2048), (4100, 300, 4109), (70003, 61, 64)])
 def test_large(device, dt, m, k, n):
     """Every tile, one and many parts of the contraction (the weight's gradient sums over m)."""
     _check(*_inputs(m, k, n, dt, m + n, device), "silu", 1 / math.sqrt(k))
@@ -321,5 +321,13 @@ def test_refusals(device):
     assert L.tfc_dense(make(a_along_k=0, b_along_k=1), None, 0, None) == -2
     assert L.tfc_dense(make(m=64, n=64, k=1 << 20, ldc=64), None, 0, None) == -1 and b"workspace" in L.tfc_last_error()
     assert L.tfc_dense(None, None, 0, None) == -1
-    assert L.tfc_dense_dz(c.data_ptr(), None, 3, 4, 0, 2, 1.0, c.data_ptr(), None, None, 0, None) == -1  # an activation without z
-    assert L.tfc_dense_dz(c.data_ptr(), c.data_ptr(), 3, 4, 0, 2, 1.0, None, c.data_ptr(), None, 0, None) == -1
+    g = torch.zeros(3, 4, device=device)
+    bwd = lambda **kw: _lib.DenseBwdDesc(**{**dict(m=3, n=4, k=80, x=x.data_ptr(), ldx=0, w=w.data_ptr(), ldw=0, dy=g.data_ptr(),  # noqa: E731
+                                                   db=c.data_ptr(), alpha=1.0, act_cst=1.0, act=2, dtype=0), **kw})
+    ws = torch.zeros(1 << 16, device=device)
+    assert L.tfc_dense_bwd(bwd(), ws.data_ptr(), ws.numel(), None) == -1 and b"needs z" in L.tfc_last_error()
+    assert L.tfc_dense_bwd(bwd(z=g.data_ptr()), None, 0, None) == -1 and b"workspace" in L.tfc_last_error()
+    for bad in (dict(dtype=9), dict(act=-1), dict(n=-1), dict(dy=None), dict(ldx=-1)):
+        assert L.tfc_dense_bwd(bwd(z=g.data_ptr(), **bad), ws.data_ptr(), ws.numel(), None) == -1, bad
+    assert L.tfc_dense_bwd(bwd(db=None), None, 0, None) == 0  # nothing asked for
+    assert L.tfc_dense_keeps_z(64, 64, 2) == 0 and L.tfc_dense_keeps_z(65, 64, 2) == 1 and L.tfc_dense_keeps_z(65, 64, 0) == 0
