@@ -1915,14 +1915,19 @@ def _on(device: torch.device):
     return _AS_IS if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
+def _at(t: Optional[torch.Tensor]):  # (a plain address: what ctypes converts fastest)
+    return None if t is None else t.data_ptr()
+
+
 def _layer_norm_run(x, w, b, eps: float, keep: bool):
     """(y, stats): rows of a contiguous [rows, d] tensor; `keep`: stats [2, rows] holds the mean and 1 / deviation of every row."""
     rows, d = x.shape
     y = torch.empty_like(x)
     stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
+    mean = _at(stats)
     with _on(x.device):
-        _lib.check(_lib.lib().tfc_layer_norm_fwd(_ptr(x), _ptr(w), _ptr(b), rows, d, eps, _dtype_codes[x.dtype], _ptr(y), _ptr(stats),
-                                                 _ptr(stats, rows) if keep else None, _stream()))
+        _lib.check(_lib.lib().tfc_layer_norm_fwd(x.data_ptr(), _at(w), _at(b), rows, d, eps, _dtype_codes[x.dtype], y.data_ptr(), mean,
+                                                 mean + 4 * rows if keep else None, _stream()))
     return y, stats
 
 
@@ -1947,12 +1952,14 @@ class _LayerNormFn(torch.autograd.Function):
         db = torch.empty_like(b) if need[2] else None
         L = _lib.lib()
         dt = _dtype_codes[x.dtype]
+        mean = stats.data_ptr()
         with _on(x.device):
-            ws = None
+            floats, ws = 0, None
             if need[1] or need[2]:
-                ws = torch.empty(int(L.tfc_layer_norm_bwd_workspace_floats(rows, d, dt)), dtype=torch.float32, device=x.device)
-            _lib.check(L.tfc_layer_norm_bwd(_ptr(g), _ptr(x), _ptr(w), _ptr(stats), _ptr(stats, rows), rows, d, dt, _ptr(dx), _ptr(dw),
-                                            _ptr(db), _ptr(ws), ws.numel() if ws is not None else 0, _stream()))
+                floats = L.tfc_layer_norm_bwd_workspace_floats(rows, d, dt)
+                ws = torch.empty(floats, dtype=torch.float32, device=x.device)
+            _lib.check(L.tfc_layer_norm_bwd(g.data_ptr(), x.data_ptr(), _at(w), mean, mean + 4 * rows, rows, d, dt, _at(dx), _at(dw), _at(db),
+                                            _at(ws), floats, _stream()))
         return dx, dw, db, None
 
 
@@ -1990,12 +1997,12 @@ def layer_norm(x, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Te
             _floats(t, name, x)
             if t.shape != (d,):
                 raise ValueError(f"layer_norm: `{name}` must have shape ({d},), got {tuple(t.shape)}")
-    rows, w, b = _tracked(x.reshape(-1, d)), _tracked(weight), _tracked(bias)
+    rows, w, b = _tracked(x if x.dim() == 2 else x.reshape(-1, d)), _tracked(weight), _tracked(bias)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
         y = _LayerNormFn.apply(rows, w, b, float(eps))
     else:
         y = _layer_norm_run(rows, w, b, float(eps), False)[0]
-    return y.reshape(x.shape)
+    return y if x.dim() == 2 else y.reshape(x.shape)
 
 
 def _operand(t: torch.Tensor):
@@ -2020,13 +2027,12 @@ def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0,
     z = torch.empty_like(c) if keep_z else None
     L = _lib.lib()
     dt = _dtype_codes[a.dtype]
-    d = _lib.DenseDesc(m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, c.data_ptr(), max(n, 1), None if bias is None else bias.data_ptr(),
-                       None if residual is None else residual.data_ptr(), 0 if residual is None else max(n, 1),
-                       None if z is None else z.data_ptr(), alpha, cst, act, dt, a_along_k, not along_n)
+    d = _lib.DenseDesc(m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, c.data_ptr(), max(n, 1), _at(bias), _at(residual), max(n, 1), _at(z),
+                       alpha, cst, act, dt, a_along_k, not along_n)
     with _on(a.device):
-        need = int(L.tfc_dense_workspace_floats(m, n, k, dt))
-        ws = torch.empty(need, dtype=torch.float32, device=a.device) if need else None
-        _lib.check(L.tfc_dense(C.byref(d), _ptr(ws), need, _stream()))
+        floats = L.tfc_dense_workspace_floats(m, n, k, dt)
+        ws = torch.empty(floats, dtype=torch.float32, device=a.device) if floats else None
+        _lib.check(L.tfc_dense(C.byref(d), _at(ws), floats, _stream()))
     return c, z
 
 
@@ -2040,15 +2046,14 @@ def _dense_bwd_run(g, x, w, b, z, act: int, alpha: float, cst: float, need):
     dx = new(m, k) if need[0] else None
     dw = (new(k, n) if along_n else new(n, k)) if need[1] else None
     db = new(n) if need[2] else None
-    at = lambda t: None if t is None else t.data_ptr()  # noqa: E731
     L = _lib.lib()
     dt = _dtype_codes[g.dtype]
-    d = _lib.DenseBwdDesc(m, n, k, x.data_ptr(), ldx, w.data_ptr(), ldw, at(b), at(z), g.data_ptr(), at(dx), at(dw), at(db), alpha, cst,
-                          act, dt, not along_n)
+    d = _lib.DenseBwdDesc(m, n, k, x.data_ptr(), ldx, w.data_ptr(), ldw, _at(b), _at(z), g.data_ptr(), _at(dx), _at(dw), _at(db), alpha,
+                          cst, act, dt, not along_n)
     with _on(g.device):
-        floats = int(L.tfc_dense_bwd_workspace_floats(m, n, k, dt, act))
+        floats = L.tfc_dense_bwd_workspace_floats(m, n, k, dt, act)
         ws = torch.empty(floats, dtype=torch.float32, device=g.device) if floats else None
-        _lib.check(L.tfc_dense_bwd(C.byref(d), _ptr(ws), floats, _stream()))
+        _lib.check(L.tfc_dense_bwd(C.byref(d), _at(ws), floats, _stream()))
     return dx, (dw if along_n or dw is None else dw.t()), db
 
 
@@ -2131,17 +2136,18 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
         if bias.shape != (n,):
             raise ValueError(f"dense: `bias` must have shape ({n},), got {tuple(bias.shape)}")
         bias = _tracked(bias)
-    rows = x.reshape(math.prod(x.shape[:-1]), k)
+    flat = x.dim() == 2
+    rows = x if flat else x.reshape(math.prod(x.shape[:-1]), k)
     if k > 1 and rows.stride(1) != 1:
         rows = rows.contiguous()
     if residual is not None:
         _floats(residual, "residual", x)
         if residual.shape != shape:
             raise ValueError(f"dense: `residual` must have shape {shape}, got {tuple(residual.shape)}")
-        residual = _tracked(residual.reshape(rows.shape[0], n))
+        residual = _tracked(residual if flat else residual.reshape(rows.shape[0], n))
     args = _lib.DENSE_ACT[act], float(alpha), float(act_cst)
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
         y = _DenseFn.apply(rows, weight, bias, residual, *args)
     else:
         y = _dense_run(rows, weight, bias, residual, *args)[0]
-    return y.reshape(shape)
+    return y if flat else y.reshape(shape)
