@@ -130,27 +130,71 @@ __global__ __launch_bounds__(1024) void tfc_adamw_begin_kernel(const Group g, co
 }
 
 // ---- e4m3 codes
-__device__ __forceinline__ bool finite(float x) { return (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u; }
+constexpr uint32_t INF_BITS = 0x7F800000u;
 
-// Scale exponent (biased) of a block whose largest finite magnitude is `top`: top 2^-(e - 127) in [128, 256).
-__device__ __forceinline__ int scale_exponent(float top) {
-    const int e = (int)(__float_as_uint(top) >> 23) - 7;
+// Largest of 64 lanes' numbers, in every lane.
+__device__ __forceinline__ uint32_t wave_max(uint32_t v) {
+#define TFC_MAX_STEP(CTRL, ROWS)                                                                             \
+    {                                                                                                        \
+        const uint32_t o = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);         \
+        v = v > o ? v : o;                                                                                   \
+    }
+    TFC_MAX_STEP(0xB1, 0xF)   // quad_perm [1,0,3,2]
+    TFC_MAX_STEP(0x4E, 0xF)   // quad_perm [2,3,0,1]
+    TFC_MAX_STEP(0x141, 0xF)  // row_half_mirror
+    TFC_MAX_STEP(0x140, 0xF)  // row_mirror
+    TFC_MAX_STEP(0x142, 0xA)  // row_bcast15 -> rows 1, 3
+    TFC_MAX_STEP(0x143, 0xC)  // row_bcast31 -> rows 2, 3
+#undef TFC_MAX_STEP
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
+}
+
+// Scale exponent (biased) of a block whose largest finite magnitude has these bits: magnitude 2^-(e - 127) in [128, 256).
+__device__ __forceinline__ int scale_exponent(uint32_t top) {
+    const int e = (int)(top >> 23) - 7;
     return e < 1 ? 1 : e;
 }
-__device__ __forceinline__ uint32_t to_code(float x, float inv_scale, uint32_t r16, bool keep_nonzero) {
-    const float a = fabsf(x) * inv_scale;
-    const bool low = a < 0x1p-6f;  // the codes' subnormals: the same spacing as the binade above them
-    const float b = low ? a + 0x1p-6f : a;
-    uint32_t c = ((__float_as_uint(b) + (r16 << 4)) >> 20) - (low ? 968u : 960u);
-    if (keep_nonzero && c == 0 && x > 0.f) c = 1;
-    if (!finite(x)) c = 0x7F;
-    return c | (x < 0.f ? 0x80u : 0u);
+
+// Four values to codes and their block's scale.  Rounding up or down at random is the conversion instruction's own: it adds the
+// upper 20 of the 32 random bits to what is dropped (16 bits of randomness here, the others zero).
+template <bool ROOT>
+__device__ __forceinline__ uint32_t to_codes(const float (&x)[4], const uint32_t (&random)[4], int& e) {
+    uint32_t top = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) top = max(top, __float_as_uint(x[j]) & 0x7FFFFFFFu);
+    top = wave_max(top);
+    const bool odd = top >= INF_BITS;  // (the same in all lanes) something is not finite: it counts for nothing
+    if (odd) {
+        top = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t b = __float_as_uint(x[j]) & 0x7FFFFFFFu;
+            top = max(top, b < INF_BITS ? b : 0u);
+        }
+        top = wave_max(top);
+    }
+    e = scale_exponent(top);
+    const float inv = __uint_as_float((uint32_t)(254 - e) << 23);
+    int w = 0;
+#define TFC_TO_CODE(J)                                                                                       \
+    {                                                                                                        \
+        float y = x[J] * inv;                                                                                \
+        if (ROOT) y = x[J] > 0.f ? fmaxf(y, 0x1p-9f) : 0.f; /* a root that is not zero does not become zero */ \
+        w = __builtin_amdgcn_cvt_sr_fp8_f32(y, random[J], w, J);                                             \
+    }
+    TFC_TO_CODE(0) TFC_TO_CODE(1) TFC_TO_CODE(2) TFC_TO_CODE(3)
+#undef TFC_TO_CODE
+    if (odd) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if ((__float_as_uint(x[j]) & INF_BITS) == INF_BITS) w = (int)(((uint32_t)w & ~(0xFFu << (8 * j))) | (0x7Fu << (8 * j)));
+    }
+    return (uint32_t)w;
 }
 
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
-    return v;
+__device__ __forceinline__ void from_codes(uint32_t w, float scale, float (&x)[4]) {
+    const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, false), hi = __builtin_amdgcn_cvt_pk_f32_fp8((int)w, true);
+    x[0] = lo[0] * scale, x[1] = lo[1] * scale, x[2] = hi[0] * scale, x[3] = hi[1] * scale;
 }
 
 template <class T, int BITS>
@@ -178,13 +222,8 @@ __global__ __launch_bounds__(256) void tfc_adamw_kernel(const Group g, const Ten
         } else {
             mc = (uint8_t*)g.t[k].m + at;  // (whole blocks: the padding behind n holds zeros)
             vc = (uint8_t*)g.t[k].v + at;
-            const uint32_t mw = *(const uint32_t*)mc, vw = *(const uint32_t*)vc;
-            const float ms = __uint_as_float((uint32_t)g.t[k].m_scale[blk / QBLOCK] << 23);
-            const float vs = __uint_as_float((uint32_t)g.t[k].v_scale[blk / QBLOCK] << 23);
-            m[0] = __builtin_amdgcn_cvt_f32_fp8(mw, 0) * ms, m[1] = __builtin_amdgcn_cvt_f32_fp8(mw, 1) * ms;
-            m[2] = __builtin_amdgcn_cvt_f32_fp8(mw, 2) * ms, m[3] = __builtin_amdgcn_cvt_f32_fp8(mw, 3) * ms;
-            r[0] = __builtin_amdgcn_cvt_f32_fp8(vw, 0) * vs, r[1] = __builtin_amdgcn_cvt_f32_fp8(vw, 1) * vs;
-            r[2] = __builtin_amdgcn_cvt_f32_fp8(vw, 2) * vs, r[3] = __builtin_amdgcn_cvt_f32_fp8(vw, 3) * vs;
+            from_codes(*(const uint32_t*)mc, __uint_as_float((uint32_t)g.t[k].m_scale[blk / QBLOCK] << 23), m);
+            from_codes(*(const uint32_t*)vc, __uint_as_float((uint32_t)g.t[k].v_scale[blk / QBLOCK] << 23), r);
 #pragma unroll
             for (int j = 0; j < 4; ++j) v[j] = r[j] * r[j];
         }
@@ -201,24 +240,21 @@ __global__ __launch_bounds__(256) void tfc_adamw_kernel(const Group g, const Ten
             tfc_store_f<float, 4>((float*)g.t[k].m + at, left, m);
             tfc_store_f<float, 4>((float*)g.t[k].v + at, left, v);
         } else {
-            float tm = 0.f, tv = 0.f;
+            if (left < 4) {  // the padding stays zero
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                tm = fmaxf(tm, finite(m[j]) ? fabsf(m[j]) : 0.f);
-                tv = fmaxf(tv, finite(r[j]) ? r[j] : 0.f);
+                for (int j = 0; j < 4; ++j)
+                    if (j >= left) m[j] = r[j] = 0.f;
             }
-            const int em = scale_exponent(wave_max(tm)), ev = scale_exponent(wave_max(tv));
-            const float im = __uint_as_float((uint32_t)(254 - em) << 23), iv = __uint_as_float((uint32_t)(254 - ev) << 23);
-            uint32_t mw = 0, vw = 0;
+            uint32_t hm[4], hv[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
                 const uint32_t h = mixed((uint32_t)(at + j) ^ st.key ^ ((uint32_t)((at + j) >> 32) * 0x2545F491u));
-                const bool in = j < left;  // the padding stays zero
-                mw |= (in ? to_code(m[j], im, h & 0xFFFFu, false) : 0u) << (8 * j);
-                vw |= (in ? to_code(r[j], iv, h >> 16, true) : 0u) << (8 * j);
+                hm[j] = h << 16;
+                hv[j] = h & 0xFFFF0000u;
             }
-            *(uint32_t*)mc = mw;
-            *(uint32_t*)vc = vw;
+            int em, ev;
+            *(uint32_t*)mc = to_codes<false>(m, hm, em);
+            *(uint32_t*)vc = to_codes<true>(r, hv, ev);
             if (lane == 0) {
                 g.t[k].m_scale[blk / QBLOCK] = (uint8_t)em;
                 g.t[k].v_scale[blk / QBLOCK] = (uint8_t)ev;

@@ -31,6 +31,7 @@ class _Table:
     def __init__(self, params, states, indexes, bits: int):
         self.params = params
         self.at = [p.data_ptr() for p in params]
+        self.sizes = [p.numel() for p in params]
         self.keep = states
         self.rows = (_lib.AdamwTensor * len(params))()
         names = list(_STATE[bits])
@@ -151,37 +152,47 @@ class AdamW(torch.optim.Optimizer):
     # ---- step
     def _gather(self):
         """[(group, table, dtype)] of the parameters that have a gradient, one entry for each (group, device, dtype)."""
-        calls, index = [], 0
+        calls, first = [], 0
         for gi, g in enumerate(self.param_groups):
-            sets = {}
-            for p in g["params"]:
-                if p.grad is not None:
-                    sets.setdefault((p.device, p.dtype), []).append((p, index))
-                index += 1
             self._check_group(g)  # (schedulers and users write to groups)
-            for (device, dtype), items in sets.items():
+            for (device, dtype), items in self._sets(gi, g["params"]):
+                params = [p for p, _ in items if p.grad is not None]
+                if not params:
+                    continue
                 if isinstance(g["lr"], torch.Tensor) and g["lr"].device != device:
                     raise RuntimeError(f"AdamW: the lr tensor is on {g['lr'].device}, the parameters on {device}")
-                calls.append((g, device, dtype, self._table(gi, device, dtype, items)))
+                calls.append((g, device, dtype, self._table(gi, device, dtype, items, params, first)))
+            first += len(g["params"])
         return calls
 
-    def _table(self, gi, device, dtype, items) -> _Table:
-        key = (gi, device, dtype)
-        table = self._tables.get(key)
-        if (table is None or len(table.params) != len(items)
-                or any(p is not q or p.data_ptr() != a for (p, _), q, a in zip(items, table.params, table.at))
-                or any(self.state[p] is not st for (p, _), st in zip(items, table.keep))):
-            if device.type != "cuda":
-                raise RuntimeError(f"matten_amd: parameters must live on a ROCm device (no CPU fallback exists); got {device}")
-            for p, _ in items:
-                if not p.is_contiguous():
-                    raise ValueError("AdamW: parameters must be contiguous")
-                if not self.state[p]:
-                    if torch.cuda.is_current_stream_capturing():
-                        raise RuntimeError("AdamW: the first step allocates the state and cannot be captured; run one step before the capture")
-                    self.state[p].update(self._new_state(p))
-            table = _Table([p for p, _ in items], [self.state[p] for p, _ in items], [i for _, i in items], self.state_bits)
-            self._tables[key] = table
+    @staticmethod
+    def _sets(gi, params):
+        """Parameters of a group by device and dtype, with their place in the group."""
+        sets = {}
+        for i, p in enumerate(params):
+            sets.setdefault((p.device, p.dtype), []).append((p, i))
+        return sets.items()
+
+    def _table(self, gi, device, dtype, items, params, first) -> _Table:
+        table = self._tables.get((gi, device, dtype))
+        state = self.state
+        if table is not None and len(table.params) == len(params):
+            for p, q, a, st in zip(params, table.params, table.at, table.keep):
+                if p is not q or p.data_ptr() != a or state.get(p) is not st:
+                    break
+            else:
+                return table
+        if device.type != "cuda":
+            raise RuntimeError(f"matten_amd: parameters must live on a ROCm device (no CPU fallback exists); got {device}")
+        for p in params:
+            if not p.is_contiguous():
+                raise ValueError("AdamW: parameters must be contiguous")
+            if not state[p]:
+                if torch.cuda.is_current_stream_capturing():
+                    raise RuntimeError("AdamW: the first step allocates the state and cannot be captured; run one step before the capture")
+                state[p].update(self._new_state(p))
+        indexes = [first + i for p, i in items if p.grad is not None]
+        table = self._tables[gi, device, dtype] = _Table(params, [state[p] for p in params], indexes, self.state_bits)
         return table
 
     @torch.no_grad()
@@ -193,9 +204,10 @@ class AdamW(torch.optim.Optimizer):
         calls = self._gather()
         copies = []  # gradients that are not contiguous
         for _, device, dtype, table in calls:
-            for row, p in zip(table.rows, table.params):
+            at = device.index
+            for row, p, n in zip(table.rows, table.params, table.sizes):
                 g = p.grad
-                if g.dtype != dtype or g.device != device or g.layout != torch.strided or g.shape != p.shape:
+                if g.dtype != dtype or g.layout != torch.strided or g.get_device() != at or g.numel() != n:
                     raise RuntimeError(f"AdamW: a gradient must be a dense {dtype} tensor of shape {tuple(p.shape)} on {device}; got "
                                        f"{g.dtype}, {tuple(g.shape)}, {g.layout} on {g.device}")
                 if not g.is_contiguous():

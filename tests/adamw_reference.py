@@ -34,12 +34,12 @@ def encode(x, r16, keep_nonzero):
         scales[b] = e
     inv = torch.ldexp(torch.ones(blocks), 127 - scales.to(torch.int32)).float()
     a = (mag * inv[:, None]).view(-1)[:n]
+    # the 20 bits that are dropped, plus the random ones, carry into the code or do not; below 2^-6 codes are 2^-9 apart
     low = a < 2.0**-6
-    bits = torch.where(low, a + 2.0**-6, a).view(torch.int32).long()
-    c = ((bits + (r16 << 4)) >> 20) - torch.where(low, 968, 960)
+    c = torch.where(low, ((a.double() * 2.0**29).long() + (r16 << 4)) >> 20, ((a.view(torch.int32).long() + (r16 << 4)) >> 20) - 960)
     if keep_nonzero:
         c = torch.where((c == 0) & (x > 0), torch.ones_like(c), c)
-    c = torch.where(fine, c, torch.full_like(c, 127)) | ((x < 0).long() << 7)
+    c = torch.where(fine, c | ((x < 0).long() << 7), torch.full_like(c, 127))
     codes[:n] = c.to(torch.uint8)
     return codes, scales
 
