@@ -9,7 +9,11 @@ stream's fork and join included) the step replays with a single host call.  The 
 (its step is Lightning's eager loop, eigenn/model/model.py:239-327).
 
 Rules for the captured function: inputs and outputs live in tensors that keep their addresses (copy new
-values into them between replays), no host synchronisation inside (`.item()`, data-dependent shapes).
+values into them between replays), no host synchronisation inside (`.item()`, data-dependent shapes).  A backward pass inside
+starts from gradients that are None, and a leaf other than a parameter that collects a gradient is made inside: autograd
+accumulates into a gradient that is there on the stream where an earlier graph of the same leaf was recorded, and while that
+graph lives (the warm-up's may) this breaks the capture and ends the process.  An optimizer step may be part of the function
+(matten_amd.optim.AdamW); the warm-up calls step it too.
 
 What may change between replays depends on `rebuild_topology`:
 

@@ -11,6 +11,7 @@ from typing import Any, Dict
 from . import keys as DataKey
 from .nn.edge_encoding import RadialBasisEdgeEncoding, SphericalHarmonicEdgeAttrs
 from .nn.embedding import SpeciesEmbedding
+from .nn.mlp import NodewiseMLP
 from .nn.nodewise import NodewiseLinear, NodewiseReduce, NodewiseSelect
 from .nn.point_conv import PointConvMessagePassing
 from .nn.readout import CartesianTensor, IrrepsToCartesianTensor
@@ -46,9 +47,14 @@ def _encoder_and_conv_layers(hparams: Dict[str, Any], dataset_hparams: Dict[str,
 
 
 def create_energy_model(hparams: Dict[str, Any], dataset_hparams: Dict[str, Any]):
-    """... -> NodewiseLinear(hidden) -> NodewiseLinear(1x0e -> atomic_energy) -> NodewiseReduce -> total_energy"""
+    """... -> NodewiseLinear(hidden) -> NodewiseLinear(1x0e -> atomic_energy) -> NodewiseReduce -> total_energy.
+
+    `output_mlp` (optional, not in the reference's hparams): {"hidden": int, "num_blocks": int, "activation": str}, any of them; puts
+    a NodewiseMLP on the hidden invariants, between the two linear maps."""
     layers = _encoder_and_conv_layers(hparams, dataset_hparams)
     layers["conv_to_output_hidden"] = (NodewiseLinear, {"irreps_out": hparams["conv_to_output_hidden_irreps_out"]})
+    if hparams.get("output_mlp") is not None:
+        layers["output_mlp"] = (NodewiseMLP, dict(hparams["output_mlp"]))
     layers["output_hidden_to_scalar"] = (NodewiseLinear, {"irreps_out": "1x0e", "out_field": DataKey.PER_ATOM_ENERGY})
     reduce = hparams["reduce"]
     layers[f"total_energy_{reduce}"] = (NodewiseReduce, {"reduce": reduce, "field": DataKey.PER_ATOM_ENERGY, "out_field": OUT_FIELD_ENERGY})

@@ -1310,8 +1310,12 @@ def _radial_mlp_composite(x, ws, act_cst: float, act_id: Optional[int] = None):
 
 def radial_mlp_general(x, weights: Sequence[torch.Tensor], act_cst: float, act_id: int):
     """FullyConnectedNet with any of the gate kernel's activations (eigenn/nn/utils.py:182 `mlp_activation`), layer by
-    layer: dense product, then the activation as a one-segment gate."""
-    return _radial_mlp_composite(x, list(weights), act_cst, act_id)
+    layer: the dense product with the activation in its epilogue."""
+    name = next(k for k, v in _lib.ACT.items() if v == act_id)
+    for i, w in enumerate(weights):
+        last = i == len(weights) - 1
+        x = dense(x, w, act="identity" if last else name, alpha=1.0 / math.sqrt(w.shape[0]), act_cst=1.0 if last else act_cst)
+    return x
 
 
 _SELF_ORDERINGS: "dict[tuple, tuple]" = _tensor_cache()

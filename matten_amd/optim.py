@@ -63,7 +63,8 @@ class AdamW(torch.optim.Optimizer):
 
     Parameters and gradients are contiguous and on a ROCm device (gradients that are not contiguous are copied); a sparse gradient
     raises.  A parameter without a gradient is skipped and its step count stands.  The first step allocates the state and
-    therefore must not be inside a graph capture."""
+    therefore must not be inside a graph capture; a captured step drops its gradients (`zero_grad()`, set to None) rather than
+    zeroing them, as matten_amd.graphs asks of every captured backward pass."""
 
     def __init__(self, params: Iterable, lr=1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2, *, state_bits: int = 32,
                  max_grad_norm: Optional[float] = None, seed: int = 0):
