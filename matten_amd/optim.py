@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from operator import is_
 from typing import Iterable, Optional
 
 import torch
@@ -28,11 +29,12 @@ _STATE = {  # state entry -> dtype, by the width of the moments ("step" besides)
 class _Table:
     """The descriptors of the tensors one call steps: everything but the gradients' addresses is set once."""
 
-    def __init__(self, params, states, indexes, bits: int):
-        self.params = params
+    def __init__(self, group, params, states, indexes, bits: int):
+        self.group, self.params, self.states = group, params, states
+        self.device, self.dtype = params[0].device, params[0].dtype
+        self.entries = [tuple(st.values()) for st in states]  # (alive as long as their addresses are used)
         self.at = [p.data_ptr() for p in params]
         self.sizes = [p.numel() for p in params]
-        self.keep = states
         self.rows = (_lib.AdamwTensor * len(params))()
         names = list(_STATE[bits])
         for row, p, st, i in zip(self.rows, params, states, indexes):
@@ -41,6 +43,13 @@ class _Table:
                 row.m, row.v = (st[k].data_ptr() for k in names)
             else:
                 row.m, row.m_scale, row.v, row.v_scale = (st[k].data_ptr() for k in names)
+
+    def holds(self, state) -> bool:
+        """Whether parameters and state still lie where the descriptors say, every parameter with a gradient."""
+        for p, at, st, entries in zip(self.params, self.at, self.states, self.entries):
+            if p.grad is None or p.data_ptr() != at or state.get(p) is not st or not all(map(is_, st.values(), entries)):
+                return False
+        return True
 
 
 class AdamW(torch.optim.Optimizer):
@@ -76,7 +85,7 @@ class AdamW(torch.optim.Optimizer):
         self.max_grad_norm = None if max_grad_norm is None else float(max_grad_norm)
         self.seed = int(seed) & 0xFFFFFFFF
         self.grad_norm: Optional[torch.Tensor] = None
-        self._tables = {}
+        self._tables = None  # the last step's, and the parameters it left alone
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay))
 
     def add_param_group(self, group):
@@ -140,11 +149,11 @@ class AdamW(torch.optim.Optimizer):
             new[p] = st
         super().load_state_dict({"state": {}, "param_groups": state_dict["param_groups"]})  # (would cast the moments)
         self.state.update(new)
-        self._tables = {}
+        self._tables = None
 
     def __setstate__(self, state):
         super().__setstate__(state)
-        self._tables = {}
+        self._tables = None
 
     def __getstate__(self):
         return {**super().__getstate__(), "state_bits": self.state_bits, "max_grad_norm": self.max_grad_norm, "seed": self.seed,
@@ -152,49 +161,39 @@ class AdamW(torch.optim.Optimizer):
 
     # ---- step
     def _gather(self):
-        """[(group, table, dtype)] of the parameters that have a gradient, one entry for each (group, device, dtype)."""
-        calls, first = [], 0
-        for gi, g in enumerate(self.param_groups):
+        """Tables of the parameters that have a gradient, one for each (group, device, dtype)."""
+        for g in self.param_groups:
             self._check_group(g)  # (schedulers and users write to groups)
-            for (device, dtype), items in self._sets(gi, g["params"]):
-                params = [p for p, _ in items if p.grad is not None]
-                if not params:
-                    continue
-                if isinstance(g["lr"], torch.Tensor) and g["lr"].device != device:
-                    raise RuntimeError(f"AdamW: the lr tensor is on {g['lr'].device}, the parameters on {device}")
-                calls.append((g, device, dtype, self._table(gi, device, dtype, items, params, first)))
+        if self._tables is not None:
+            tables, rest, groups = self._tables
+            if (groups == [(id(g), len(g["params"])) for g in self.param_groups] and all(t.holds(self.state) for t in tables)
+                    and all(p.grad is None for p in rest)):
+                return tables
+        tables, rest, first = [], [], 0
+        for g in self.param_groups:
+            sets = {}
+            for i, p in enumerate(g["params"]):
+                if p.grad is None:
+                    rest.append(p)
+                else:
+                    sets.setdefault((p.device, p.dtype), []).append((p, first + i))
             first += len(g["params"])
-        return calls
+            for (device, _), items in sets.items():
+                tables.append(self._table(g, device, [p for p, _ in items], [i for _, i in items]))
+        self._tables = tables, rest, [(id(g), len(g["params"])) for g in self.param_groups]
+        return tables
 
-    @staticmethod
-    def _sets(gi, params):
-        """Parameters of a group by device and dtype, with their place in the group."""
-        sets = {}
-        for i, p in enumerate(params):
-            sets.setdefault((p.device, p.dtype), []).append((p, i))
-        return sets.items()
-
-    def _table(self, gi, device, dtype, items, params, first) -> _Table:
-        table = self._tables.get((gi, device, dtype))
-        state = self.state
-        if table is not None and len(table.params) == len(params):
-            for p, q, a, st in zip(params, table.params, table.at, table.keep):
-                if p is not q or p.data_ptr() != a or state.get(p) is not st:
-                    break
-            else:
-                return table
+    def _table(self, group, device, params, indexes) -> _Table:
         if device.type != "cuda":
             raise RuntimeError(f"matten_amd: parameters must live on a ROCm device (no CPU fallback exists); got {device}")
         for p in params:
             if not p.is_contiguous():
                 raise ValueError("AdamW: parameters must be contiguous")
-            if not state[p]:
+            if not self.state[p]:
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("AdamW: the first step allocates the state and cannot be captured; run one step before the capture")
-                state[p].update(self._new_state(p))
-        indexes = [first + i for p, i in items if p.grad is not None]
-        table = self._tables[gi, device, dtype] = _Table(params, [state[p] for p in params], indexes, self.state_bits)
-        return table
+                self.state[p].update(self._new_state(p))
+        return _Table(group, params, [self.state[p] for p in params], indexes, self.state_bits)
 
     @torch.no_grad()
     def step(self, closure=None):
@@ -202,14 +201,17 @@ class AdamW(torch.optim.Optimizer):
         if closure is not None:
             with torch.enable_grad():
                 loss = closure()
-        calls = self._gather()
+        tables = self._gather()
         copies = []  # gradients that are not contiguous
-        for _, device, dtype, table in calls:
-            at = device.index
-            for row, p, n in zip(table.rows, table.params, table.sizes):
+        for t in tables:
+            dtype, at = t.dtype, t.device.index
+            lr = t.group["lr"]
+            if isinstance(lr, torch.Tensor) and lr.device != t.device:
+                raise RuntimeError(f"AdamW: the lr tensor is on {lr.device}, the parameters on {t.device}")
+            for row, p, n in zip(t.rows, t.params, t.sizes):
                 g = p.grad
                 if g.dtype != dtype or g.layout != torch.strided or g.get_device() != at or g.numel() != n:
-                    raise RuntimeError(f"AdamW: a gradient must be a dense {dtype} tensor of shape {tuple(p.shape)} on {device}; got "
+                    raise RuntimeError(f"AdamW: a gradient must be a dense {dtype} tensor of shape {tuple(p.shape)} on {t.device}; got "
                                        f"{g.dtype}, {tuple(g.shape)}, {g.layout} on {g.device}")
                 if not g.is_contiguous():
                     g = g.contiguous()
@@ -218,29 +220,30 @@ class AdamW(torch.optim.Optimizer):
         L = _lib.lib()
         partials, n_partials = None, 0
         self.grad_norm = None
-        if self.max_grad_norm is not None and calls:
-            device = calls[0][1]
-            if any(c[1] != device for c in calls):
+        if self.max_grad_norm is not None and tables:
+            device = tables[0].device
+            if any(t.device != device for t in tables):
                 raise RuntimeError("AdamW: max_grad_norm needs all parameters on one device")
-            counts = [int(L.tfc_grad_sumsq_partials(t.rows, len(t.rows))) for _, _, _, t in calls]
+            counts = [L.tfc_grad_sumsq_partials(t.rows, len(t.rows)) for t in tables]
             n_partials = sum(counts)
             with ops._on(device):
-                partials = torch.empty(max(n_partials, 1), dtype=torch.float64, device=device)
                 self.grad_norm = torch.empty((), dtype=torch.float32, device=device) if n_partials else torch.zeros((), device=device)
-                at = 0
-                for (_, _, dtype, t), n in zip(calls, counts):
-                    _lib.check(L.tfc_grad_sumsq(t.rows, len(t.rows), ops._dtype_codes[dtype], ops._ptr(partials, at), ops._stream()))
-                    at += n
-        for g, device, dtype, t in calls:
+                partials = torch.empty(max(n_partials, 1), dtype=torch.float64, device=device)
+                at = partials.data_ptr()
+                for t, n in zip(tables, counts):
+                    _lib.check(L.tfc_grad_sumsq(t.rows, len(t.rows), ops._dtype_codes[t.dtype], at, ops._stream()))
+                    at += 8 * n
+        for t in tables:
+            g = t.group
             h = _lib.AdamwHyper(beta1=g["betas"][0], beta2=g["betas"][1], eps=g["eps"], weight_decay=g["weight_decay"],
                                 max_norm=self.max_grad_norm if n_partials else 0.0, seed=self.seed)
             if isinstance(g["lr"], torch.Tensor):
                 h.lr_device = g["lr"].data_ptr()
             else:
                 h.lr = g["lr"]
-            with ops._on(device):
-                ws = torch.empty(int(L.tfc_adamw_workspace_bytes(len(t.rows))), dtype=torch.uint8, device=device)
-                _lib.check(L.tfc_adamw_step(t.rows, len(t.rows), ops._dtype_codes[dtype], self.state_bits, C.byref(h), ops._ptr(partials),
-                                            n_partials, ops._ptr(self.grad_norm), ops._ptr(ws), ws.numel(), ops._stream()))
+            with ops._on(t.device):
+                ws = torch.empty(L.tfc_adamw_workspace_bytes(len(t.rows)), dtype=torch.uint8, device=t.device)
+                _lib.check(L.tfc_adamw_step(t.rows, len(t.rows), ops._dtype_codes[t.dtype], self.state_bits, C.byref(h), ops._at(partials),
+                                            n_partials, ops._at(self.grad_norm), ws.data_ptr(), ws.numel(), ops._stream()))
             torch.autograd.graph.increment_version(t.params)  # (written behind torch's back: saved tensors and caches see it)
         return loss

@@ -275,6 +275,41 @@ def test_state_dict(device):
             optim.AdamW(_tensors([1024, 31], torch.bfloat16, device, 9), state_bits=bits).load_state_dict(saved)
 
 
+def test_state_and_storage_that_are_replaced(device):
+    """State entries, parameters' storage and the set of gradients may change between steps: the next step works on what is there."""
+    from matten_amd import optim
+
+    params = _tensors([500, 40, 7], torch.float32, device, 14)
+    refs = [Reference(p, i, 32) for i, p in enumerate(params)]
+    opt = optim.AdamW(params)
+    for k in range(6):
+        _grads(params, 80 + k)
+        if k == 1:
+            opt.state[params[0]]["exp_avg"] = opt.state[params[0]]["exp_avg"].clone()
+        if k == 2:
+            params[1].data = params[1].detach().clone()
+        if k == 3:
+            opt.state[params[2]] = {n: t.clone() for n, t in opt.state[params[2]].items()}
+        skip = {1} if k == 4 else set()
+        for i in skip:
+            params[i].grad = None
+        junk = [torch.full((500,), 7.0, device=device) for _ in range(8)]  # whatever was let go is somebody else's now
+        opt.step()
+        for i, (p, r) in enumerate(zip(params, refs)):
+            if i not in skip:
+                r.step(p.grad)
+            _same(opt, p, r)
+        assert all(bool((j == 7.0).all()) for j in junk)
+    more = _tensors([60], torch.float32, device, 15)
+    opt.add_param_group({"params": more, "lr": 0.5})
+    refs.append(Reference(more[0], 3, 32, lr=0.5))
+    _grads(params + more, 90)
+    opt.step()
+    for p, r in zip(params + more, refs):
+        r.step(p.grad)
+        _same(opt, p, r)
+
+
 def test_schedulers_closures_and_versions(device):
     from matten_amd import optim
 
@@ -374,7 +409,7 @@ def test_refusals_on_the_device(device):
     L = _lib.lib()
     opt = optim.AdamW([p])
     opt.step()
-    t = next(iter(opt._tables.values()))
+    t = opt._tables[0][0]
     h = _lib.AdamwHyper(lr=1e-3, beta1=0.9, beta2=0.999, eps=1e-8)
     before = p.detach().clone()
     assert L.tfc_adamw_step(t.rows, 1, 0, 16, h, None, 0, None, None, 0, None) == -1
