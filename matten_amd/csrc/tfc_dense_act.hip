@@ -285,6 +285,16 @@ __device__ __forceinline__ void write_out(const Args& g, const floatx16 (&acc)[M
     }
 }
 
+// (row of tiles << 32) + column of this workgroup's tile.  Neighbouring workgroups of an XCD share its L2: they take tiles in columns of
+// GROUP (64 tiles in flight read 8 + 8 operand panels instead of 2 + 32 when they go along the rows of a wide C:
+// 16384 x 1024 x 4096, 204 -> 196 us).
+__device__ __forceinline__ long tile_of(const Args& g) {
+    constexpr unsigned GROUP = 8;
+    const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x), strip = GROUP * (unsigned)g.tiles_n;
+    const unsigned top = tile / strip * GROUP, in = tile % strip, high = min(GROUP, (unsigned)g.tiles_m - top);
+    return ((long)(top + in % high) << 32) + in / high;
+}
+
 // BM x BN tile, waves 2 x 2.  SPLIT: this workgroup's part of the contraction to g.part.
 template <class T, bool AK, bool BK, int BM, int BN, bool SPLIT>
 __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
@@ -296,12 +306,8 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
     __shared__ __attribute__((aligned(16))) uint16_t lds[LDS];
     uint16_t* la = lds;
     uint16_t* lb = lds + A::IMAGE;
-    // Neighbouring workgroups of an XCD share its L2: they take tiles in columns of GROUP (64 tiles in flight read 8 + 8 operand panels
-    // instead of 2 + 32 when they go along the rows of a wide C: its product 204 -> 196 us).
-    constexpr unsigned GROUP = 8;
-    const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x), strip = GROUP * (unsigned)g.tiles_n;
-    const unsigned top = tile / strip * GROUP, in = tile % strip, high = min(GROUP, (unsigned)g.tiles_m - top);
-    const long m0 = (long)(top + in % high) * BM, n0 = (long)(in / high) * BN;
+    const long tile = tile_of(g);
+    const long m0 = (tile >> 32) * BM, n0 = (tile & 0xFFFFFFFF) * BN;
     const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
     const long k1 = SPLIT ? (k0 + g.k_split < g.k ? k0 + g.k_split : g.k) : g.k;
     const int wave = threadIdx.x >> 6;
@@ -357,6 +363,136 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
     step(std::integral_constant<int, 0>(), 0);
     __syncthreads();
     write_out<T, MI, NI, SPLIT>(g, acc, (float*)lds + wave * corner_floats(NI), m0 + wm, n0 + wn);
+}
+
+// ------------------------------------------------------------------------------------------------ large 16-bit products
+// 256 x 256 tile of eight waves (2 x 4, 128 x 64 of C each: eight 32 x 32 products for six operand reads).  The operands of a step of
+// 32 go straight from memory to LDS, three steps ahead of the one that is multiplied (four images of 32 KB, one barrier a
+// step): what bounds the kernel above on large products is the wait for operands one step ahead, at half the matrix rate.
+// Rows of an image have no padding (a wave's 64 x 16 bytes land side by side); their 16-byte units are swizzled by which unit a lane
+// asks memory for, so that the reads meet all banks: along k, unit ^ (row / 2 % 4); along the rows, 64-byte part ^ (k % 4).
+// Operands start at multiples of 16 bytes, have strides and, along the rows, sizes of multiples of 8; the contraction is a
+// multiple of 32.  Rows behind the last one are the last one again.
+constexpr int DEEP = 256, DEEP_K = 32, DEEP_IMAGE = DEEP * DEEP_K;
+
+// 16 bytes a lane from base + off to `to` + 16 lane.  Written out, because for the transposing LDS reads the compiler cannot tell the
+// image being filled from the one being read and waits for every access of the wave; nothing is loaded into registers, and
+// the kernel's own waits (TFC_DEEP_STEP) are the ones there are.  M0 is read one state after it was set.
+__device__ __forceinline__ void memory_to_lds(const char* base, uint32_t off, uint16_t* to) {
+    const uint32_t lds = (uint32_t)tfc_uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+}
+
+template <class T, bool ALONG_K>
+struct DeepStage {
+    uint32_t off[2];  // bytes, of this lane's two accesses a step
+    const char* base;
+    long adv;
+
+    __device__ __forceinline__ void start(const Operand& o, long r0, long rows, long k0) {
+        const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, last = (int)(rows < DEEP ? rows : DEEP) - 1;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t r, k;
+            if constexpr (ALONG_K) {
+                const int row = (i * 8 + wave) * 16 + lane / 4;
+                r = min(row, last), k = ((lane & 3) ^ ((row >> 1) & 3)) * 8;
+                off[i] = 2u * (r * (uint32_t)o.ld + k);
+            } else {
+                k = (i * 8 + wave) * 2 + lane / 32;
+                r = min((int)((((lane & 31) >> 2) ^ (k & 3)) * 32 + (lane & 3) * 8), last & ~7);
+                off[i] = 2u * (k * (uint32_t)o.ld + r);
+            }
+        }
+        base = (const char*)o.p + 2 * (ALONG_K ? r0 * o.ld + k0 : k0 * o.ld + r0);
+        adv = 2 * (ALONG_K ? DEEP_K : DEEP_K * o.ld);
+    }
+    __device__ __forceinline__ void load(uint16_t* image) {
+        const int wave = tfc_uniform(threadIdx.x >> 6);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) memory_to_lds(base, off[i], image + (i * 8 + wave) * 512);
+        base += adv;
+    }
+    static __device__ __forceinline__ uintx4 fragment(const uint16_t* im, int r0, int kk) {
+        const int lane = threadIdx.x & 63;
+        if constexpr (ALONG_K) {
+            const int r = r0 + (lane & 31), u = kk / 8 + (lane >> 5);
+            return *(const uintx4*)(im + r * DEEP_K + ((u ^ ((r >> 1) & 3)) << 3));
+        }
+        const int k = kk + (lane >> 5) * 8 + ((lane & 15) >> 2), r = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
+        const uint16_t* q = im + k * DEEP + (((r >> 5) ^ (k & 3)) << 5) + (r & 31);  // (k + 4: the same swizzle)
+        typedef __attribute__((address_space(3))) shortx4* Lds;
+        struct {
+            shortx4 a, b;
+        } both = {__builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q)), __builtin_amdgcn_ds_read_tr16_b64_v4i16((Lds)(q + 4 * DEEP))};
+        return __builtin_bit_cast(uintx4, both);
+    }
+};
+
+template <class T, bool AK, bool BK, bool SPLIT>
+__global__ __launch_bounds__(512, 2) void tfc_dense_deep_kernel(const Args g) {
+    __shared__ __attribute__((aligned(16))) uint16_t s0[2 * DEEP_IMAGE], s1[2 * DEEP_IMAGE], s2[2 * DEEP_IMAGE], s3[2 * DEEP_IMAGE];
+    const long tile = tile_of(g);
+    const long m0 = (tile >> 32) * DEEP, n0 = (tile & 0xFFFFFFFF) * DEEP;
+    const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
+    const long k1 = SPLIT ? (k0 + g.k_split < g.k ? k0 + g.k_split : g.k) : g.k;
+    const int wave = threadIdx.x >> 6, wm = (wave >> 2) * 128, wn = (wave & 3) * 64;
+    floatx16 acc[4][2];
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) acc[i][j] = floatx16(0.f);
+    DeepStage<T, AK> sa;
+    DeepStage<T, BK> sb;
+    sa.start(g.a, m0, g.m - m0, k0);
+    sb.start(g.b, n0, g.n - n0, k0);
+    int ahead = (int)((k1 - k0) / DEEP_K), todo = ahead;  // steps to ask for, steps to multiply
+    auto ask = [&](uint16_t* s) {
+        if (ahead > 0) {
+            sa.load(s);
+            sb.load(s + DEEP_IMAGE);
+            --ahead;
+        }
+    };
+    auto multiply = [&](const uint16_t* s) {
+#pragma unroll
+        for (int kk = 0; kk < DEEP_K; kk += 16) {
+            uintx4 fa[4], fb[2];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) fa[i] = DeepStage<T, AK>::fragment(s, wm + 32 * i, kk);
+#pragma unroll
+            for (int j = 0; j < 2; ++j) fb[j] = DeepStage<T, BK>::fragment(s + DEEP_IMAGE, wn + 32 * j, kk);
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int j = 0; j < 2; ++j) acc[i][j] = mma(T(), fb[j], fa[i], acc[i][j]);
+        }
+        --todo;
+    };
+    // Every wave waits for its own accesses of the step in hand (at most those of the two steps behind it, four each, may be on their
+    // way) and for its reads of the image before, and then for the other waves; behind the barrier that image is free.
+#define TFC_DEEP_STEP(HERE, FREE)                                                \
+    if (todo > 2)                                                                \
+        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory"); \
+    else                                                                         \
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); \
+    ask(FREE);                                                                   \
+    multiply(HERE);                                                              \
+    if (todo == 0) break;
+    ask(s0);
+    ask(s1);
+    ask(s2);
+    while (true) {
+        TFC_DEEP_STEP(s0, s3)
+        TFC_DEEP_STEP(s1, s0)
+        TFC_DEEP_STEP(s2, s1)
+        TFC_DEEP_STEP(s3, s2)
+    }
+#undef TFC_DEEP_STEP
+    __syncthreads();
+    static_assert(2 * corner_floats(2) * 4 <= 4 * DEEP_IMAGE, "two waves' corners in an image pair");
+    uint16_t* part = (wave & 3) == 0 ? s0 : (wave & 3) == 1 ? s1 : (wave & 3) == 2 ? s2 : s3;
+    write_out<T, 4, 2, SPLIT>(g, acc, (float*)part + (wave >> 2) * corner_floats(2), m0 + wm, n0 + wn);
 }
 
 // 256 / W quads of columns x W walkers: walker w adds the parts w, w + W, ..., the walkers are joined in order.
@@ -454,11 +590,20 @@ struct Plan {
     int64_t tiles_m, tiles_n, splits, k_split;
 };
 
+// What the kernel for large products asks of sizes and of operands.
+bool deep_shape(int64_t m, int64_t n, int64_t k, int dtype) {
+    return dtype != TFC_F32 && m >= DEEP && n >= DEEP && k % DEEP_K == 0;
+}
+bool deep_operands(const tfc_dense_desc& d) {
+    return deep_shape(d.m, d.n, d.k, d.dtype) && (((uintptr_t)d.a | (uintptr_t)d.b) & 15) == 0 && d.lda % 8 == 0 && d.ldb % 8 == 0 &&
+           (d.a_along_k || d.m % 8 == 0) && (d.b_along_k || d.n % 8 == 0);
+}
+
 // Tiles: 128 x 128, or narrower ones for a narrow C (64 x 64 moves twice as many operand bytes through LDS for each product).  Where
 // the tiles alone do not put three workgroups (fp32: two, by LDS) on every CU the contraction is split, in parts of at least eight
 // steps; and where the partial tiles would not stay in the caches (over 16 MB) in parts long enough that writing and adding them
 // up takes less than half the time of the products: 1024 of k for 16 bits, 192 for fp32, whose products cost six times as much.
-Plan plan(int64_t m, int64_t n, int64_t k, int dtype) {
+Plan plan(int64_t m, int64_t n, int64_t k, int dtype, bool deep) {
     Plan p{};
     const bool wide = dtype == TFC_F32;
     const int64_t step = wide ? 32 : 64, steps = (k + step - 1) / step, want = wide ? 512 : 768;
@@ -477,6 +622,7 @@ Plan plan(int64_t m, int64_t n, int64_t k, int dtype) {
         p.splits = steps ? (steps + each - 1) / each : 1;
         return have * p.splits >= 256;
     };
+    if (deep && take(256, 256, 256)) return p;
     if (!wide && m >= 256 && n >= 128 && take(256, 128, 512) && p.tiles_m * p.tiles_n * p.splits >= 512) return p;
     if (m > 64 && n > 64 && take(128, 128, want)) return p;
     if (m > 64 && take(128, 64, want)) return p;
@@ -497,8 +643,18 @@ int launch_tile(const Args& g, const Plan& p, hipStream_t s) {
 
 template <class T, bool AK, bool BK>
 int launch_layout(const Args& g, const Plan& p, hipStream_t s) {
-    if constexpr (sizeof(T) == 2)
+    if constexpr (sizeof(T) == 2) {
+        if (p.bn == 256) {
+            const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
+            if (p.splits > 1)
+                hipLaunchKernelGGL((tfc_dense_deep_kernel<T, AK, BK, true>), grid, dim3(512), 0, s, g);
+            else
+                hipLaunchKernelGGL((tfc_dense_deep_kernel<T, AK, BK, false>), grid, dim3(512), 0, s, g);
+            TFC_LAUNCH_CHECK("tfc_dense_deep");
+            return TFC_OK;
+        }
         if (p.bm == 256) return launch_tile<T, AK, BK, 256, 128>(g, p, s);
+    }
     if (p.bn == 128) return launch_tile<T, AK, BK, 128, 128>(g, p, s);
     if (p.bm == 128) return launch_tile<T, AK, BK, 128, 64>(g, p, s);
     return launch_tile<T, AK, BK, 64, 64>(g, p, s);
@@ -561,8 +717,8 @@ bool act_ok(int act) {
 
 extern "C" int64_t tfc_dense_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype) {
     if (m <= 0 || n <= 0 || k <= 0 || !tfc_dtype_ok(dtype)) return 0;
-    const Plan p = plan(m, n, k, dtype);
-    return p.splits > 1 ? p.splits * m * n : 0;
+    const int64_t a = plan(m, n, k, dtype, false).splits, b = deep_shape(m, n, k, dtype) ? plan(m, n, k, dtype, true).splits : 1;
+    return std::max(a, b) > 1 ? std::max(a, b) * m * n : 0;
 }
 
 extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
@@ -575,7 +731,7 @@ extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t work
     TFC_REQUIRE(d->a_along_k || !d->b_along_k, TFC_EUNSUPPORTED,
                 "tfc_dense: an A that runs along its rows needs a B that runs along its columns");
     TFC_REQUIRE(d->lda >= 0 && d->ldb >= 0 && d->ldc >= d->n && (!d->residual || d->ldr >= 0), TFC_EINVAL, "tfc_dense: bad stride");
-    const Plan p = d->k ? plan(d->m, d->n, d->k, d->dtype) : Plan{64, 64, 1, 1, 1, 0};
+    const Plan p = d->k ? plan(d->m, d->n, d->k, d->dtype, deep_operands(*d)) : Plan{64, 64, 1, 1, 1, 0};
     // (a thread's offset in a tile has 32 bits: 256 rows, or a step of 64, of the longest row)
     TFC_REQUIRE(d->lda < 1 << 22 && d->ldb < 1 << 22, TFC_EUNSUPPORTED, "tfc_dense: operand rows of 2^22 elements or more");
     TFC_REQUIRE(p.tiles_m * p.tiles_n < (int64_t)1 << 31, TFC_EUNSUPPORTED, "tfc_dense: %lld x %lld has too many tiles",

@@ -128,6 +128,14 @@ def test_large(device, dt, m, k, n):
     _check(*_inputs(m, k, n, dt, m + n, device), "silu", 1 / math.sqrt(k))
 
 
+@pytest.mark.parametrize("dt", TYPES[1:])
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("m,k,n", [(4096, 512, 4096), (4128, 544, 4384)])
+def test_tiles_of_256(device, dt, transposed, m, k, n):
+    """Sizes at which all three products take the kernel for large ones, whole tiles and edges."""
+    _check(*_inputs(m, k, n, dt, m + k, device, transposed=transposed), "gelu", 1 / math.sqrt(k))
+
+
 def test_layouts(device):
     """Row strides, odd starts, transposed and broadcast operands, more axes: the same bits as packed copies."""
     from matten_amd import ops
