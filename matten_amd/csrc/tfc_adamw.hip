@@ -276,7 +276,7 @@ int64_t fill_group(const tfc_adamw_tensor* t, int n, int64_t chunk, Group& g) {
     return blocks;
 }
 
-// The tensors are taken TENSORS at a time, and fewer where their workgroups would not fit one grid.
+// The tensors are taken TENSORS at a time.
 template <class F>
 int by_groups(const tfc_adamw_tensor* t, int n_tensors, int64_t chunk, F&& f) {
     for (int i = 0; i < n_tensors; i += TENSORS) {

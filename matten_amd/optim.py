@@ -9,7 +9,6 @@ from __future__ import annotations
 
 import ctypes as C
 import math
-from operator import is_
 from typing import Iterable, Optional
 
 import torch
@@ -32,8 +31,8 @@ class _Table:
     def __init__(self, group, params, states, indexes, bits: int):
         self.group, self.params, self.states = group, params, states
         self.device, self.dtype = params[0].device, params[0].dtype
-        self.entries = [tuple(st.values()) for st in states]  # (alive as long as their addresses are used)
-        self.at = [p.data_ptr() for p in params]
+        self.entries = [t for st in states for t in st.values()]  # (alive as long as their addresses are used)
+        self.at = [t.data_ptr() for t in (*params, *self.entries)]
         self.sizes = [p.numel() for p in params]
         self.rows = (_lib.AdamwTensor * len(params))()
         names = list(_STATE[bits])
@@ -46,10 +45,15 @@ class _Table:
 
     def holds(self, state) -> bool:
         """Whether parameters and state still lie where the descriptors say, every parameter with a gradient."""
-        for p, at, st, entries in zip(self.params, self.at, self.states, self.entries):
-            if p.grad is None or p.data_ptr() != at or state.get(p) is not st or not all(map(is_, st.values(), entries)):
+        entries = []
+        for p, st in zip(self.params, self.states):
+            if p.grad is None or state.get(p) is not st:
                 return False
-        return True
+            entries += st.values()
+        try:
+            return [t.data_ptr() for t in (*self.params, *entries)] == self.at
+        except AttributeError:  # (not a tensor: for _check_state to name)
+            return False
 
 
 class AdamW(torch.optim.Optimizer):
@@ -71,7 +75,7 @@ class AdamW(torch.optim.Optimizer):
       number is fixed, a tensor can be written to between replays.
 
     Parameters and gradients are contiguous and on a ROCm device (gradients that are not contiguous are copied); a sparse gradient
-    raises.  A parameter without a gradient is skipped and its step count stands.  The first step allocates the state and
+    raises, and so do parameters that share memory (they are stepped at the same time).  `amsgrad` and `maximize` do not exist.  A parameter without a gradient is skipped and its step count stands.  The first step allocates the state and
     therefore must not be inside a graph capture; a captured step drops its gradients (`zero_grad()`, set to None) rather than
     zeroing them, as matten_amd.graphs asks of every captured backward pass."""
 
@@ -96,6 +100,8 @@ class AdamW(torch.optim.Optimizer):
             for p in g["params"]:
                 if p.dtype not in ops._dtype_codes:
                     raise TypeError(f"AdamW: parameters must be float32, bfloat16 or float16, got {p.dtype}")
+            if len(set(g["params"])) != len(g["params"]):
+                raise ValueError("AdamW: a parameter is in its group twice")
         except Exception:
             self.param_groups.pop()
             raise
@@ -114,16 +120,29 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: eps and weight_decay must be finite and not negative, got {g['eps']}, {g['weight_decay']}")
 
     # ---- state
-    def _new_state(self, p) -> dict:
+    def _length(self, p, name: str) -> int:
         blocks = -(-p.numel() // BLOCK)
+        return 1 if name == "step" else p.numel() if self.state_bits == 32 else blocks if name.endswith("scale") else blocks * BLOCK
+
+    def _new_state(self, p) -> dict:
         st = {"step": torch.zeros((), dtype=torch.int32, device=p.device)}
         for k, dt in _STATE[self.state_bits].items():
             if self.state_bits == 32:
                 st[k] = torch.zeros_like(p, dtype=dt, memory_format=torch.contiguous_format)
             else:  # (a scale's exponent is 1 where all its values are zero)
-                n, fill = (blocks, 1) if k.endswith("scale") else (blocks * BLOCK, 0)
-                st[k] = torch.full((n,), fill, dtype=torch.uint8, device=p.device).view(dt)
+                st[k] = torch.full((self._length(p, k),), int(k.endswith("scale")), dtype=torch.uint8, device=p.device).view(dt)
         return st
+
+    def _check_state(self, p):
+        """Users may write to `state`: what the kernel is given has the types and sizes it takes for granted."""
+        st, want = self.state[p], {"step": torch.int32, **_STATE[self.state_bits]}
+        if set(st) != set(want):
+            raise ValueError(f"AdamW: state entries {sorted(st)} are not those of moments in {self.state_bits} bits")
+        for k, dt in want.items():
+            t, n = st[k], self._length(p, k)
+            if not isinstance(t, torch.Tensor) or t.dtype != dt or t.device != p.device or t.numel() != n or not t.is_contiguous():
+                got = f"{t.dtype}, {tuple(t.shape)} on {t.device}" if isinstance(t, torch.Tensor) else type(t).__name__
+                raise ValueError(f"AdamW: state entry `{k}` must be a contiguous {dt} tensor of {n} elements on {p.device}; got {got}")
 
     def load_state_dict(self, state_dict):
         """Takes copies.  The moments must have this optimizer's width and the parameters' sizes."""
@@ -180,6 +199,11 @@ class AdamW(torch.optim.Optimizer):
             first += len(g["params"])
             for (device, _), items in sets.items():
                 tables.append(self._table(g, device, [p for p, _ in items], [i for _, i in items]))
+        end = 0
+        for at, n in sorted((p.data_ptr(), p.numel() * p.element_size()) for t in tables for p in t.params if p.numel()):
+            if at < end:
+                raise ValueError("AdamW: two parameters share memory")
+            end = at + n
         self._tables = tables, rest, [(id(g), len(g["params"])) for g in self.param_groups]
         return tables
 
@@ -193,6 +217,7 @@ class AdamW(torch.optim.Optimizer):
                 if torch.cuda.is_current_stream_capturing():
                     raise RuntimeError("AdamW: the first step allocates the state and cannot be captured; run one step before the capture")
                 self.state[p].update(self._new_state(p))
+            self._check_state(p)
         return _Table(group, params, [self.state[p] for p in params], indexes, self.state_bits)
 
     @torch.no_grad()

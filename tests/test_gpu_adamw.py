@@ -310,6 +310,41 @@ def test_state_and_storage_that_are_replaced(device):
         _same(opt, p, r)
 
 
+def test_state_storage_that_moves(device):
+    """State whose storage is taken away and brought back between steps (`.data`, as programs do that keep it on the host
+    meanwhile), and a state dict that went through a file that loads without executing anything."""
+    import io
+
+    from matten_amd import optim
+
+    for bits in (32, 8):
+        params = _tensors([300, 1000], torch.float32, device, 16)
+        refs = [Reference(p, i, bits) for i, p in enumerate(params)]
+        opt = optim.AdamW(params, lr=1e-3, state_bits=bits)
+        for k in range(4):
+            _grads(params, 100 + k)
+            opt.step()
+            for p, r in zip(params, refs):
+                r.step(p.grad)
+                _same(opt, p, r)
+            if k < 2:
+                host = [(t, t.data.cpu()) for st in opt.state.values() for t in st.values()]
+                for t, h in host:
+                    t.data = h
+                with pytest.raises(ValueError, match="state entry"):  # (on the host still)
+                    opt.step()
+                junk = [torch.full((500,), 7.0, device=device) for _ in range(8)]
+                for t, h in host:
+                    t.data = h.to(device)
+            elif k == 2:
+                f = io.BytesIO()
+                torch.save(opt.state_dict(), f)
+                f.seek(0)
+                opt = optim.AdamW(params, lr=1e-3, state_bits=bits)
+                opt.load_state_dict(torch.load(f, weights_only=True))
+        assert all(bool((j == 7.0).all()) for j in junk)
+
+
 def test_schedulers_closures_and_versions(device):
     from matten_amd import optim
 
@@ -403,7 +438,22 @@ def test_refusals_on_the_device(device):
     e.grad = torch.sparse_coo_tensor(torch.tensor([[0]]), torch.ones(1, 3), (4, 3), device=device)
     with pytest.raises(RuntimeError, match="dense"):
         optim.AdamW([e]).step()
+    flat = torch.zeros(100, device=device)
+    shared = [torch.nn.Parameter(flat[:60]), torch.nn.Parameter(flat[59:])]
+    for t in shared:
+        t.grad = torch.ones_like(t)
+    with pytest.raises(ValueError, match="share memory"):
+        optim.AdamW([{"params": shared[:1]}, {"params": shared[1:]}]).step()
+    assert not flat.any()
     p.grad = torch.zeros_like(p)
+    for k, bad in [("exp_avg", torch.zeros(63, device=device)), ("exp_avg", torch.zeros(64, device=device).half()), ("step", 3),
+                   ("exp_avg_sq", torch.zeros(64)), ("exp_avg", torch.zeros(128, device=device)[::2]),
+                   ("step", torch.zeros((), device=device)), ("more", torch.zeros(64, device=device))]:
+        opt = optim.AdamW([p])
+        opt.step()
+        opt.state[p][k] = bad
+        with pytest.raises(ValueError, match="state entr"):
+            opt.step()
     with pytest.raises(RuntimeError, match="lr tensor"):
         optim.AdamW([p], lr=torch.tensor(1e-3)).step()
     L = _lib.lib()

@@ -42,6 +42,17 @@ def test_other_types_and_devices():
     assert len(opt.param_groups) == n
 
 
+@pytest.mark.filterwarnings("ignore:optimizer contains a parameter group")
+def test_a_parameter_twice():
+    from matten_amd import optim
+
+    p, q = _param(3), _param(2)
+    with pytest.raises(ValueError, match="twice"):
+        optim.AdamW([p, q, p])
+    with pytest.raises(ValueError):
+        optim.AdamW([{"params": [p]}, {"params": [q, p]}])
+
+
 def test_plain_step_equals_torch_adamw():
     """The written-out step against torch.optim.AdamW in 64 bits: fp32 roundings only (12 operations, each 2^-24)."""
     g = torch.Generator().manual_seed(0)
