@@ -59,8 +59,8 @@ __device__ __forceinline__ float act_eval(int act, float x) {
         case TFC_ACT_ABS: return fabsf(x);
         case TFC_ACT_SIGMOID: return sigmoid_<FAST>(x);
         case TFC_ACT_GELU: {
-            const float h = x * tail_<FAST>(x);
-            return x > 0.f ? x - h : h;
+            const float h = tail_<FAST>(x);
+            return x * (x > 0.f ? 1.f - h : h);  // (+inf stays +inf)
         }
         default: return x;
     }

@@ -380,7 +380,7 @@ constexpr int DEEP = 256, DEEP_K = 32, DEEP_IMAGE = DEEP * DEEP_K;
 // the kernel's own waits (TFC_DEEP_STEP) are the ones there are.  M0 is read one state after it was set.
 __device__ __forceinline__ void memory_to_lds(const char* base, uint32_t off, uint16_t* to) {
     const uint32_t lds = (uint32_t)tfc_uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
 }
 
 template <class T, bool ALONG_K>

@@ -1948,7 +1948,7 @@ class _LayerNormFn(torch.autograd.Function):
         x, w, b, stats = ctx.saved_tensors
         need = ctx.needs_input_grad
         if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
-            return (*_differentiable_grads(lambda: _layer_norm_composite(x, w, b, ctx.eps), (x, w, b), need, g), None)
+            return (*_differentiable_grads(lambda *t: _layer_norm_composite(*t, ctx.eps), (x, w, b), need, g), None)
         rows, d = x.shape
         g = g.contiguous()
         dx = torch.empty_like(x) if need[0] else None
@@ -1968,9 +1968,11 @@ class _LayerNormFn(torch.autograd.Function):
 
 
 def _differentiable_grads(fn, inputs, need, g):
-    """Gradients of fn() with respect to the `inputs` that need one, as a graph of their own (None for the others)."""
+    """Gradients of fn(*inputs) with respect to the `inputs` that need one, as a graph of their own (None for the others).  Each is
+    the partial one: fn is given views, since inputs may be one tensor, or computed from one another."""
     with torch.enable_grad():
-        grads = iter(torch.autograd.grad(fn(), [t for t, n in zip(inputs, need) if n], g, create_graph=True))
+        inputs = [None if t is None else t.view_as(t) for t in inputs]
+        grads = iter(torch.autograd.grad(fn(*inputs), [t for t, n in zip(inputs, need) if n], g, create_graph=True))
     return [next(grads) if n else None for _, n in zip(inputs, need)]
 
 
@@ -2079,7 +2081,7 @@ class _DenseFn(torch.autograd.Function):
         if not any(need[:3]):
             return None, None, None, dr, None, None, None
         if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
-            return (*_differentiable_grads(lambda: _dense_composite(x, w, b, *ctx.args), (x, w, b), need, g), dr, None, None, None)
+            return (*_differentiable_grads(lambda *t: _dense_composite(*t, *ctx.args), (x, w, b), need, g), dr, None, None, None)
         return (*_dense_bwd_run(g.contiguous(), x, w, b, z, *ctx.args, need), dr, None, None, None)
 
 

@@ -218,6 +218,78 @@ def test_values_that_are_not_finite(device):
         assert torch.equal(y, ops.dense(torch.zeros_like(x), w, b, r))
 
 
+def test_infinities_through_activations(device):
+    """Sums of 16 bits that are infinite: limits where there are any."""
+    from matten_amd import ops
+
+    inf = float("inf")
+    for dt in TYPES[1:]:
+        x = torch.tensor([[inf], [-inf]], dtype=dt, device=device)
+        w = torch.ones(1, 1, dtype=dt, device=device)
+        for act, hi, lo in [("identity", inf, -inf), ("ssp", inf, -math.log(2)), ("tanh", 1, -1), ("abs", inf, inf), ("sigmoid", 1, 0),
+                            ("silu", inf, None), ("gelu", inf, None)]:
+            y = ops.dense(x, w, act=act)[:, 0].tolist()
+            assert y[0] == hi and (lo is None or abs(y[1] - lo) <= 2.0**-8 or y[1] == lo), (act, y)
+
+
+def test_smallest_and_largest_fp32(device):
+    """Pieces below the least normal number may be lost: 2^-126 of what the other operand multiplies."""
+    from matten_amd import ops
+
+    x = torch.tensor([[2.0**-149], [1.5 * 2.0**-130], [2.0**-126], [1.2345678 * 2.0**-115], [2.0**-100 / 3], [3.4e38], [-3.4028234e38]], device=device)
+    for scale in (1.0, 2.0**90):
+        w = torch.full((1, 3), scale, device=device)
+        if scale > 1:
+            x = x[:5]
+        y, want = ops.dense(x, w).double(), x.double() @ w.double()
+        assert ((y - want).abs() <= 3 * U * want.abs() + 2.0**-126 * 3 * scale).all()
+
+
+def test_offsets_beyond_32_bits(device):
+    """2^32 elements and more on either side: the last rows equal the same rows alone, sums see them all."""
+    from matten_amd import ops
+
+    m, k, n = (1 << 26) + 77, 65, 66
+    dt = torch.bfloat16
+    x = torch.zeros(m, k, dtype=dt, device=device)
+    x[-3000:], w, b, _, dy = _inputs(3000, k, n, dt, 21, device, residual=False)
+    args = dict(act="silu", alpha=0.1)
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    y = ops.dense(*leaves, **args)
+    few = [t.detach().clone().requires_grad_(True) for t in (x[-3000:], w, b)]
+    ref = ops.dense(*few, **args)
+    assert torch.equal(y[-3000:], ref) and torch.equal(y[0], y[m // 2])
+    g = torch.zeros(m, n, dtype=dt, device=device)
+    g[-3000:] = dy
+    got, want = torch.autograd.grad(y, leaves, g), torch.autograd.grad(ref, few, dy)
+    del y, g
+    assert torch.equal(got[0][-3000:], want[0]) and not got[0][: m - 3000].any()
+    for p, q in zip(got[1:], want[1:]):  # (the same products, added up in other groups)
+        assert (p.double() - q.double()).abs().max() <= 2.0**-7 * q.abs().max()
+
+
+def test_inputs_that_depend_on_one_another(device):
+    """One tensor as both operands, a bias computed from x: the differentiable backward counts every path once."""
+    from matten_amd import ops
+
+    x, w, _, _, dy = _inputs(8, 8, 8, torch.float32, 23, device, residual=False)
+
+    def grads(f, create, args):
+        args = [t.clone().requires_grad_(True) for t in args]
+        return torch.autograd.grad(f(*args), args, dy.to(args[0].dtype), create_graph=create)
+
+    def mine(x, w):
+        return ops.dense(x, x, act="silu", alpha=0.3) + ops.dense(x, w, x.sum(0), act="tanh", alpha=0.3)
+
+    def plain(x, w):
+        return torch.nn.functional.silu(0.3 * x @ x) + torch.tanh(0.3 * x @ w + x.sum(0))
+
+    want = grads(plain, False, [x.double(), w.double()])
+    for create in (False, True):
+        for a, e in zip(grads(mine, create, [x, w]), want):
+            assert (a.double() - e).abs().max() <= 256 * U * e.abs().max()
+
+
 def test_gradients_against_differences(device):
     """Differences of the forward (fp32, L = <dy, y>) along a direction in (x, w, b) against <gradient, direction>.  Allowed: what the
     same difference is off in 64 bits, and the forward's error bound over the step."""

@@ -182,6 +182,48 @@ def test_second_order(device):
         assert (a.double() - e).abs().max() <= 512 * U * e.abs().max()
 
 
+def test_one_tensor_as_weight_and_bias(device):
+    """The differentiable backward counts every path once."""
+    from matten_amd import ops
+
+    g = torch.Generator(device=device).manual_seed(31)
+    x, w, dy = (torch.randn(*s, generator=g, device=device) for s in ((7, 12), (12,), (7, 12)))
+
+    def grads(f, create, args):
+        args = [t.clone().requires_grad_(True) for t in args]
+        return torch.autograd.grad(f(*args), args, dy.to(args[0].dtype), create_graph=create)
+
+    want = grads(lambda x, w: torch.nn.functional.layer_norm(x, (12,), w, w * x[0]), False, [x.double(), w.double()])
+    for create in (False, True):
+        for a, e in zip(grads(lambda x, w: ops.layer_norm(x, w, w * x[0]), create, [x, w]), want):
+            assert (a.double() - e).abs().max() <= 256 * 2.0**-24 * e.abs().max()
+    want = grads(lambda x, w: torch.nn.functional.layer_norm(x, (12,), w, w), False, [x.double(), w.double()])
+    for create in (False, True):
+        for a, e in zip(grads(lambda x, w: ops.layer_norm(x, w, w), create, [x, w]), want):
+            assert (a.double() - e).abs().max() <= 256 * 2.0**-24 * e.abs().max()
+
+
+def test_offsets_beyond_32_bits(device):
+    from matten_amd import ops
+
+    for rows, d in [((1 << 26) + 77, 65), (131100, 32800)]:  # (a wave a row; rows walked again)
+        g = torch.Generator(device=device).manual_seed(32)
+        x = torch.zeros(rows, d, dtype=torch.bfloat16, device=device)
+        x[-2000:] = torch.randn(2000, d, generator=g, device=device)
+        w, b = (torch.randn(d, generator=g, device=device).bfloat16() for _ in range(2))
+        leaves = [t.requires_grad_(True) for t in (x, w, b)]
+        few = [t.detach().clone().requires_grad_(True) for t in (x[-2000:], w, b)]
+        y, ref = ops.layer_norm(*leaves), ops.layer_norm(*few)
+        assert torch.equal(y[-2000:], ref) and torch.equal(y[0], b) and torch.equal(y[rows // 2], b)
+        dy = torch.zeros_like(x)
+        dy[-2000:] = torch.randn(2000, d, generator=g, device=device)
+        got, want = torch.autograd.grad(y, leaves, dy), torch.autograd.grad(ref, few, dy[-2000:].clone())
+        del y, dy
+        assert torch.equal(got[0][-2000:], want[0]) and not got[0][: rows - 2000].any()
+        for p, q in zip(got[1:], want[1:]):  # (the same terms, added up in other groups)
+            assert (p.double() - q.double()).abs().max() <= 2.0**-7 * q.abs().max()
+
+
 def test_runs_agree_on_streams_and_in_graphs(device):
     from matten_amd import ops
 
