@@ -586,13 +586,14 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
  * (eigenn/nn/utils.py:182,247-252) is a chain of these.
  *   a [m, k]: a_along_k: element (i, kk) at i lda + kk, else at kk lda + i;
  *   b [k, n]: b_along_k: element (kk, j) at j ldb + kk, else at kk ldb + j.  (a along its rows with b along k: not built.)
- *   c: row stride ldc; residual (nullable) [m, n] with row stride ldr; bias (nullable) [n]; z (nullable) [m, n] packed: receives
- *   alpha a b + bias.  Workspace: tfc_dense_workspace_floats() (0: none).  k = 0: the epilogue of zeros.
+ *   c: row stride ldc; residual (nullable) [m, n] with row stride ldr; bias (nullable) [n]; z (nullable), of
+ *   tfc_dense_z_bytes(): receives alpha a b + bias for tfc_dense_bwd, in a form of its own.  Workspace: tfc_dense_workspace_floats() (0: none).  k = 0: the epilogue of zeros.
  * Operand rows are shorter than 2^22 elements.
  * tfc_dense_bwd: from dy [m, n] packed, with dz = act_cst act'(alpha x w + bias) dy:  dx = alpha dz w^T [m, k] packed,
  *   dw = alpha x^T dz, packed in the order of w ([k, n], or [n, k] where w_along_k), db = the column sums of dz [n]; each nullable.
  *   x [m, k] with row stride ldx.  z is what the forward call left, wanted where tfc_dense_keeps_z() says so (layers of at
- *   most 64 x 64 form it again, from x, w and bias: one kernel, bound by reading x and dy once). */
+ *   most 64 x 64 form it again, from x, w and bias: one kernel, bound by reading x and dy once).  dz goes into the products in
+ *   fp32, for 16-bit types in two pieces, or rounded to the type where m n, m k and n k are all 2^14 or more. */
 #define TFC_ACT_GELU 6 /* x Phi(x) with the normal distribution function Phi (tfc_dense only) */
 typedef struct tfc_dense_desc {
     int64_t m, n, k;
@@ -629,6 +630,7 @@ typedef struct tfc_dense_bwd_desc {
 } tfc_dense_bwd_desc;
 
 int tfc_dense_keeps_z(int64_t n, int64_t k, int32_t act);
+int64_t tfc_dense_z_bytes(int64_t m, int64_t n, int32_t dtype);
 int64_t tfc_dense_bwd_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act);
 int tfc_dense_bwd(const tfc_dense_bwd_desc* desc, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
 

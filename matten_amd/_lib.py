@@ -238,6 +238,7 @@ SIGNATURES = {
     "tfc_dense_workspace_floats": (_I64, [_I64, _I64, _I64, _I32]),
     "tfc_dense": (C.c_int, [C.POINTER(DenseDesc), _P, _I64, _P]),
     "tfc_dense_keeps_z": (C.c_int, [_I64, _I64, _I32]),
+    "tfc_dense_z_bytes": (_I64, [_I64, _I64, _I32]),
     "tfc_dense_bwd_workspace_floats": (_I64, [_I64, _I64, _I64, _I32, _I32]),
     "tfc_dense_bwd": (C.c_int, [C.POINTER(DenseBwdDesc), _P, _I64, _P]),
     "tfc_grad_sumsq_partials": (_I64, [C.POINTER(AdamwTensor), _I32]),

@@ -29,24 +29,28 @@ template <bool FAST>
 __device__ __forceinline__ float sigmoid_(float x) {
     return inv_<FAST>(1.f + exp_<FAST>(-x));
 }
-// Half of erfc(|x| / sqrt 2): the normal distribution's tail beyond |x|.  FAST: erfc(z) = t exp(-z^2 + q(t)), t = 1 / (1 + z / 2), with
-// q a Chebyshev fit of degree 9 of log(erfc(z) exp(z^2) / t), off by at most 2.1e-7 (relative, in the tail too).
+// The normal distribution's tail beyond |x|, half of erfc(z) with z = |x| / sqrt 2; bell = exp(-x^2 / 2).  FAST: erfc(z) = t q(t) exp(-z^2),
+// t = 1 / (1 + z / 2), with q a fit of degree 8 of erfc(z) exp(z^2) / t on 0 < t <= 1 that is off by at most 6e-7 (relative, in the
+// tail too).
 template <bool FAST>
-__device__ __forceinline__ float tail_(float x) {
+__device__ __forceinline__ float tail_(float x, float bell) {
     const float z = 0.70710678118654752440f * fabsf(x);
     if (!FAST) return 0.5f * erfcf(z);
     const float t = __builtin_amdgcn_rcpf(1.f + 0.5f * z);
-    float q = 0.16738100959847832f;
-    q = q * t - 0.8013252602706117f;
-    q = q * t + 1.435545460278193f;
-    q = q * t - 1.0600993927570561f;
-    q = q * t + 0.2137827400077032f;
-    q = q * t - 0.15077300610628097f;
-    q = q * t + 0.0846820952510744f;
-    q = q * t + 0.3765501918286564f;
-    q = q * t + 0.9997568084310646f;
-    q = q * t - 1.265500578284187f;
-    return 0.5f * t * __expf(q - z * z);
+    float q = -0.021927181631326675f;
+    q = q * t + 0.11047209799289703f;
+    q = q * t - 0.18857893347740173f;
+    q = q * t + 0.08813999593257904f;
+    q = q * t + 0.013894896022975445f;
+    q = q * t + 0.09286484122276306f;
+    q = q * t + 0.12302764505147934f;
+    q = q * t + 0.1410595327615738f;
+    q = q * t + 0.14104732871055603f;
+    return t * q * bell;
+}
+template <bool FAST>
+__device__ __forceinline__ float bell_(float x) {
+    return exp_<FAST>(-0.5f * x * x);
 }
 
 template <bool FAST>
@@ -59,7 +63,7 @@ __device__ __forceinline__ float act_eval(int act, float x) {
         case TFC_ACT_ABS: return fabsf(x);
         case TFC_ACT_SIGMOID: return sigmoid_<FAST>(x);
         case TFC_ACT_GELU: {
-            const float h = tail_<FAST>(x);
+            const float h = tail_<FAST>(x, FAST ? bell_<FAST>(x) : 0.f);
             return x * (x > 0.f ? 1.f - h : h);  // (+inf stays +inf)
         }
         default: return x;
@@ -104,8 +108,8 @@ __device__ __forceinline__ float act_grad(int act, float x) {
             return s * (1.f - s);
         }
         case TFC_ACT_GELU: {
-            const float h = tail_<FAST>(x);
-            return (x > 0.f ? 1.f - h : h) + x * 0.39894228040143267794f * exp_<FAST>(-0.5f * x * x);
+            const float bell = bell_<FAST>(x), h = tail_<FAST>(x, bell);
+            return (x > 0.f ? 1.f - h : h) + x * 0.39894228040143267794f * bell;
         }
         default: return 1.f;
     }
@@ -155,6 +159,15 @@ __device__ __forceinline__ Unit3 split8(const float (&x)[8]) {
         r.l[i] = __builtin_bit_cast(unsigned, ll);
     }
     return r;
+}
+
+// What is left of x behind its rounding to 16 bits.  fp16: times 2^11, so that it does not fall below the type's range (products with
+// it are scaled back).
+constexpr float TFC_LO_SCALE = 2048.f;
+template <class T>
+__device__ __forceinline__ float second_piece(T, float x) {
+    const float hi = (float)(T)x, left = x - hi;
+    return fabsf(hi) < __builtin_inff() ? (std::is_same<T, tfc_f16>::value ? left * TFC_LO_SCALE : left) : 0.f;
 }
 
 __device__ __forceinline__ floatx16 mma(tfc_bf16, uintx4 a, uintx4 b, floatx16 c) {

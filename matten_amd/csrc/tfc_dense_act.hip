@@ -11,6 +11,11 @@
 // times the rate of the fp32 matrix instruction and no less exact (an infinity has no pieces: it gives NaN).
 // The instruction's rows are the columns of C, so that a lane ends up with four neighbouring columns of a row.
 //
+// What the backward pass needs of the forward one is z = alpha A B + bias.  Rounded to a 16-bit type it would be wrong by as much as the
+// results are, and the gradients by 1.5 times what their own rounding is worth: store_z() keeps more of it.  dz is rounded for the
+// products, as the matrix instruction takes it; where the products are not what the time goes into it is kept in two
+// pieces (dz_pieces()).
+//
 // Few tiles and a long contraction (a weight's gradient over many rows): the contraction is split, partial tiles go to the
 // workspace and a second kernel adds them in order and applies the epilogue.
 #include "tfc_dense_act.h"
@@ -149,13 +154,64 @@ struct Args {
     long ldc;
     const void *bias, *res;
     long ldr;
-    void* z;  // [m, n] packed: alpha A B + bias, for the backward pass
+    void* z;  // alpha A B + bias, for the backward pass (store_z)
     float alpha, cst;
     int act;
     float* part;  // split contraction: [split][m][n]
     long k_split;
     int tiles_m, tiles_n;
+    int passes;        // 2 (16 bits only): one operand is the sum of two pieces, the second lo_a or lo_b bytes behind the first
+    long lo_a, lo_b;
 };
+
+// z [m, n], packed.  fp32: as it is.  bf16: as fp16, three bits better in the same two bytes: what lies beyond that range is cut to its
+// end, where every act' has reached its limit, and what is not zero does not become zero (abs).  fp16: the upper three bytes of the
+// fp32 number, a plane of two and behind it a plane of one.
+__device__ __forceinline__ tfc_f16 z_half(float v) {
+    const float a = fminf(fmaxf(fabsf(v), 0x1p-24f), 65504.f);
+    return v != 0.f && v == v ? (tfc_f16)__builtin_copysignf(a, v) : (tfc_f16)v;
+}
+template <class T, int N>
+__device__ __forceinline__ void store_z(void* z, long count, long at, const float (&v)[N]) {
+    if constexpr (std::is_same<T, float>::value) {
+        tfc_store<float, N>((float*)z + at, tfc_pack<float, N>(v));
+    } else if constexpr (std::is_same<T, tfc_bf16>::value) {
+        tfc_f16 h[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) h[j] = z_half(v[j]);
+        __builtin_memcpy((tfc_f16*)z + at, h, sizeof(h));
+    } else {
+        uint16_t hi[N];
+        uint8_t lo[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+            const uint32_t u = __float_as_uint(v[j]);
+            hi[j] = (uint16_t)(u >> 16), lo[j] = (uint8_t)(u >> 8);
+        }
+        __builtin_memcpy((uint16_t*)z + at, hi, sizeof(hi));
+        __builtin_memcpy((uint8_t*)z + 2 * count + at, lo, sizeof(lo));
+    }
+}
+template <class T, int N>
+__device__ __forceinline__ void load_z(const void* z, long count, long at, long left, float (&v)[N]) {
+    if constexpr (std::is_same<T, float>::value) {
+        tfc_load_f<float, N>((const float*)z + at, left, v);
+    } else if constexpr (std::is_same<T, tfc_bf16>::value) {
+        tfc_load_f<tfc_f16, N>((const tfc_f16*)z + at, left, v);
+    } else if (left >= N) {
+        TfcRaw<T, N> hi;
+        typename TfcWords<N>::type lo;
+        __builtin_memcpy(&hi, (const uint16_t*)z + at, sizeof(hi));
+        __builtin_memcpy(&lo, (const uint8_t*)z + 2 * count + at, sizeof(lo));
+#pragma unroll
+        for (int j = 0; j < N; ++j) v[j] = __uint_as_float((hi[j / 2] >> (j % 2 * 16)) << 16 | (lo[j / 4] >> (j % 4 * 8) & 255) << 8);
+    } else {
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+            v[j] = j < left ? __uint_as_float((uint32_t)((const uint16_t*)z)[at + j] << 16 | (uint32_t)((const uint8_t*)z)[2 * count + at + j] << 8)
+                            : 0.f;
+    }
+}
 
 // N neighbouring columns of one row of C, all inside; `res`: their residual where there is one.
 template <class T, int N>
@@ -168,7 +224,7 @@ __device__ __forceinline__ void epilogue(const Args& g, long row, long col, floa
 #pragma unroll
         for (int j = 0; j < N; ++j) v[j] += b[j];
     }
-    if (g.z) tfc_store<T, N>((T*)g.z + row * g.n + col, tfc_pack<T, N>(v));
+    if (g.z) store_z<T, N>(g.z, g.m * g.n, row * g.n + col, v);
     act_apply<sizeof(T) == 2>(g.act, v);
 #pragma unroll
     for (int j = 0; j < N; ++j) v[j] *= g.cst;
@@ -320,8 +376,6 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
     A sa;
     B sb;
     const long ra = g.m - m0, rb = g.n - n0;
-    sa.start(g.a, m0, ra, k0);
-    sb.start(g.b, n0, rb, k0);
     // One step: its operands to LDS, then (MORE) the loads of the next one and the products.
     auto step = [&](auto more, long left) {
         __syncthreads();  // the step before has been read
@@ -351,16 +405,28 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
                         acc[i][j] = mma(Mma<T>(), fb[j][P == 3 ? TFC_TERM_B[q] : 0], fa[i][P == 3 ? TFC_TERM_A[q] : 0], acc[i][j]);
         }
     };
-    long left = k1 - k0;  // of the contraction, from the step in hand on
-    long plain = plain_part(k0, k1, g.k, K, AK || ra >= BM, g.a.ld, BK || rb >= BN, g.b.ld);
-    if (plain > 0)
-        sa.template load<true>(ra, left), sb.template load<true>(rb, left);
-    else
-        sa.template load<false>(ra, left), sb.template load<false>(rb, left);
-    for (; plain > K; plain -= K, left -= K) step(std::integral_constant<int, 1>(), left - K);
+    const int passes = P == 1 ? g.passes : 1;
 #pragma unroll 1
-    for (; left > K; left -= K) step(std::integral_constant<int, 2>(), left - K);
-    step(std::integral_constant<int, 0>(), 0);
+    for (int lo = passes - 1; lo >= 0; --lo) {  // (the second pieces first: the smaller terms)
+        sa.start({(const char*)g.a.p + lo * g.lo_a, g.a.ld}, m0, ra, k0);
+        sb.start({(const char*)g.b.p + lo * g.lo_b, g.b.ld}, n0, rb, k0);
+        long left = k1 - k0;  // of the contraction, from the step in hand on
+        long plain = plain_part(k0, k1, g.k, K, AK || ra >= BM, g.a.ld, BK || rb >= BN, g.b.ld);
+        if (plain > 0)
+            sa.template load<true>(ra, left), sb.template load<true>(rb, left);
+        else
+            sa.template load<false>(ra, left), sb.template load<false>(rb, left);
+        for (; plain > K; plain -= K, left -= K) step(std::integral_constant<int, 1>(), left - K);
+#pragma unroll 1
+        for (; left > K; left -= K) step(std::integral_constant<int, 2>(), left - K);
+        step(std::integral_constant<int, 0>(), 0);
+        if (std::is_same<T, tfc_f16>::value && lo) {
+#pragma unroll
+            for (int i = 0; i < MI; ++i)
+#pragma unroll
+                for (int j = 0; j < NI; ++j) acc[i][j] *= 1.f / TFC_LO_SCALE;
+        }
+    }
     __syncthreads();
     write_out<T, MI, NI, SPLIT>(g, acc, (float*)lds + wave * corner_floats(NI), m0 + wm, n0 + wn);
 }
@@ -380,7 +446,7 @@ constexpr int DEEP = 256, DEEP_K = 32, DEEP_IMAGE = DEEP * DEEP_K;
 // the kernel's own waits (TFC_DEEP_STEP) are the ones there are.  M0 is read one state after it was set.
 __device__ __forceinline__ void memory_to_lds(const char* base, uint32_t off, uint16_t* to) {
     const uint32_t lds = (uint32_t)tfc_uniform((int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) void*)to);
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(off), "s"(base) : "memory");
 }
 
 template <class T, bool ALONG_K>
@@ -540,11 +606,11 @@ __global__ __launch_bounds__(256) void tfc_dense_empty_kernel(const Args g) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward, elementwise
-// dz = cst act'(z) dy and the column sums of dz: a workgroup walks a slab of rows, cw threads side by side on a chunk of
+// dz = cst act'(z) dy, its second pieces `lo` elements behind the first (0: none), and the column sums of dz: a workgroup walks a slab of rows, cw threads side by side on a chunk of
 // columns, 256 / cw rows at a time; its sums go to one partial row.  z null: act is the identity.
 template <class T>
-__global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__ dy, const T* __restrict__ z, long rows, long n,
-                                                           int act, float cst, int cw, long slab, T* __restrict__ dz,
+__global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__ dy, const void* __restrict__ z, long rows, long n,
+                                                           int act, float cst, int cw, long slab, T* __restrict__ dz, long lo,
                                                            float* __restrict__ part) {
     constexpr int V = TfcType<T>::V;
     const int cl = threadIdx.x % cw, rl = threadIdx.x / cw, step = 256 / cw;
@@ -558,7 +624,7 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
             float g[V], x[V];
             tfc_load_f<T, V>(dy + r * n + c, left, g);
             if (z) {
-                tfc_load_f<T, V>(z + r * n + c, left, x);
+                load_z<T, V>(z, rows * n, r * n + c, left, x);
                 act_grad_apply<sizeof(T) == 2>(act, x);
 #pragma unroll
                 for (int j = 0; j < V; ++j) g[j] *= x[j];
@@ -569,6 +635,11 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
                 sum[j] += j < left ? g[j] : 0.f;
             }
             if (dz) tfc_store_f<T, V>(dz + r * n + c, left, g);
+            if (sizeof(T) == 2 && lo) {
+#pragma unroll
+                for (int j = 0; j < V; ++j) g[j] = second_piece(T(), g[j]);
+                tfc_store_f<T, V>(dz + lo + r * n + c, left, g);
+            }
         }
     }
     if (!part) return;
@@ -603,6 +674,7 @@ bool deep_operands(const tfc_dense_desc& d) {
 // the tiles alone do not put three workgroups (fp32: two, by LDS) on every CU the contraction is split, in parts of at least eight
 // steps; and where the partial tiles would not stay in the caches (over 16 MB) in parts long enough that writing and adding them
 // up takes less than half the time of the products: 1024 of k for 16 bits, 192 for fp32, whose products cost six times as much.
+// deep: whether the kernel for large products may be taken.
 Plan plan(int64_t m, int64_t n, int64_t k, int dtype, bool deep) {
     Plan p{};
     const bool wide = dtype == TFC_F32;
@@ -623,7 +695,6 @@ Plan plan(int64_t m, int64_t n, int64_t k, int dtype, bool deep) {
         return have * p.splits >= 256;
     };
     if (deep && take(256, 256, 256)) return p;
-    if (!wide && m >= 256 && n >= 128 && take(256, 128, 512) && p.tiles_m * p.tiles_n * p.splits >= 512) return p;
     if (m > 64 && n > 64 && take(128, 128, want)) return p;
     if (m > 64 && take(128, 64, want)) return p;
     take(64, 64, want);
@@ -653,7 +724,6 @@ int launch_layout(const Args& g, const Plan& p, hipStream_t s) {
             TFC_LAUNCH_CHECK("tfc_dense_deep");
             return TFC_OK;
         }
-        if (p.bm == 256) return launch_tile<T, AK, BK, 256, 128>(g, p, s);
     }
     if (p.bn == 128) return launch_tile<T, AK, BK, 128, 128>(g, p, s);
     if (p.bm == 128) return launch_tile<T, AK, BK, 128, 64>(g, p, s);
@@ -700,10 +770,10 @@ DzPlan dz_plan(int64_t rows, int64_t n, int dtype) {
 }
 
 template <class T>
-int dense_dz(const DzPlan& p, const void* dy, const void* z, int64_t rows, int64_t n, int act, float cst, void* dz, float* part,
-             hipStream_t s) {
-    hipLaunchKernelGGL(tfc_dense_dz_kernel<T>, dim3((unsigned)p.chunks, (unsigned)p.slabs), dim3(256), 0, s, (const T*)dy, (const T*)z,
-                       (long)rows, (long)n, act, cst, p.cw, (long)p.slab, (T*)dz, part);
+int dense_dz(const DzPlan& p, const void* dy, const void* z, int64_t rows, int64_t n, int act, float cst, void* dz, int64_t lo,
+             float* part, hipStream_t s) {
+    hipLaunchKernelGGL(tfc_dense_dz_kernel<T>, dim3((unsigned)p.chunks, (unsigned)p.slabs), dim3(256), 0, s, (const T*)dy, z, (long)rows,
+                       (long)n, act, cst, p.cw, (long)p.slab, (T*)dz, (long)lo, part);
     TFC_LAUNCH_CHECK("tfc_dense_dz");
     return TFC_OK;
 }
@@ -717,11 +787,14 @@ bool act_ok(int act) {
 
 extern "C" int64_t tfc_dense_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype) {
     if (m <= 0 || n <= 0 || k <= 0 || !tfc_dtype_ok(dtype)) return 0;
-    const int64_t a = plan(m, n, k, dtype, false).splits, b = deep_shape(m, n, k, dtype) ? plan(m, n, k, dtype, true).splits : 1;
-    return std::max(a, b) > 1 ? std::max(a, b) * m * n : 0;
+    int64_t splits = plan(m, n, k, dtype, false).splits;
+    if (deep_shape(m, n, k, dtype)) splits = std::max(splits, plan(m, n, k, dtype, true).splits);
+    return splits > 1 ? splits * m * n : 0;
 }
 
-extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
+// lo_a, lo_b: bytes from an operand's first pieces to its second ones (0: there are none).
+static int dense_product(const tfc_dense_desc* d, int64_t lo_a, int64_t lo_b, float* workspace, int64_t workspace_floats,
+                         tfc_stream_t stream) {
     TFC_REQUIRE(d, TFC_EINVAL, "tfc_dense: null descriptor");
     TFC_REQUIRE(tfc_dtype_ok(d->dtype), TFC_EINVAL, "tfc_dense: unknown dtype %d", (int)d->dtype);
     TFC_REQUIRE(act_ok(d->act), TFC_EINVAL, "tfc_dense: unknown activation %d", (int)d->act);
@@ -731,7 +804,7 @@ extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t work
     TFC_REQUIRE(d->a_along_k || !d->b_along_k, TFC_EUNSUPPORTED,
                 "tfc_dense: an A that runs along its rows needs a B that runs along its columns");
     TFC_REQUIRE(d->lda >= 0 && d->ldb >= 0 && d->ldc >= d->n && (!d->residual || d->ldr >= 0), TFC_EINVAL, "tfc_dense: bad stride");
-    const Plan p = d->k ? plan(d->m, d->n, d->k, d->dtype, deep_operands(*d)) : Plan{64, 64, 1, 1, 1, 0};
+    const Plan p = d->k ? plan(d->m, d->n, d->k, d->dtype, !lo_a && !lo_b && deep_operands(*d)) : Plan{64, 64, 1, 1, 1, 0};
     // (a thread's offset in a tile has 32 bits: 256 rows, or a step of 64, of the longest row)
     TFC_REQUIRE(d->lda < 1 << 22 && d->ldb < 1 << 22, TFC_EUNSUPPORTED, "tfc_dense: operand rows of 2^22 elements or more");
     TFC_REQUIRE(p.tiles_m * p.tiles_n < (int64_t)1 << 31, TFC_EUNSUPPORTED, "tfc_dense: %lld x %lld has too many tiles",
@@ -745,17 +818,22 @@ extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t work
     g.m = d->m, g.n = d->n, g.k = d->k;
     g.c = d->c, g.ldc = d->ldc, g.bias = d->bias, g.res = d->residual, g.ldr = d->ldr, g.z = d->z;
     g.alpha = d->alpha, g.cst = d->act_cst, g.act = d->act, g.part = workspace;
+    g.passes = lo_a || lo_b ? 2 : 1, g.lo_a = lo_a, g.lo_b = lo_b;
     return TFC_BY_DTYPE(d->dtype, dense, g, p, d->a_along_k != 0, d->b_along_k != 0, s);
 }
 
-static int dense_dz_pass(const void* dy, const void* z, int64_t rows, int64_t n, int dtype, int act, float cst, void* dz, void* db,
-                         float* part, hipStream_t s) {
+extern "C" int tfc_dense(const tfc_dense_desc* d, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
+    return dense_product(d, 0, 0, workspace, workspace_floats, stream);
+}
+
+static int dense_dz_pass(const void* dy, const void* z, int64_t rows, int64_t n, int dtype, int act, float cst, void* dz, int64_t lo,
+                         void* db, float* part, hipStream_t s) {
     if (rows == 0) return db ? tfc_join_columns(nullptr, 0, n, db, 0, nullptr, dtype, s) : TFC_OK;
     const DzPlan p = dz_plan(rows, n, dtype);
     {
         TfcProfScope prof("tfc_dense_dz", s);
         const int rc = TFC_BY_DTYPE(dtype, dense_dz, p, dy, act == TFC_ACT_IDENTITY ? nullptr : z, rows, n, act, cst, dz,
-                                    db ? part : nullptr, s);
+                                    lo, db ? part : nullptr, s);
         if (rc) return rc;
     }
     return db ? tfc_join_columns(part, p.slabs, n, db, 0, nullptr, dtype, s) : TFC_OK;
@@ -763,13 +841,25 @@ static int dense_dz_pass(const void* dy, const void* z, int64_t rows, int64_t n,
 
 extern "C" int tfc_dense_keeps_z(int64_t n, int64_t k, int32_t act) { return act != TFC_ACT_IDENTITY && !tfc_dense_is_narrow(n, k); }
 
+extern "C" int64_t tfc_dense_z_bytes(int64_t m, int64_t n, int32_t dtype) {
+    return m > 0 && n > 0 && tfc_dtype_ok(dtype) ? m * n * (dtype == TFC_F32 ? 4 : dtype == TFC_BF16 ? 2 : 3) : 0;
+}
+
+// Pieces of the element type that dz is kept in.  One is what the matrix instruction takes; the gradients' error then is sqrt 2 of what
+// their own rounding is worth.  Two take that away and double the products (backward pass in bf16 with one and two, in us:
+// 16384 x 1024 x 4096: 415, 814; 200000 x 128 x 128: 103, 141; 414 x 1281 x 21: 29, 35).  One where there are elements enough on all
+// sides for the errors to come out at that; a gradient of few elements, or from few of dz, may have several times its share.
+static int dz_pieces(int64_t m, int64_t n, int64_t k, int dtype, int act) {
+    return dtype == TFC_F32 || act == TFC_ACT_IDENTITY || std::min(m * n, std::min(m * k, n * k)) >= 1 << 14 ? 1 : 2;
+}
+
 // The general backward pass's workspace: [dz | what one of its parts needs at a time], in floats.
 struct BwdSpace {
     int64_t dz, rest;
 };
 static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int dtype, int act) {
     BwdSpace w{};
-    if (act != TFC_ACT_IDENTITY) w.dz = (m * n * (int64_t)tfc_dtype_size(dtype) + 15) / 16 * 4;
+    if (act != TFC_ACT_IDENTITY) w.dz = (m * n * dz_pieces(m, n, k, dtype, act) * (int64_t)tfc_dtype_size(dtype) + 15) / 16 * 4;
     w.rest = std::max(m > 0 && n > 0 ? dz_plan(m, n, dtype).slabs * n : 0,
                       std::max(tfc_dense_workspace_floats(m, k, n, dtype),
                                std::max(tfc_dense_workspace_floats(k, n, m, dtype), tfc_dense_workspace_floats(n, k, m, dtype))));
@@ -802,9 +892,10 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
     const bool plain = d->act == TFC_ACT_IDENTITY;  // its constant goes into the products' own factor
     const void* dz = plain ? d->dy : (const void*)workspace;
     float* rest = workspace + space.dz;
+    const int64_t lo = dz_pieces(m, n, k, d->dtype, d->act) == 2 ? m * n : 0;
     if (n > 0 && ((!plain && (d->dx || d->dw)) || d->db)) {
         const int rc = dense_dz_pass(d->dy, d->z, m, n, d->dtype, d->act, d->act_cst, plain || !(d->dx || d->dw) ? nullptr : workspace,
-                                     d->db, rest, s);
+                                     d->dx || d->dw ? lo : 0, d->db, rest, s);
         if (rc) return rc;
     }
     tfc_dense_desc g{};
@@ -815,7 +906,7 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
         g.a = dz, g.lda = n, g.a_along_k = 1;
         g.b = d->w, g.ldb = d->ldw, g.b_along_k = !d->w_along_k;
         g.c = d->dx, g.ldc = k;
-        const int rc = tfc_dense(&g, rest, space.rest, stream);
+        const int rc = dense_product(&g, 2 * lo, 0, rest, space.rest, stream);
         if (rc) return rc;
     }
     if (d->dw) {  // x^T dz, or its transpose, in the weight's own order
@@ -828,7 +919,7 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
             g.a = d->x, g.lda = d->ldx, g.b = dz, g.ldb = n;
         }
         g.c = d->dw, g.ldc = g.n;
-        return tfc_dense(&g, rest, space.rest, stream);
+        return dense_product(&g, d->w_along_k ? 2 * lo : 0, d->w_along_k ? 0 : 2 * lo, rest, space.rest, stream);
     }
     return TFC_OK;
 }

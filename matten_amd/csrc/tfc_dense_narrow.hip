@@ -8,7 +8,8 @@
 // LDS, dx = dz W^T goes out, and x^T dz stays in the accumulators over all tiles; one partial result a workgroup, joined in a
 // fixed order (tfc_join_columns).  The next tile's x and dy are in flight meanwhile.
 //
-// LDS holds x, dz and W as [64][64] images of 16-bit elements (fp32: three of them, the bf16 pieces), 16-byte units swizzled by
+// LDS holds x, dz and W as [64][64] images of 16-bit elements (fp32: three of them, the bf16 pieces; dz of 16-bit types: two pieces, which
+// costs nothing here and makes the gradients as good as their own rounding), 16-byte units swizzled by
 // the row, so that both ways of reading are served by one image: eight neighbours of a row in one access, or four rows of a
 // column by the transposing read.  fp32: 72 KB, two workgroups on a CU.
 #include "tfc_dense_act.h"
@@ -54,7 +55,7 @@ __device__ __forceinline__ uintx4 frag_col(const uint16_t* im, int c0, int r0) {
     return __builtin_bit_cast(uintx4, both);
 }
 
-// Eight (four) neighbours of a row into the image(s); c a multiple of 8 (4).
+// Eight neighbours of a row into the image(s) of x or W; c a multiple of 8.
 template <class T>
 __device__ __forceinline__ void put8(uint16_t* im, int row, int c, const float (&v)[8]) {
     if constexpr (std::is_same<T, float>::value) {
@@ -66,6 +67,7 @@ __device__ __forceinline__ void put8(uint16_t* im, int row, int c, const float (
         *(uintx4*)(im + at(row, c)) = tfc_pack<T, 8>(v);
     }
 }
+// Four neighbours of a row into the images of dz; c a multiple of 4.
 template <class T>
 __device__ __forceinline__ void put4(uint16_t* im, int row, int c, const float (&v)[4]) {
     if constexpr (std::is_same<T, float>::value) {
@@ -76,6 +78,10 @@ __device__ __forceinline__ void put4(uint16_t* im, int row, int c, const float (
         *(tfc_u32x2*)(im + 2 * IMAGE + at(row, c)) = tfc_u32x2{u.l[0], u.l[1]};
     } else {
         *(tfc_u32x2*)(im + at(row, c)) = tfc_pack<T, 4>(v);
+        float lo[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) lo[j] = second_piece(T(), v[j]);
+        *(tfc_u32x2*)(im + IMAGE + at(row, c)) = tfc_pack<T, 4>(lo);
     }
 }
 
@@ -88,11 +94,12 @@ __device__ __forceinline__ void terms(const uintx4 (&a)[P], const uintx4 (&b)[P]
 
 template <class T>
 __global__ __launch_bounds__(256, 2) void tfc_dense_narrow_bwd_kernel(const Narrow g) {
-    constexpr int P = Pieces<T>::N;
-    __shared__ __attribute__((aligned(16))) uint16_t lds[(3 * P * IMAGE > 4 * IMAGE ? 3 * P * IMAGE : 4 * IMAGE)];
+    constexpr int P = Pieces<T>::N, D = P == 3 ? 3 : 2;  // pieces of x and W; of dz
+    __shared__ __attribute__((aligned(16))) uint16_t lds[(2 * P + D) * IMAGE];
     uint16_t *wi = lds, *xi = lds + P * IMAGE, *di = lds + 2 * P * IMAGE;
-    static_assert(2 * P * IMAGE * 2 >= S * S * 4, "dx passes through the images of x and dz");
+    static_assert((P + D) * IMAGE * 2 >= S * S * 4, "dx passes through the images of x and dz");
     const int t = threadIdx.x, lane = t & 63, wave = t >> 6, half = lane >> 5;
+    constexpr float LO = std::is_same<T, tfc_f16>::value ? 1.f / TFC_LO_SCALE : 1.f;
     const int r32 = (wave >> 1) * 32, c32 = (wave & 1) * 32;  // the wave's quarter of every 64 x 64 product
     // ---- weights, once: image [k][n]
 #pragma unroll
@@ -126,7 +133,7 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_narrow_bwd_kernel(const Narr
             rd[q] = tfc_load_left<T, 4>((const T*)g.dy + row * g.n + c, row < g.m ? g.n - c : 0);
         }
     };
-    floatx16 dw = floatx16(0.f);
+    floatx16 dw = floatx16(0.f), dw_lo = floatx16(0.f);  // (16 bits: products with the second pieces of dz apart)
     float db[16];
 #pragma unroll
     for (int q = 0; q < 16; ++q) db[q] = 0.f;
@@ -181,21 +188,32 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_narrow_bwd_kernel(const Narr
             put4<T>(di, r32 + (lane & 31), c32 + 8 * q + half * 4, v);
         }
         __syncthreads();
-        floatx16 dx = floatx16(0.f);
+        floatx16 dx = floatx16(0.f), dx_lo = floatx16(0.f);
 #pragma unroll
         for (int kk = 0; kk < S; kk += 16) {
-            uintx4 a[P], b[P];
+            uintx4 w[P], d[D];
             if (g.dx) {  // rows r32.., columns (of k) c32..
 #pragma unroll
-                for (int p = 0; p < P; ++p) a[p] = frag_row(wi + p * IMAGE, c32, kk), b[p] = frag_row(di + p * IMAGE, r32, kk);
-                terms<T, P>(a, b, dx);
+                for (int p = 0; p < P; ++p) w[p] = frag_row(wi + p * IMAGE, c32, kk);
+#pragma unroll
+                for (int p = 0; p < D; ++p) d[p] = frag_row(di + p * IMAGE, r32, kk);
+                if constexpr (P == 3)
+                    terms<T, P>(w, d, dx);
+                else
+                    dx_lo = mma(T(), w[0], d[1], dx_lo), dx = mma(T(), w[0], d[0], dx);
             }
             if (g.want_dw) {  // rows (of k) r32.., columns c32..
 #pragma unroll
-                for (int p = 0; p < P; ++p) a[p] = frag_col(di + p * IMAGE, c32, kk), b[p] = frag_col(xi + p * IMAGE, r32, kk);
-                terms<T, P>(a, b, dw);
+                for (int p = 0; p < P; ++p) w[p] = frag_col(xi + p * IMAGE, r32, kk);
+#pragma unroll
+                for (int p = 0; p < D; ++p) d[p] = frag_col(di + p * IMAGE, c32, kk);
+                if constexpr (P == 3)
+                    terms<T, P>(d, w, dw);
+                else
+                    dw_lo = mma(T(), d[1], w[0], dw_lo), dw = mma(T(), d[0], w[0], dw);
             }
         }
+        if constexpr (P == 1) dx += dx_lo * LO;
         if (!g.dx) continue;
         // dx through LDS ([64][64] floats where x and dz lay, units swizzled), out in whole rows
         __syncthreads();
@@ -222,6 +240,7 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_narrow_bwd_kernel(const Narr
         }
     }
     // ---- partial sums
+    if constexpr (P == 1) dw += dw_lo * LO;
     float* part = g.part + (long)blockIdx.x * ((long)g.k * g.n + g.n);
     if (g.want_dw) {
         const int k = r32 + (lane & 31);

@@ -2030,9 +2030,9 @@ def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0,
     if not a_along_k and not along_n:
         a, lda, a_along_k = a.contiguous(), max(k, 1), True
     c = torch.empty(m, n, dtype=a.dtype, device=a.device)
-    z = torch.empty_like(c) if keep_z else None
     L = _lib.lib()
     dt = _dtype_codes[a.dtype]
+    z = torch.empty(L.tfc_dense_z_bytes(m, n, dt), dtype=torch.uint8, device=a.device) if keep_z else None
     d = _lib.DenseDesc(m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, c.data_ptr(), max(n, 1), _at(bias), _at(residual), max(n, 1), _at(z),
                        alpha, cst, act, dt, a_along_k, not along_n)
     with _on(a.device):
@@ -2064,7 +2064,7 @@ def _dense_bwd_run(g, x, w, b, z, act: int, alpha: float, cst: float, need):
 
 
 class _DenseFn(torch.autograd.Function):
-    """x [m, k], w [k, n]; the pre-activation is kept, in x's type, where the backward kernels want it."""
+    """x [m, k], w [k, n]; the pre-activation is kept where the backward kernels want it."""
 
     @staticmethod
     def forward(ctx, x, w, b, r, act: int, alpha: float, cst: float):
@@ -2123,10 +2123,12 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
 
     Sums are fp32 and the epilogue is applied to them before the one rounding to the result's type.  fp32 operands are cut into
     three bf16 pieces, which loses nothing, but an operand that is not finite gives NaN.  Results are the same from run to
-    run.  For the backward pass the pre-activation is kept in x's type (layers of at most 64 x 64 form it again); the gradient
-    at it is rounded to x's type before the two products that need it, as the matrix instruction takes it.  Differentiable to any order: the first-order backward
-    is fused, a backward that is itself differentiated (`create_graph=True`) goes through torch's activations and this
-    kernel's products."""
+    run.  For the backward pass the pre-activation is kept (bf16: to 11 significant bits, fp16: to 16; layers of at most
+    64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces, and
+    rounded to x's type where x, the weight and y all have 2^14 elements or more.  Operand rows of 2^22 elements and more are refused.
+
+    Differentiable to any order: the first-order backward is fused, a backward that is itself differentiated
+    (`create_graph=True`) goes through torch's activations and this kernel's products."""
     _floats(x, "x")
     _floats(weight, "weight", x)
     if act not in _lib.DENSE_ACT:

@@ -5,7 +5,9 @@ fp32: fp32 operands lose at most 2^-24 |a b| of a product (the dropped pieces: t
 instruction rounds the running sum once, 6 for each 16 of k, with at most 1024 partial sums joined on top: (3 + 6 k / 16 + 64) u of
 sum |a b| at worst.  That worst case grows with k like no random sum does, but it is proven; k stays below 5000 where it matters.
 Behind the sum come alpha, bias, activation, constant and residual: under 16 roundings of the largest of them, the activation with a
-few u of its own.  In the backward pass of a 16-bit call z and dz are rounded to the type (2 h, with act'' to carry the first)."""
+few u of its own.  In the backward pass of a 16-bit call z is kept in fp16 (bf16: 2^-12, or 2^-24 absolute) or cut to 24 bits
+(fp16: 2^-15), carried by act'', and dz is rounded to the type (h), or in two
+pieces where x, the weight or y has less than 2^14 elements (h^2)."""
 import math
 
 import pytest
@@ -83,13 +85,15 @@ def _check(x, w, b, r, dy, act, alpha, cst=1.0):
     want = cst * a + (0 if r is None else r.detach().double())
     _close("y", y, want, ey + 4 * U * (want.abs() + (cst * a).abs()))
     dz = cst * da * G
-    edz = abs(cst) * G.abs() * (dda * (ez + h * z.abs()) + 16 * U * (1 + z.abs())) + 4 * U * dz.abs()
+    kept = {torch.float32: 0 * z, torch.bfloat16: 2.0**-12 * z.abs() + 2.0**-24, torch.float16: 2.0**-15 * z.abs()}[x.dtype]
+    edz = abs(cst) * G.abs() * (dda * (ez + kept) + 16 * U * (1 + z.abs())) + 4 * U * dz.abs()
     if act != "identity":
-        edz = edz + h * (dz.abs() + edz)
-        if x.dtype == torch.float16:
-            edz = edz + 2.0**-25
+        rounded = min(m * k, k * n, m * n) >= 2**14 and max(k, n) > 64
+        edz = edz + (h if rounded else h * h) * (dz.abs() + edz)
+        if x.dtype == torch.float16:  # (and half the least step)
+            edz = edz + 2.0 ** (-25 if rounded else -36)
     if act == "abs":  # the sign of a z within its error of zero is either
-        edz = torch.where(z.abs() <= ez + 2.0**-20, 2 * abs(cst) * G.abs(), edz)
+        edz = torch.where(z.abs() <= ez, 2 * abs(cst) * G.abs(), edz)
     c = abs(alpha)
     _close("dx", grads["dx"], alpha * (dz @ W.t()), c * (_sum_bound(dz.abs() + edz, W.t(), n) + edz @ W.t().abs()) + 4 * U * c * (dz.abs() @ W.t().abs()))
     _close("dw", grads["dw"], alpha * (X.t() @ dz), c * (_sum_bound(X.t(), dz.abs() + edz, m) + X.t().abs() @ edz) + 4 * U * c * (X.t().abs() @ dz.abs()))
@@ -119,6 +123,8 @@ def test_activations(device, dt, act):
     _check(x, w, b, None, dy, act, 3.0)  # large arguments
     _check(x, w, None, r, dy, act, 1e-3)  # small ones
     _check(x, w, None, None, dy, act, 0.1, -0.5)
+    _check(x, w, None, None, dy, act, 2.0**-40)  # below and beyond the range of 16 bits
+    _check(x, w, None, None, dy, act, 2.0**20, 2.0**-20)
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -401,6 +407,8 @@ def test_refusals(device):
     assert L.tfc_dense(make(a_along_k=0, b_along_k=1), None, 0, None) == -2
     assert L.tfc_dense(make(m=64, n=64, k=1 << 20, ldc=64), None, 0, None) == -1 and b"workspace" in L.tfc_last_error()
     assert L.tfc_dense(None, None, 0, None) == -1
+    with pytest.raises(_lib.TfcError, match="2\\^22"):
+        ops.dense(torch.zeros(2, 1 << 22, device=device), torch.zeros(1 << 22, 1, device=device))
     g = torch.zeros(3, 4, device=device)
     bwd = lambda **kw: _lib.DenseBwdDesc(**{**dict(m=3, n=4, k=80, x=x.data_ptr(), ldx=0, w=w.data_ptr(), ldw=0, dy=g.data_ptr(),  # noqa: E731
                                                    db=c.data_ptr(), alpha=1.0, act_cst=1.0, act=2, dtype=0), **kw})
