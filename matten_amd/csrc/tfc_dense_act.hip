@@ -433,13 +433,15 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_kernel(const Args g) {
 
 // ------------------------------------------------------------------------------------------------ large 16-bit products
 // 256 x 256 tile of eight waves (2 x 4, 128 x 64 of C each: eight 32 x 32 products for six operand reads).  The operands of a step of
-// 32 go straight from memory to LDS, three steps ahead of the one that is multiplied (four images of 32 KB, one barrier a
-// step): what bounds the kernel above on large products is the wait for operands one step ahead, at half the matrix rate.
+// 64 go straight from memory to LDS while the step before is multiplied (two images of 64 KB, one barrier a step): what bounds
+// the kernel above on large products is the wait for operands on their way through registers.  A step of 64 and not 32: a
+// row's part of it is a whole line of 128 bytes (16384 x 4096 x 1024 along k: 128 us with steps of 32, three of them in flight,
+// 121 with steps of 64).  A wave reads the operands of the next 16 k between the products of this one (121 -> 115).
 // Rows of an image have no padding (a wave's 64 x 16 bytes land side by side); their 16-byte units are swizzled by which unit a lane
-// asks memory for, so that the reads meet all banks: along k, unit ^ (row / 2 % 4); along the rows, 64-byte part ^ (k % 4).
+// asks memory for, so that 16 lanes of a read meet all banks: along k, unit ^ (row / 2 % 8); along the rows, 64-byte part ^ (k % 4).
 // Operands start at multiples of 16 bytes, have strides and, along the rows, sizes of multiples of 8; the contraction is a
-// multiple of 32.  Rows behind the last one are the last one again.
-constexpr int DEEP = 256, DEEP_K = 32, DEEP_IMAGE = DEEP * DEEP_K;
+// multiple of 64.  Rows behind the last one are the last one again.
+constexpr int DEEP = 256, DEEP_K = 64, DEEP_IMAGE = DEEP * DEEP_K;
 
 // 16 bytes a lane from base + off to `to` + 16 lane.  Written out, because for the transposing LDS reads the compiler cannot tell the
 // image being filled from the one being read and waits for every access of the wave; nothing is loaded into registers, and
@@ -451,18 +453,18 @@ __device__ __forceinline__ void memory_to_lds(const char* base, uint32_t off, ui
 
 template <class T, bool ALONG_K>
 struct DeepStage {
-    uint32_t off[2];  // bytes, of this lane's two accesses a step
+    uint32_t off[4];  // bytes, of this lane's four accesses a step
     const char* base;
     long adv;
 
     __device__ __forceinline__ void start(const Operand& o, long r0, long rows, long k0) {
         const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, last = (int)(rows < DEEP ? rows : DEEP) - 1;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
+        for (int i = 0; i < 4; ++i) {
             uint32_t r, k;
             if constexpr (ALONG_K) {
-                const int row = (i * 8 + wave) * 16 + lane / 4;
-                r = min(row, last), k = ((lane & 3) ^ ((row >> 1) & 3)) * 8;
+                const int row = (i * 8 + wave) * 8 + lane / 8;
+                r = min(row, last), k = ((lane & 7) ^ ((row >> 1) & 7)) * 8;
                 off[i] = 2u * (r * (uint32_t)o.ld + k);
             } else {
                 k = (i * 8 + wave) * 2 + lane / 32;
@@ -476,14 +478,14 @@ struct DeepStage {
     __device__ __forceinline__ void load(uint16_t* image) {
         const int wave = tfc_uniform(threadIdx.x >> 6);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) memory_to_lds(base, off[i], image + (i * 8 + wave) * 512);
+        for (int i = 0; i < 4; ++i) memory_to_lds(base, off[i], image + (i * 8 + wave) * 512);
         base += adv;
     }
     static __device__ __forceinline__ uintx4 fragment(const uint16_t* im, int r0, int kk) {
         const int lane = threadIdx.x & 63;
         if constexpr (ALONG_K) {
             const int r = r0 + (lane & 31), u = kk / 8 + (lane >> 5);
-            return *(const uintx4*)(im + r * DEEP_K + ((u ^ ((r >> 1) & 3)) << 3));
+            return *(const uintx4*)(im + r * DEEP_K + ((u ^ ((r >> 1) & 7)) << 3));
         }
         const int k = kk + (lane >> 5) * 8 + ((lane & 15) >> 2), r = r0 + ((lane >> 4) & 1) * 16 + (lane & 3) * 4;
         const uint16_t* q = im + k * DEEP + (((r >> 5) ^ (k & 3)) << 5) + (r & 31);  // (k + 4: the same swizzle)
@@ -497,7 +499,7 @@ struct DeepStage {
 
 template <class T, bool AK, bool BK, bool SPLIT>
 __global__ __launch_bounds__(512, 2) void tfc_dense_deep_kernel(const Args g) {
-    __shared__ __attribute__((aligned(16))) uint16_t s0[2 * DEEP_IMAGE], s1[2 * DEEP_IMAGE], s2[2 * DEEP_IMAGE], s3[2 * DEEP_IMAGE];
+    __shared__ __attribute__((aligned(16))) uint16_t s0[2 * DEEP_IMAGE], s1[2 * DEEP_IMAGE];
     const long tile = tile_of(g);
     const long m0 = (tile >> 32) * DEEP, n0 = (tile & 0xFFFFFFFF) * DEEP;
     const long k0 = SPLIT ? (long)blockIdx.y * g.k_split : 0;
@@ -521,44 +523,52 @@ __global__ __launch_bounds__(512, 2) void tfc_dense_deep_kernel(const Args g) {
         }
     };
     auto multiply = [&](const uint16_t* s) {
+        uintx4 fa[2][4], fb[2][2];
+        auto read = [&](int q) {
 #pragma unroll
-        for (int kk = 0; kk < DEEP_K; kk += 16) {
-            uintx4 fa[4], fb[2];
+            for (int j = 0; j < 2; ++j) fb[q & 1][j] = DeepStage<T, BK>::fragment(s + DEEP_IMAGE, wn + 32 * j, 16 * q);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) fa[i] = DeepStage<T, AK>::fragment(s, wm + 32 * i, kk);
+            for (int i = 0; i < 4; ++i) fa[q & 1][i] = DeepStage<T, AK>::fragment(s, wm + 32 * i, 16 * q);
+        };
+        read(0);
 #pragma unroll
-            for (int j = 0; j < 2; ++j) fb[j] = DeepStage<T, BK>::fragment(s + DEEP_IMAGE, wn + 32 * j, kk);
+        for (int q = 0; q < DEEP_K / 16; ++q) {
+            if (q + 1 < DEEP_K / 16) read(q + 1);
 #pragma unroll
             for (int i = 0; i < 4; ++i)
 #pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j] = mma(T(), fb[j], fa[i], acc[i][j]);
+                for (int j = 0; j < 2; ++j) acc[i][j] = mma(T(), fb[q & 1][j], fa[q & 1][i], acc[i][j]);
+        }
+        constexpr int READS = (AK ? 4 : 8) + (BK ? 2 : 4);  // of a part of 16
+        __builtin_amdgcn_sched_group_barrier(0x100, READS, 0);
+#pragma unroll
+        for (int q = 0; q < DEEP_K / 16; ++q) {
+            int left = q + 1 < DEEP_K / 16 ? READS : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                if (left > 0) __builtin_amdgcn_sched_group_barrier(0x100, READS > 8 ? 2 : 1, 0);
+                left -= READS > 8 ? 2 : 1;
+            }
         }
         --todo;
     };
-    // Every wave waits for its own accesses of the step in hand (at most those of the two steps behind it, four each, may be on their
-    // way) and for its reads of the image before, and then for the other waves; behind the barrier that image is free.
-#define TFC_DEEP_STEP(HERE, FREE)                                                \
-    if (todo > 2)                                                                \
-        asm volatile("s_waitcnt vmcnt(8) lgkmcnt(0)\n\ts_barrier" ::: "memory"); \
-    else                                                                         \
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); \
-    ask(FREE);                                                                   \
-    multiply(HERE);                                                              \
+    // Every wave waits for its own accesses of the step in hand and for its reads of the image before, and then for the other waves; behind
+    // the barrier that image is free.
+#define TFC_DEEP_STEP(HERE, FREE)                                            \
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory"); \
+    ask(FREE);                                                               \
+    multiply(HERE);                                                          \
     if (todo == 0) break;
     ask(s0);
-    ask(s1);
-    ask(s2);
     while (true) {
-        TFC_DEEP_STEP(s0, s3)
+        TFC_DEEP_STEP(s0, s1)
         TFC_DEEP_STEP(s1, s0)
-        TFC_DEEP_STEP(s2, s1)
-        TFC_DEEP_STEP(s3, s2)
     }
 #undef TFC_DEEP_STEP
     __syncthreads();
-    static_assert(2 * corner_floats(2) * 4 <= 4 * DEEP_IMAGE, "two waves' corners in an image pair");
-    uint16_t* part = (wave & 3) == 0 ? s0 : (wave & 3) == 1 ? s1 : (wave & 3) == 2 ? s2 : s3;
-    write_out<T, 4, 2, SPLIT>(g, acc, (float*)part + (wave >> 2) * corner_floats(2), m0 + wm, n0 + wn);
+    static_assert(4 * corner_floats(2) * 4 <= 4 * DEEP_IMAGE, "four waves' corners in an image pair");
+    write_out<T, 4, 2, SPLIT>(g, acc, (float*)(wave & 1 ? s1 : s0) + (wave >> 1) * corner_floats(2), m0 + wm, n0 + wn);
 }
 
 // 256 / W quads of columns x W walkers: walker w adds the parts w, w + W, ..., the walkers are joined in order.

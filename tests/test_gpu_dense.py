@@ -136,7 +136,7 @@ def test_large(device, dt, m, k, n):
 
 @pytest.mark.parametrize("dt", TYPES[1:])
 @pytest.mark.parametrize("transposed", [False, True])
-@pytest.mark.parametrize("m,k,n", [(4096, 512, 4096), (4128, 544, 4384)])
+@pytest.mark.parametrize("m,k,n", [(4096, 1024, 4096), (4160, 832, 4416)])
 def test_tiles_of_256(device, dt, transposed, m, k, n):
     """Sizes at which all three products take the kernel for large ones, whole tiles and edges."""
     _check(*_inputs(m, k, n, dt, m + k, device, transposed=transposed), "gelu", 1 / math.sqrt(k))
