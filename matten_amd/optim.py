@@ -116,6 +116,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: lr must be finite and not negative, got {lr}")
         if not (0.0 <= b1 < 1.0 and 0.0 <= b2 < 1.0):
             raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
+        if g.get("amsgrad") or g.get("maximize"):  # (a loaded state dict's)
+            raise ValueError("AdamW: `amsgrad` and `maximize` do not exist here")
         if not 0.0 <= g["eps"] < math.inf or not 0.0 <= g["weight_decay"] < math.inf:
             raise ValueError(f"AdamW: eps and weight_decay must be finite and not negative, got {g['eps']}, {g['weight_decay']}")
 
@@ -145,7 +147,10 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: state entry `{k}` must be a contiguous {dt} tensor of {n} elements on {p.device}; got {got}")
 
     def load_state_dict(self, state_dict):
-        """Takes copies.  The moments must have this optimizer's width and the parameters' sizes."""
+        """Takes copies.  The moments must have this optimizer's width and the parameters' sizes; those of torch.optim.AdamW fit
+        32 bits where the parameters are fp32."""
+        for g in state_dict["param_groups"]:
+            self._check_group(g)
         names = _STATE[self.state_bits]
         ids = [i for g in state_dict["param_groups"] for i in g["params"]]
         params = [p for g in self.param_groups for p in g["params"]]

@@ -310,6 +310,34 @@ def test_state_and_storage_that_are_replaced(device):
         _same(opt, p, r)
 
 
+def test_state_dict_of_torch(device):
+    from matten_amd import optim
+
+    mine = _tensors([300, 33], torch.float32, device, 17)
+    other = [torch.nn.Parameter(p.detach().clone()) for p in mine]
+    theirs = torch.optim.AdamW(other, lr=3e-3, betas=(0.8, 0.99), weight_decay=0.1)
+    for k in range(3):
+        _grads(other, 110 + k)
+        theirs.step()
+    opt = optim.AdamW(mine)
+    opt.load_state_dict(theirs.state_dict())
+    assert all(int(opt.state[p]["step"]) == 3 for p in mine)
+    with torch.no_grad():
+        for p, q in zip(mine, other):
+            p.copy_(q)
+    for k in range(2):
+        _grads(other, 120 + k)
+        for p, q in zip(mine, other):
+            p.grad = q.grad.clone()
+        theirs.step(), opt.step()
+    for p, q in zip(mine, other):  # the same 12 roundings of 2^-24, in another order, of values up to |p| + lr
+        assert (p - q).abs().max() <= 2 * 2 * 12 * 2.0**-24 * (1 + q.abs().max())
+    for key in ("amsgrad", "maximize"):
+        with pytest.raises(ValueError, match="do not exist"):
+            opt.load_state_dict(torch.optim.AdamW(other, **{key: True}).state_dict())
+    assert opt.param_groups[0]["betas"] == (0.8, 0.99)
+
+
 def test_state_storage_that_moves(device):
     """State whose storage is taken away and brought back between steps (`.data`, as programs do that keep it on the host
     meanwhile), and a state dict that went through a file that loads without executing anything."""
