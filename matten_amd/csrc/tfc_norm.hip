@@ -7,6 +7,8 @@
 // rows, so that no lane idles at d = 32, or a whole workgroup - each holding NV vectors of 16 bytes.  Lanes keep their
 // columns of w and b in registers over all rows they visit.  The backward pass also keeps the column sums of dw and db there:
 // a fixed number of workgroups walks the rows and writes one partial row each; tfc_join_columns adds them in a fixed order.
+// Measured: 65536 x 1024 in bf16 46 us forward (5.8 TB/s, some of it from the last-level cache), 79 + 4 backward (5.1 TB/s); 6911 x
+// 1001 in fp32 (rows that start anywhere) 11.4 and 17.4 + 4.8 (4.8 TB/s); 2048 x 64 3.7 and 5.0 + 2.2, launches.
 #include "tfc_types.h"
 
 #include <algorithm>
