@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes as C
 import math
+from operator import is_
 from typing import Iterable, Optional
 
 import torch
@@ -190,8 +191,9 @@ class AdamW(torch.optim.Optimizer):
             self._check_group(g)  # (schedulers and users write to groups)
         if self._tables is not None:
             tables, rest, groups = self._tables
-            if (groups == [(id(g), len(g["params"])) for g in self.param_groups] and all(t.holds(self.state) for t in tables)
-                    and all(p.grad is None for p in rest)):
+            if (len(groups) == len(self.param_groups)
+                    and all(g is h and len(g["params"]) == len(ps) and all(map(is_, g["params"], ps)) for (h, ps), g in zip(groups, self.param_groups))
+                    and all(t.holds(self.state) for t in tables) and all(p.grad is None for p in rest)):
                 return tables
         tables, rest, first = [], [], 0
         for g in self.param_groups:
@@ -209,7 +211,7 @@ class AdamW(torch.optim.Optimizer):
             if at < end:
                 raise ValueError("AdamW: two parameters share memory")
             end = at + n
-        self._tables = tables, rest, [(id(g), len(g["params"])) for g in self.param_groups]
+        self._tables = tables, rest, [(g, list(g["params"])) for g in self.param_groups]
         return tables
 
     def _table(self, group, device, params, indexes) -> _Table:
@@ -265,12 +267,12 @@ class AdamW(torch.optim.Optimizer):
                     at += 8 * n
         for t in tables:
             g = t.group
-            h = _lib.AdamwHyper(beta1=g["betas"][0], beta2=g["betas"][1], eps=g["eps"], weight_decay=g["weight_decay"],
+            h = _lib.AdamwHyper(beta1=float(g["betas"][0]), beta2=float(g["betas"][1]), eps=float(g["eps"]), weight_decay=float(g["weight_decay"]),
                                 max_norm=self.max_grad_norm if n_partials else 0.0, seed=self.seed)
             if isinstance(g["lr"], torch.Tensor):
                 h.lr_device = g["lr"].data_ptr()
             else:
-                h.lr = g["lr"]
+                h.lr = float(g["lr"])
             with ops._on(t.device):
                 ws = torch.empty(L.tfc_adamw_workspace_bytes(len(t.rows)), dtype=torch.uint8, device=t.device)
                 _lib.check(L.tfc_adamw_step(t.rows, len(t.rows), ops._dtype_codes[t.dtype], self.state_bits, C.byref(h), ops._at(partials),

@@ -7,6 +7,7 @@ import copy
 import io
 import math
 
+import numpy as np
 import pytest
 import torch
 
@@ -300,6 +301,19 @@ def test_state_and_storage_that_are_replaced(device):
                 r.step(p.grad)
             _same(opt, p, r)
         assert all(bool((j == 7.0).all()) for j in junk)
+    swapped = _tensors([params[0].numel()], torch.float32, device, 18)[0]  # another parameter in its place
+    old, opt.param_groups[0]["params"][0] = params[0].detach().clone(), swapped
+    refs[0], kept = Reference(swapped, 0, 32), params[0]
+    opt.param_groups[0]["lr"] = np.float32(1e-3)
+    for r in refs:
+        r.lr = float(np.float32(1e-3))
+    params = [swapped, *params[1:]]
+    _grads(params, 89)
+    opt.step()
+    for p, r in zip(params, refs):
+        r.step(p.grad)
+        _same(opt, p, r)
+    assert torch.equal(kept, old)
     more = _tensors([60], torch.float32, device, 15)
     opt.add_param_group({"params": more, "lr": 0.5})
     refs.append(Reference(more[0], 3, 32, lr=0.5))
