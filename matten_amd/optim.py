@@ -26,6 +26,11 @@ _STATE = {  # state entry -> dtype, by the width of the moments ("step" besides)
 }
 
 
+# (unbound: a step asks for these of every tensor, and host time is what a step of a small model costs)
+_address, _numel, _device, _packed = torch.Tensor.data_ptr, torch.Tensor.numel, torch.Tensor.get_device, torch.Tensor.is_contiguous
+_type, _layout = torch.Tensor.dtype.__get__, torch.Tensor.layout.__get__
+
+
 class _Table:
     """The descriptors of the tensors one call steps: everything but the gradients' addresses is set once."""
 
@@ -33,11 +38,12 @@ class _Table:
         self.group, self.params, self.states = group, params, states
         self.device, self.dtype = params[0].device, params[0].dtype
         self.entries = [t for st in states for t in st.values()]  # (alive as long as their addresses are used)
-        self.at = [t.data_ptr() for t in (*params, *self.entries)]
+        self.at = list(map(_address, (*params, *self.entries)))
         self.sizes = [p.numel() for p in params]
         self.rows = (_lib.AdamwTensor * len(params))()
+        self.each = list(self.rows)
         names = list(_STATE[bits])
-        for row, p, st, i in zip(self.rows, params, states, indexes):
+        for row, p, st, i in zip(self.each, params, states, indexes):
             row.p, row.n, row.index, row.step = p.data_ptr(), p.numel(), i, st["step"].data_ptr()
             if bits == 32:
                 row.m, row.v = (st[k].data_ptr() for k in names)
@@ -52,8 +58,8 @@ class _Table:
                 return False
             entries += st.values()
         try:
-            return [t.data_ptr() for t in (*self.params, *entries)] == self.at
-        except AttributeError:  # (not a tensor: for _check_state to name)
+            return list(map(_address, (*self.params, *entries))) == self.at
+        except TypeError:  # (not a tensor: for _check_state to name)
             return False
 
 
@@ -240,15 +246,18 @@ class AdamW(torch.optim.Optimizer):
             lr = t.group["lr"]
             if isinstance(lr, torch.Tensor) and lr.device != t.device:
                 raise RuntimeError(f"AdamW: the lr tensor is on {lr.device}, the parameters on {t.device}")
-            for row, p, n in zip(t.rows, t.params, t.sizes):
-                g = p.grad
-                if g.dtype != dtype or g.layout != torch.strided or g.get_device() != at or g.numel() != n:
-                    raise RuntimeError(f"AdamW: a gradient must be a dense {dtype} tensor of shape {tuple(p.shape)} on {t.device}; got "
-                                       f"{g.dtype}, {tuple(g.shape)}, {g.layout} on {g.device}")
-                if not g.is_contiguous():
-                    g = g.contiguous()
-                    copies.append(g)
-                row.g = g.data_ptr()
+            grads = [p.grad for p in t.params]
+            if set(map(_type, grads)) != {dtype} or set(map(_layout, grads)) != {torch.strided} or set(map(_device, grads)) != {at} \
+                    or list(map(_numel, grads)) != t.sizes:
+                p, g = next((p, g) for p, g, n in zip(t.params, grads, t.sizes)
+                            if g.dtype != dtype or g.layout != torch.strided or g.get_device() != at or g.numel() != n)
+                raise RuntimeError(f"AdamW: a gradient must be a dense {dtype} tensor of shape {tuple(p.shape)} on {t.device}; got "
+                                   f"{g.dtype}, {tuple(g.shape)}, {g.layout} on {g.device}")
+            if not all(map(_packed, grads)):
+                grads = [g.contiguous() for g in grads]
+                copies += grads
+            for row, address in zip(t.each, map(_address, grads)):
+                row.g = address
         L = _lib.lib()
         partials, n_partials = None, 0
         self.grad_norm = None
