@@ -611,7 +611,7 @@ typedef struct tfc_dense_desc {
     int32_t act, dtype, a_along_k, b_along_k;
 } tfc_dense_desc;
 
-int64_t tfc_dense_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype);
+int64_t tfc_dense_workspace_floats(const tfc_dense_desc* desc);
 int tfc_dense(const tfc_dense_desc* desc, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
 typedef struct tfc_dense_bwd_desc {
     int64_t m, n, k;

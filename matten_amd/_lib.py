@@ -235,7 +235,7 @@ SIGNATURES = {
     "tfc_layer_norm_fwd": (C.c_int, [_P, _P, _P, _I64, _I64, _F, _I32, _P, _P, _P, _P]),
     "tfc_layer_norm_bwd_workspace_floats": (_I64, [_I64, _I64, _I32]),
     "tfc_layer_norm_bwd": (C.c_int, [_P, _P, _P, _P, _P, _I64, _I64, _I32, _P, _P, _P, _P, _I64, _P]),
-    "tfc_dense_workspace_floats": (_I64, [_I64, _I64, _I64, _I32]),
+    "tfc_dense_workspace_floats": (_I64, [C.POINTER(DenseDesc)]),
     "tfc_dense": (C.c_int, [C.POINTER(DenseDesc), _P, _I64, _P]),
     "tfc_dense_keeps_z": (C.c_int, [_I64, _I64, _I32]),
     "tfc_dense_z_bytes": (_I64, [_I64, _I64, _I32]),

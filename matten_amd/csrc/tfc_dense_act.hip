@@ -18,7 +18,7 @@
 //
 // Measured, with the library's product of the same sizes without an epilogue: fp32 6912 x 511 x 2048 118 us (library 157), with bias, ssp
 // and z 132, its gradients' products 106 and 98 (169, 125); bf16 16384 x 1024 x 4096 173 us (139), with gelu, z and residual 240,
-// its gradients' 119 and 130 (98, 197); bf16 1 x 4096 x 4096 12.5 us of kernels for 7.1 us of weights.
+// its gradients' 119 and 130 (98, 197); bf16 1 x 4096 x 4096 7.3 us for 7.1 us of weights.
 //
 // Few tiles and a long contraction (a weight's gradient over many rows): the contraction is split, partial tiles go to the
 // workspace and a second kernel adds them in order and applies the epilogue.
@@ -575,6 +575,153 @@ __global__ __launch_bounds__(512, 2) void tfc_dense_deep_kernel(const Args g) {
     write_out<T, 4, 2, SPLIT>(g, acc, (float*)(wave & 1 ? s1 : s0) + (wave >> 1) * corner_floats(2), m0 + wm, n0 + wn);
 }
 
+// ------------------------------------------------------------------------------------------------ a few rows
+// At most ROWS rows (a single token): bound by reading B once.  One launch without partial results, where the tiles above, mostly empty,
+// split the contraction and join it in a second one (1 x 4096 x 4096 with B along k: bf16 12.9 -> 7.3 us, which is reading B at the speed of
+// a copy, fp32 28 -> 13; 4 rows 13.5 -> 9.3, 29 -> 14).  The products
+// are fp32 multiply-adds on the vector units, which up to four rows keep pace with memory.
+// B along k: a workgroup has COLS columns, its four waves take turns along the contraction; sums over the lanes, then the waves.
+// B along the rows: a workgroup has 128 bytes of every row (fp32; 16 bits: 64, so that there are workgroups enough) and 16 waves side by
+// side along the contraction.
+constexpr int ROWS = 4, COLS = 4, STRIP = 32;
+
+// Row r of A from k on: N elements as far as `left` goes, with their second pieces where there are any.
+template <class T, int N, bool WHOLE>
+__device__ __forceinline__ void row_part(const Args& g, int r, long k, long left, float (&x)[N]) {
+    const T* p = (const T*)g.a.p + min((long)r, g.m - 1) * g.a.ld + k;
+    tfc_unpack<T, N>(WHOLE ? tfc_load<T, N>(p) : tfc_load_left<T, N>(p, left), x);
+    if (sizeof(T) == 2 && g.lo_a) {
+        const T* q = (const T*)((const char*)p + g.lo_a);
+        float lo[N];
+        tfc_unpack<T, N>(WHOLE ? tfc_load<T, N>(q) : tfc_load_left<T, N>(q, left), lo);
+#pragma unroll
+        for (int j = 0; j < N; ++j) x[j] += lo[j] * (std::is_same<T, tfc_f16>::value ? 1.f / TFC_LO_SCALE : 1.f);
+    }
+}
+
+template <class T, int M>
+__global__ __launch_bounds__(256) void tfc_dense_rows_k_kernel(const Args g) {
+    constexpr int V = TfcType<T>::V, STEP = 4 * 64 * V;
+    __shared__ float lds[4][M * COLS];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const long n0 = (long)blockIdx.x * COLS;
+    const T* w[COLS];
+#pragma unroll
+    for (int c = 0; c < COLS; ++c) w[c] = (const T*)g.b.p + min(n0 + c, g.n - 1) * g.b.ld;
+    float acc[M][COLS];
+#pragma unroll
+    for (int r = 0; r < M; ++r)
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) acc[r][c] = 0.f;
+    auto part = [&](auto whole, long k) {
+        TfcRaw<T, V> raw[COLS];
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) raw[c] = whole ? tfc_load<T, V>(w[c] + k) : tfc_load_left<T, V>(w[c] + k, g.k - k);
+        float x[M][V];
+#pragma unroll
+        for (int r = 0; r < M; ++r) row_part<T, V, whole>(g, r, k, g.k - k, x[r]);
+#pragma unroll
+        for (int c = 0; c < COLS; ++c) {
+            float v[V];
+            tfc_unpack<T, V>(raw[c], v);
+#pragma unroll
+            for (int r = 0; r < M; ++r)
+#pragma unroll
+                for (int j = 0; j < V; ++j) acc[r][c] += x[r][j] * v[j];
+        }
+    };
+    const long mine = (long)(wave * 64 + lane) * V;
+    long k0 = 0;
+    for (; k0 + STEP <= g.k; k0 += STEP) part(std::true_type(), k0 + mine);
+    if (k0 + mine < g.k) part(std::false_type(), k0 + mine);
+    if constexpr (M * COLS == 16) {
+        float v[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = acc[i / COLS][i % COLS];
+        const float s = tfc_wave_reduce16(v);
+        if ((lane & 3) == 0) lds[wave][tfc_reduce16_index(lane)] = s;
+    } else {
+#pragma unroll
+        for (int r = 0; r < M; ++r) {
+            float v[4] = {acc[r][0], acc[r][1], acc[r][2], acc[r][3]};
+            const float s = tfc_wave_reduce4(v);
+            if ((lane & 15) == 0) lds[wave][r * COLS + tfc_reduce4_index(lane)] = s;
+        }
+    }
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t < M * COLS && t / COLS < g.m && n0 + t % COLS < g.n) {
+        float v[1] = {(lds[0][t] + lds[1][t]) + (lds[2][t] + lds[3][t])};
+        epilogue<T, 1>(g, t / COLS, n0 + t % COLS, v, residual<T, 1>(g, t / COLS, n0 + t % COLS));
+    }
+}
+
+template <class T, int M>
+__global__ __launch_bounds__(1024) void tfc_dense_rows_n_kernel(const Args g) {
+    constexpr int V = TfcType<T>::V, LC = STRIP / V, STEP = 1024 / LC * V;  // lanes side by side; a lane has V neighbouring k
+    __shared__ float lds[16][M * STRIP];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, cl = (threadIdx.x % LC) * V;
+    const long n0 = (long)blockIdx.x * STRIP, left = g.n - n0 - cl;
+    const T* w = (const T*)g.b.p + n0 + cl;
+    float acc[M][V];
+#pragma unroll
+    for (int r = 0; r < M; ++r)
+#pragma unroll
+        for (int j = 0; j < V; ++j) acc[r][j] = 0.f;
+    auto multiply = [&](TfcRaw<T, V> raw, const float (&x)[M][V], int u) {
+        float v[V];
+        tfc_unpack<T, V>(raw, v);
+#pragma unroll
+        for (int r = 0; r < M; ++r)
+#pragma unroll
+            for (int j = 0; j < V; ++j) acc[r][j] += x[r][u] * v[j];
+    };
+    long k = (long)(threadIdx.x / LC) * V;
+    if (g.n - n0 >= STRIP) {
+        for (; k + V <= g.k; k += STEP) {
+            TfcRaw<T, V> raw[V];
+#pragma unroll
+            for (int u = 0; u < V; ++u) raw[u] = tfc_load<T, V>(w + (k + u) * g.b.ld);
+            float x[M][V];
+#pragma unroll
+            for (int r = 0; r < M; ++r) row_part<T, V, true>(g, r, k, V, x[r]);
+#pragma unroll
+            for (int u = 0; u < V; ++u) multiply(raw[u], x, u);
+        }
+    }
+    for (; k < g.k; k += STEP) {
+        float x[M][V];
+#pragma unroll
+        for (int r = 0; r < M; ++r) row_part<T, V, false>(g, r, k, g.k - k, x[r]);
+#pragma unroll
+        for (int u = 0; u < V; ++u)
+            if (k + u < g.k) multiply(tfc_load_left<T, V>(w + (k + u) * g.b.ld, left), x, u);
+    }
+    // Sums over the lanes of a column: rows of 16 lanes pair by pair, each keeping half of the V columns, then inside the rows.
+    const int half = lane >> 5, odd = lane >> 4 & 1, p = lane & 15;
+#pragma unroll
+    for (int r = 0; r < M; ++r) {
+        float h[V / 2], q[V / 4];
+#pragma unroll
+        for (int j = 0; j < V / 2; ++j) h[j] = tfc_swap_add32(acc[r][j], acc[r][j + V / 2]);
+#pragma unroll
+        for (int j = 0; j < V / 4; ++j) {
+            q[j] = tfc_swap_add16(h[j], h[j + V / 4]);
+            q[j] += tfc_dpp<0x128>(q[j]);                        // row_ror:8
+            if constexpr (LC == 4) q[j] += tfc_dpp<0x124>(q[j]);  // row_ror:4
+            if (p < LC) lds[wave][r * STRIP + p * V + half * (V / 2) + odd * (V / 4) + j] = q[j];
+        }
+    }
+    __syncthreads();
+    const int t = threadIdx.x;
+    if (t < M * STRIP && t / STRIP < g.m && n0 + t % STRIP < g.n) {
+        float v[1] = {0.f};
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[0] += lds[i][t];
+        epilogue<T, 1>(g, t / STRIP, n0 + t % STRIP, v, residual<T, 1>(g, t / STRIP, n0 + t % STRIP));
+    }
+}
+
 // 256 / W quads of columns x W walkers: walker w adds the parts w, w + W, ..., the walkers are joined in order.
 template <class T, int W>
 __global__ __launch_bounds__(256) void tfc_dense_join_kernel(const Args g, int splits) {
@@ -715,6 +862,29 @@ Plan plan(int64_t m, int64_t n, int64_t k, int dtype, bool deep) {
     return p;
 }
 
+// Whether the kernels for a few rows are taken.  A workgroup's share of B grows with k: along k (16 bits, 16 columns of 16384: 4.4 us,
+// 9 with four rows; tiles 8) up to 32 KB a column.  Along the rows (16 bits, 4096 x 128: 6.1 us, 9 with four
+// rows, tiles 8; 4096 x 4096: 14.2, 17, tiles 12.9, 14.5; fp32 4096 x 4096: 19, 21, tiles 28; 8192 x 64: 12.5, 13, the same) up to 2048 of 16
+// bits, 4096 of fp32.
+bool few_rows(const tfc_dense_desc& d) {
+    const int64_t size = (int64_t)tfc_dtype_size(d.dtype);
+    return d.a_along_k && d.m <= ROWS && d.k > 0 && d.k <= (d.b_along_k ? (1 << 15) / size : 1024 * size);
+}
+
+template <class T, int M>
+int launch_rows(const Args& g, bool b_k, hipStream_t s) {
+    if (b_k)
+        hipLaunchKernelGGL((tfc_dense_rows_k_kernel<T, M>), dim3((unsigned)((g.n + COLS - 1) / COLS)), dim3(256), 0, s, g);
+    else
+        hipLaunchKernelGGL((tfc_dense_rows_n_kernel<T, M>), dim3((unsigned)((g.n + STRIP - 1) / STRIP)), dim3(1024), 0, s, g);
+    TFC_LAUNCH_CHECK("tfc_dense_rows");
+    return TFC_OK;
+}
+template <class T>
+int dense_rows(const Args& g, bool b_k, hipStream_t s) {
+    return g.m == 1 ? launch_rows<T, 1>(g, b_k, s) : g.m == 2 ? launch_rows<T, 2>(g, b_k, s) : launch_rows<T, ROWS>(g, b_k, s);
+}
+
 template <class T, bool AK, bool BK, int BM, int BN>
 int launch_tile(const Args& g, const Plan& p, hipStream_t s) {
     const dim3 grid((unsigned)(p.tiles_m * p.tiles_n), (unsigned)p.splits);
@@ -799,11 +969,18 @@ bool act_ok(int act) {
 
 }  // namespace
 
-extern "C" int64_t tfc_dense_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype) {
-    if (m <= 0 || n <= 0 || k <= 0 || !tfc_dtype_ok(dtype)) return 0;
+// For operands of any layout, aligned or not.
+static int64_t product_floats(int64_t m, int64_t n, int64_t k, int dtype) {
+    if (m <= 0 || n <= 0 || k <= 0) return 0;
     int64_t splits = plan(m, n, k, dtype, false).splits;
     if (deep_shape(m, n, k, dtype)) splits = std::max(splits, plan(m, n, k, dtype, true).splits);
     return splits > 1 ? splits * m * n : 0;
+}
+
+extern "C" int64_t tfc_dense_workspace_floats(const tfc_dense_desc* d) {
+    if (!d || d->m <= 0 || d->n <= 0 || d->k <= 0 || !tfc_dtype_ok(d->dtype) || few_rows(*d)) return 0;
+    const int64_t splits = plan(d->m, d->n, d->k, d->dtype, deep_operands(*d)).splits;
+    return splits > 1 ? splits * d->m * d->n : 0;
 }
 
 // lo_a, lo_b: bytes from an operand's first pieces to its second ones (0: there are none).
@@ -818,7 +995,8 @@ static int dense_product(const tfc_dense_desc* d, int64_t lo_a, int64_t lo_b, fl
     TFC_REQUIRE(d->a_along_k || !d->b_along_k, TFC_EUNSUPPORTED,
                 "tfc_dense: an A that runs along its rows needs a B that runs along its columns");
     TFC_REQUIRE(d->lda >= 0 && d->ldb >= 0 && d->ldc >= d->n && (!d->residual || d->ldr >= 0), TFC_EINVAL, "tfc_dense: bad stride");
-    const Plan p = d->k ? plan(d->m, d->n, d->k, d->dtype, !lo_a && !lo_b && deep_operands(*d)) : Plan{64, 64, 1, 1, 1, 0};
+    const bool few = few_rows(*d) && !lo_b;
+    const Plan p = d->k && !few ? plan(d->m, d->n, d->k, d->dtype, !lo_a && !lo_b && deep_operands(*d)) : Plan{64, 64, 1, 1, 1, 0};
     // (a thread's offset in a tile has 32 bits: 256 rows, or a step of 64, of the longest row)
     TFC_REQUIRE(d->lda < 1 << 22 && d->ldb < 1 << 22, TFC_EUNSUPPORTED, "tfc_dense: operand rows of 2^22 elements or more");
     TFC_REQUIRE(p.tiles_m * p.tiles_n < (int64_t)1 << 31, TFC_EUNSUPPORTED, "tfc_dense: %lld x %lld has too many tiles",
@@ -833,6 +1011,7 @@ static int dense_product(const tfc_dense_desc* d, int64_t lo_a, int64_t lo_b, fl
     g.c = d->c, g.ldc = d->ldc, g.bias = d->bias, g.res = d->residual, g.ldr = d->ldr, g.z = d->z;
     g.alpha = d->alpha, g.cst = d->act_cst, g.act = d->act, g.part = workspace;
     g.passes = lo_a || lo_b ? 2 : 1, g.lo_a = lo_a, g.lo_b = lo_b;
+    if (few) return TFC_BY_DTYPE(d->dtype, dense_rows, g, d->b_along_k != 0, s);
     return TFC_BY_DTYPE(d->dtype, dense, g, p, d->a_along_k != 0, d->b_along_k != 0, s);
 }
 
@@ -875,8 +1054,8 @@ static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int dtype, int act) {
     BwdSpace w{};
     if (act != TFC_ACT_IDENTITY) w.dz = (m * n * dz_pieces(m, n, k, dtype, act) * (int64_t)tfc_dtype_size(dtype) + 15) / 16 * 4;
     w.rest = std::max(m > 0 && n > 0 ? dz_plan(m, n, dtype).slabs * n : 0,
-                      std::max(tfc_dense_workspace_floats(m, k, n, dtype),
-                               std::max(tfc_dense_workspace_floats(k, n, m, dtype), tfc_dense_workspace_floats(n, k, m, dtype))));
+                      std::max(product_floats(m, k, n, dtype),
+                               std::max(product_floats(k, n, m, dtype), product_floats(n, k, m, dtype))));
     return w;
 }
 

@@ -2036,7 +2036,7 @@ def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0,
     d = _lib.DenseDesc(m, n, k, a.data_ptr(), lda, b.data_ptr(), ldb, c.data_ptr(), max(n, 1), _at(bias), _at(residual), max(n, 1), _at(z),
                        alpha, cst, act, dt, a_along_k, not along_n)
     with _on(a.device):
-        floats = L.tfc_dense_workspace_floats(m, n, k, dt)
+        floats = L.tfc_dense_workspace_floats(C.byref(d))
         ws = torch.empty(floats, dtype=torch.float32, device=a.device) if floats else None
         _lib.check(L.tfc_dense(C.byref(d), _at(ws), floats, _stream()))
     return c, z
@@ -2122,7 +2122,7 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
     fp16.  `act`: identity, ssp, silu, tanh, abs, sigmoid or gelu.
 
     Sums are fp32 and the epilogue is applied to them before the one rounding to the result's type.  fp32 operands are cut into
-    three bf16 pieces, which loses nothing, but an operand that is not finite gives NaN.  Results are the same from run to
+    three bf16 pieces, which loses nothing, but an operand that is not finite may give NaN for an infinity.  Results are the same from run to
     run.  For the backward pass the pre-activation is kept (bf16: to 11 significant bits, fp16: to 16; layers of at most
     64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces, and
     rounded to x's type where x, the weight and y all have 2^14 elements or more.  Operand rows of 2^22 elements and more are refused.

@@ -104,7 +104,8 @@ def _check(x, w, b, r, dy, act, alpha, cst=1.0):
 
 
 SIZES = [(1, 1, 1), (1, 7, 5), (2, 64, 3), (3, 33, 65), (31, 32, 31), (64, 64, 64), (65, 63, 66), (100, 129, 130), (127, 16, 257), (128, 256, 128),
-         (129, 255, 129), (300, 511, 200), (1, 4096, 1000), (17, 1000, 4096), (513, 40, 512)]
+         (129, 255, 129), (300, 511, 200), (1, 4096, 1000), (17, 1000, 4096), (513, 40, 512), (4, 4100, 129), (2, 9000, 70), (1, 1, 300),
+         (4, 640, 32), (3, 2047, 31)]
 
 
 @pytest.mark.parametrize("dt", TYPES)
@@ -182,6 +183,29 @@ def test_layouts(device):
         want = (dy.double() @ w.double().t()).sum(0)
         h = torch.finfo(dt).eps / 2
         assert ((g[0].double() - want).abs() <= (96 + 2) * h * (dy.double().abs() @ w.double().abs().t()).sum(0)).all()
+
+
+def test_a_few_rows(device):
+    """One to four rows: views give the bits of packed operands, more rows the same to rounding; both sides of the longest contraction."""
+    from matten_amd import ops
+
+    for dt in TYPES:
+        for m, k, n in [(1, 72, 80), (3, 1030, 33), (4, 2049, 65), (2, 20000, 40)]:
+            x, w, b, r, _ = _inputs(m, k, n, dt, 17 + m, device)
+            wide, wwide = torch.zeros(m, k + 28, dtype=dt, device=device), torch.zeros(k, n + 21, dtype=dt, device=device)
+            wide[:, 11 : k + 11], wwide[:, 3 : n + 3] = x, w
+            wt = w.t().contiguous()
+            tall = torch.zeros(n, k + 9, dtype=dt, device=device)
+            tall[:, 5 : k + 5] = wt
+            args = dict(act="silu", alpha=1 / math.sqrt(k))
+            ref, ref_t = ops.dense(x, w, b, r, **args), ops.dense(x, wt.t(), b, r, **args)
+            assert torch.equal(ops.dense(wide[:, 11 : k + 11], wwide[:, 3 : n + 3], b, r, **args), ref)
+            assert torch.equal(ops.dense(wide[:, 11 : k + 11], tall[:, 5 : k + 5].t(), b, r, **args), ref_t)
+            assert torch.equal(ops.dense(x[:1].expand(m, k), w, b, r, **args), ops.dense(x[:1].repeat(m, 1), w, b, r, **args))
+            more = ops.dense(torch.cat([x, x, x, x, x]), w, b, torch.cat([r, r, r, r, r]), **args)[:m]
+            tol = 2 * (1.2 * _sum_bound(x.double(), w.double(), k) / math.sqrt(k) + 64 * U) + 2 * torch.finfo(dt).eps * more.double().abs()
+            for y in (ref, ref_t):
+                assert ((y.double() - more.double()).abs() <= tol + torch.finfo(dt).smallest_normal).all()
 
 
 def test_empty(device):
