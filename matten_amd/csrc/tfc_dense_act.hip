@@ -17,8 +17,8 @@
 // pieces (dz_pieces()).
 //
 // Measured, with the library's product of the same sizes without an epilogue: fp32 6912 x 511 x 2048 118 us (library 157), with bias, ssp
-// and z 132, its gradients' products 106 and 98 (169, 125); bf16 16384 x 1024 x 4096 173 us (139), with gelu, z and residual 240,
-// its gradients' 119 and 130 (98, 197); bf16 1 x 4096 x 4096 7.3 us for 7.1 us of weights.
+// and z 132, its gradients' products 106 and 98 (169, 125); bf16 16384 x 1024 x 4096 173 us (139), with gelu, z and residual 221,
+// its gradients' 117 and 124 (98, 197); bf16 1 x 4096 x 4096 7.3 us for 7.1 us of weights.
 //
 // Few tiles and a long contraction (a weight's gradient over many rows): the contraction is split, partial tiles go to the
 // workspace and a second kernel adds them in order and applies the epilogue.
@@ -346,10 +346,10 @@ __device__ __forceinline__ void write_out(const Args& g, const floatx16 (&acc)[M
 }
 
 // (row of tiles << 32) + column of this workgroup's tile.  Neighbouring workgroups of an XCD share its L2: they take tiles in columns of
-// GROUP (64 tiles in flight read 8 + 8 operand panels instead of 2 + 32 when they go along the rows of a wide C:
-// 16384 x 1024 x 4096 in bf16 180 -> 173 us, its weight's gradient 134 -> 130; with residual and z, bound by writing, 233 -> 241).
+// GROUP, so that those in flight read few panels of both operands and write long stretches of rows.  16384 x 1024 x 4096 in bf16,
+// GROUP 1, 4, 8, 32: 180, 175, 175, 186 us; with residual and z, bound by writing, 232, 221, 241, 232.
 __device__ __forceinline__ long tile_of(const Args& g) {
-    constexpr unsigned GROUP = 8;
+    constexpr unsigned GROUP = 4;
     const unsigned tile = tfc_xcd_remap(blockIdx.x, gridDim.x), strip = GROUP * (unsigned)g.tiles_n;
     const unsigned top = tile / strip * GROUP, in = tile % strip, high = min(GROUP, (unsigned)g.tiles_m - top);
     return ((long)(top + in % high) << 32) + in / high;
