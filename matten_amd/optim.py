@@ -58,7 +58,8 @@ class _Table:
                 return False
             entries += st.values()
         try:
-            return list(map(_address, (*self.params, *entries))) == self.at
+            return (list(map(_address, (*self.params, *entries))) == self.at and list(map(_numel, self.params)) == self.sizes
+                    and all(map(_packed, self.params)))
         except TypeError:  # (not a tensor: for _check_state to name)
             return False
 

@@ -480,6 +480,18 @@ def test_refusals_on_the_device(device):
     e.grad = torch.sparse_coo_tensor(torch.tensor([[0]]), torch.ones(1, 3), (4, 3), device=device)
     with pytest.raises(RuntimeError, match="dense"):
         optim.AdamW([e]).step()
+    square = torch.nn.Parameter(torch.zeros(8, 8, device=device))
+    opt = optim.AdamW([square])
+    square.grad = torch.ones_like(square)
+    opt.step()
+    square.data = square.data.t()  # the same address, another order
+    with pytest.raises(ValueError, match="contiguous"):
+        opt.step()
+    square.data = square.data.t()[:4]  # and fewer elements, with the gradient and the state of all
+    before = square.detach().clone()
+    with pytest.raises((ValueError, RuntimeError)):
+        opt.step()
+    assert torch.equal(square, before)
     flat = torch.zeros(100, device=device)
     shared = [torch.nn.Parameter(flat[:60]), torch.nn.Parameter(flat[59:])]
     for t in shared:
