@@ -1923,6 +1923,18 @@ def _at(t: Optional[torch.Tensor]):  # (a plain address: what ctypes converts fa
     return None if t is None else t.data_ptr()
 
 
+def _stream_of(device: torch.device) -> int:
+    return torch._C._cuda_getCurrentRawStream(device.index)
+
+
+def _wants_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _layer_norm_run(x, w, b, eps: float, keep: bool):
     """(y, stats): rows of a contiguous [rows, d] tensor; `keep`: stats [2, rows] holds the mean and 1 / deviation of every row."""
     rows, d = x.shape
@@ -1931,7 +1943,7 @@ def _layer_norm_run(x, w, b, eps: float, keep: bool):
     mean = _at(stats)
     with _on(x.device):
         _lib.check(_lib.lib().tfc_layer_norm_fwd(x.data_ptr(), _at(w), _at(b), rows, d, eps, _dtype_codes[x.dtype], y.data_ptr(), mean,
-                                                 mean + 4 * rows if keep else None, _stream()))
+                                                 mean + 4 * rows if keep else None, _stream_of(x.device)))
     return y, stats
 
 
@@ -1963,7 +1975,7 @@ class _LayerNormFn(torch.autograd.Function):
                 floats = L.tfc_layer_norm_bwd_workspace_floats(rows, d, dt)
                 ws = torch.empty(floats, dtype=torch.float32, device=x.device)
             _lib.check(L.tfc_layer_norm_bwd(g.data_ptr(), x.data_ptr(), _at(w), mean, mean + 4 * rows, rows, d, dt, _at(dx), _at(dw), _at(db),
-                                            _at(ws), floats, _stream()))
+                                            _at(ws), floats, _stream_of(x.device)))
         return dx, dw, db, None
 
 
@@ -2004,7 +2016,7 @@ def layer_norm(x, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Te
             if t.shape != (d,):
                 raise ValueError(f"layer_norm: `{name}` must have shape ({d},), got {tuple(t.shape)}")
     rows, w, b = _tracked(x if x.dim() == 2 else x.reshape(-1, d)), _tracked(weight), _tracked(bias)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias)):
+    if _wants_grad(x, weight, bias):
         y = _LayerNormFn.apply(rows, w, b, float(eps))
     else:
         y = _layer_norm_run(rows, w, b, float(eps), False)[0]
@@ -2029,7 +2041,7 @@ def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0,
     b, ldb, along_n = _operand(b)
     if not a_along_k and not along_n:
         a, lda, a_along_k = a.contiguous(), max(k, 1), True
-    c = torch.empty(m, n, dtype=a.dtype, device=a.device)
+    c = a.new_empty((m, n))
     L = _lib.lib()
     dt = _dtype_codes[a.dtype]
     z = torch.empty(L.tfc_dense_z_bytes(m, n, dt), dtype=torch.uint8, device=a.device) if keep_z else None
@@ -2038,7 +2050,7 @@ def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0,
     with _on(a.device):
         floats = L.tfc_dense_workspace_floats(C.byref(d))
         ws = torch.empty(floats, dtype=torch.float32, device=a.device) if floats else None
-        _lib.check(L.tfc_dense(C.byref(d), _at(ws), floats, _stream()))
+        _lib.check(L.tfc_dense(C.byref(d), _at(ws), floats, _stream_of(a.device)))
     return c, z
 
 
@@ -2059,7 +2071,7 @@ def _dense_bwd_run(g, x, w, b, z, act: int, alpha: float, cst: float, need):
     with _on(g.device):
         floats = L.tfc_dense_bwd_workspace_floats(m, n, k, dt, act)
         ws = torch.empty(floats, dtype=torch.float32, device=g.device) if floats else None
-        _lib.check(L.tfc_dense_bwd(C.byref(d), _at(ws), floats, _stream()))
+        _lib.check(L.tfc_dense_bwd(C.byref(d), _at(ws), floats, _stream_of(g.device)))
     return dx, (dw if along_n or dw is None else dw.t()), db
 
 
@@ -2154,7 +2166,7 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
             raise ValueError(f"dense: `residual` must have shape {shape}, got {tuple(residual.shape)}")
         residual = _tracked(residual if flat else residual.reshape(rows.shape[0], n))
     args = _lib.DENSE_ACT[act], float(alpha), float(act_cst)
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual)):
+    if _wants_grad(x, weight, bias, residual):
         y = _DenseFn.apply(rows, weight, bias, residual, *args)
     else:
         y = _dense_run(rows, weight, bias, residual, *args)[0]
