@@ -219,3 +219,42 @@ def test_training_steps_together(device, bits):
     assert all(not torch.equal(p, q) for p, q in zip(b.parameters(), start))
     for p, q in zip(a.parameters(), b.parameters()):
         assert int(oa.state[p]["step"]) == int(ob.state[q]["step"]) == 7
+
+
+@pytest.mark.gpu
+def test_two_threads_at_once(device):
+    """The operators from two host threads, each on its own stream, give the bits they give one after the other."""
+    import threading
+
+    from matten_amd import ops, optim
+
+    def work(seed, out):
+        g = torch.Generator(device=device).manual_seed(seed)
+        w, v = (torch.nn.Parameter(torch.randn(130, 130, generator=g, device=device)) for _ in range(2))
+        n = torch.nn.Parameter(torch.ones(130, device=device))
+        opt = optim.AdamW([w, v, n], lr=1e-2, state_bits=8, max_grad_norm=1.0, seed=seed)
+        x = torch.randn(1500 + seed, 130, generator=g, device=device)
+        for _ in range(15):
+            opt.zero_grad()
+            y = ops.dense(ops.dense(ops.layer_norm(x, n), w, act="gelu", alpha=0.09), v, residual=x, alpha=0.09)
+            (y * y).mean().backward()
+            opt.step()
+        out[seed] = [t.detach().clone() for t in (w, v, n, y)]
+
+    alone, together = {}, {}
+    for seed in (1, 2):
+        work(seed, alone)
+    torch.cuda.synchronize()
+
+    def on_its_own_stream(seed):
+        with torch.cuda.stream(torch.cuda.Stream()):
+            work(seed, together)
+            torch.cuda.current_stream().synchronize()
+
+    threads = [threading.Thread(target=on_its_own_stream, args=(seed,)) for seed in (1, 2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for seed in (1, 2):
+        assert all(torch.equal(p, q) for p, q in zip(alone[seed], together[seed]))
