@@ -18,6 +18,7 @@ from dataclasses import dataclass
 from typing import List, NamedTuple, Optional, Sequence, Tuple
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from ._lib import FctpIns, GateSeg, GemmDesc, IMap, IrBlock, LinearIns, Path
@@ -1927,7 +1928,12 @@ def _stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
-def _wants_grad(*tensors) -> bool:
+def _watched(*tensors) -> bool:
+    """Whether the call has to be an autograd.Function: one of the tensors wants a gradient, or a trace or forward-mode
+    differentiation is under way.  The launch behind a bare `torch.empty` is visible to neither: a trace would keep the
+    uninitialised result, a dual tensor lose its tangent without a word (as a Function it is refused)."""
+    if torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0:
+        return True
     if torch.is_grad_enabled():
         for t in tensors:
             if t is not None and t.requires_grad:
@@ -1937,7 +1943,7 @@ def _wants_grad(*tensors) -> bool:
 
 def _layer_norm_run(x, w, b, eps: float, keep: bool):
     """(y, stats): rows of a contiguous [rows, d] tensor; `keep`: stats [2, rows] holds the mean and 1 / deviation of every row."""
-    rows, d = x.shape
+    rows, d = map(int, x.shape)  # (in a trace sizes are tensors)
     y = torch.empty_like(x)
     stats = torch.empty(2, rows, dtype=torch.float32, device=x.device) if keep else None
     mean = _at(stats)
@@ -1961,7 +1967,7 @@ class _LayerNormFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
             return (*_differentiable_grads(lambda *t: _layer_norm_composite(*t, ctx.eps), (x, w, b), need, g), None)
-        rows, d = x.shape
+        rows, d = map(int, x.shape)
         g = g.contiguous()
         dx = torch.empty_like(x) if need[0] else None
         dw = torch.empty_like(w) if need[1] else None
@@ -2016,7 +2022,7 @@ def layer_norm(x, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Te
             if t.shape != (d,):
                 raise ValueError(f"layer_norm: `{name}` must have shape ({d},), got {tuple(t.shape)}")
     rows, w, b = _tracked(x if x.dim() == 2 else x.reshape(-1, d)), _tracked(weight), _tracked(bias)
-    if _wants_grad(x, weight, bias):
+    if _watched(x, weight, bias):
         y = _LayerNormFn.apply(rows, w, b, float(eps))
     else:
         y = _layer_norm_run(rows, w, b, float(eps), False)[0]
@@ -2166,7 +2172,7 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
             raise ValueError(f"dense: `residual` must have shape {shape}, got {tuple(residual.shape)}")
         residual = _tracked(residual if flat else residual.reshape(rows.shape[0], n))
     args = _lib.DENSE_ACT[act], float(alpha), float(act_cst)
-    if _wants_grad(x, weight, bias, residual):
+    if _watched(x, weight, bias, residual):
         y = _DenseFn.apply(rows, weight, bias, residual, *args)
     else:
         y = _dense_run(rows, weight, bias, residual, *args)[0]

@@ -1,0 +1,45 @@
+"""-m gpu: the dense product, the layer norm and the radial networks under a trace and under forward-mode differentiation."""
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+pytestmark = pytest.mark.gpu
+
+
+def _calls(device):
+    from matten_amd import _lib, ops
+
+    g = torch.Generator(device=device).manual_seed(3)
+    r = lambda *s: torch.randn(*s, generator=g, device=device)  # noqa: E731
+    w, v, b, s = r(130, 70), r(70, 33), r(70), r(130)
+    return r, {
+        "dense": lambda x: ops.dense(x, w, b, act="silu", alpha=0.1),
+        "dense_row": lambda x: ops.dense(x[:1], w, b, act="silu", alpha=0.1),
+        "layer_norm": lambda x: ops.layer_norm(x, s, s),
+        "radial": lambda x: ops.radial_mlp_general(x, [w, v], 1.7, _lib.ACT["silu"]),
+        "together": lambda x: ops.dense(ops.layer_norm(x, s), w, b, ops.dense(x, w)),
+    }
+
+
+@pytest.mark.filterwarnings("ignore::torch.jit.TracerWarning")
+@pytest.mark.filterwarnings("ignore::DeprecationWarning")
+@pytest.mark.parametrize("name", ["dense", "dense_row", "layer_norm", "radial", "together"])
+def test_a_trace_gives_the_bits_of_the_call(device, name):
+    r, calls = _calls(device)
+    f = calls[name]
+    with torch.no_grad():
+        traced = torch.jit.trace(f, (r(40, 130),), check_trace=False)
+        for _ in range(3):
+            x = r(40, 130)
+            assert torch.equal(traced(x), f(x))
+
+
+@pytest.mark.parametrize("name", ["dense", "layer_norm", "radial"])
+def test_forward_mode_is_refused(device, name):
+    r, calls = _calls(device)
+    f = calls[name]
+    x = r(40, 130)
+    with forward_ad.dual_level():
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            f(forward_ad.make_dual(x, torch.ones_like(x)))
+        assert torch.equal(f(x), f(x.clone()))
