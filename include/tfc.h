@@ -593,7 +593,7 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
  *   dw = alpha x^T dz, packed in the order of w ([k, n], or [n, k] where w_along_k), db = the column sums of dz [n]; each nullable.
  *   x [m, k] with row stride ldx.  z is what the forward call left, wanted where tfc_dense_keeps_z() says so (layers of at
  *   most 64 x 64 form it again, from x, w and bias: one kernel, bound by reading x and dy once).  dz goes into the products in
- *   fp32, for 16-bit types in two pieces, or rounded to the type where m n, m k and n k are all 2^14 or more. */
+ *   fp32, for 16-bit types in two pieces (bf16: rounded to the type where m n, m k and n k are all 2^14 or more). */
 #define TFC_ACT_GELU 6 /* x Phi(x) with the normal distribution function Phi (tfc_dense only) */
 typedef struct tfc_dense_desc {
     int64_t m, n, k;

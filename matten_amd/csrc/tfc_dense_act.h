@@ -170,6 +170,10 @@ __device__ __forceinline__ float second_piece(T, float x) {
     return fabsf(hi) < __builtin_inff() ? (std::is_same<T, tfc_f16>::value ? left * TFC_LO_SCALE : left) : 0.f;
 }
 
+// Factor of dz = act'(z) dy in 16 bits, undone in the products' own: act' is up to 1.13, and dy up to the type's largest.  (act_cst goes into
+// the products' factor for the same reason.)
+constexpr float TFC_DZ_SCALE = 0.5f;
+
 __device__ __forceinline__ floatx16 mma(tfc_bf16, uintx4 a, uintx4 b, floatx16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }

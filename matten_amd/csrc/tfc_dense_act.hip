@@ -13,8 +13,7 @@
 //
 // What the backward pass needs of the forward one is z = alpha A B + bias.  Rounded to a 16-bit type it would be wrong by as much as the
 // results are, and the gradients by 1.5 times what their own rounding is worth: store_z() keeps more of it.  dz is rounded for the
-// products, as the matrix instruction takes it; where the products are not what the time goes into it is kept in two
-// pieces (dz_pieces()).
+// products, as the matrix instruction takes it, or kept in two pieces (dz_pieces()).
 //
 // Measured, with the library's product of the same sizes without an epilogue: fp32 6912 x 511 x 2048 118 us (library 157), with bias, ssp
 // and z 132, its gradients' products 106 and 98 (169, 125); bf16 16384 x 1024 x 4096 173 us (139), with gelu, z and residual 221,
@@ -767,7 +766,8 @@ __global__ __launch_bounds__(256) void tfc_dense_empty_kernel(const Args g) {
 }
 
 // ------------------------------------------------------------------------------------------------ backward, elementwise
-// dz = cst act'(z) dy, its second pieces `lo` elements behind the first (0: none), and the column sums of dz: a workgroup walks a slab of rows, cw threads side by side on a chunk of
+// dz / cst = act'(z) dy, for 16 bits times TFC_DZ_SCALE (both are undone in the products' factor), its second pieces `lo` elements behind
+// the first (0: none), and the column sums of dz: a workgroup walks a slab of rows, cw threads side by side on a chunk of
 // columns, 256 / cw rows at a time; its sums go to one partial row.  z null: act is the identity.
 template <class T>
 __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__ dy, const void* __restrict__ z, long rows, long n,
@@ -792,8 +792,8 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
             }
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                g[j] *= cst;
                 sum[j] += j < left ? g[j] : 0.f;
+                if (sizeof(T) == 2) g[j] *= TFC_DZ_SCALE;
             }
             if (dz) tfc_store_f<T, V>(dz + r * n + c, left, g);
             if (sizeof(T) == 2 && lo) {
@@ -812,6 +812,8 @@ __global__ __launch_bounds__(256) void tfc_dense_dz_kernel(const T* __restrict__
         for (int k = 1; k < step; ++k)
 #pragma unroll
             for (int j = 0; j < V; ++j) sum[j] += lds[(k * V + j) * cw + cl];
+#pragma unroll
+        for (int j = 0; j < V; ++j) sum[j] *= cst;
         tfc_store_f<float, V>(part + (long)blockIdx.y * n + c, left, sum);
     }
 }
@@ -1040,10 +1042,14 @@ extern "C" int64_t tfc_dense_z_bytes(int64_t m, int64_t n, int32_t dtype) {
 
 // Pieces of the element type that dz is kept in.  One is what the matrix instruction takes; the gradients' error then is sqrt 2 of what
 // their own rounding is worth.  Two take that away and double the products (backward pass in bf16 with one and two, in us:
-// 16384 x 1024 x 4096: 389, 830; 200000 x 128 x 128: 103, 144; 414 x 1281 x 21: 29, 35).  One where there are elements enough on all
-// sides for the errors to come out at that; a gradient of few elements, or from few of dz, may have several times its share.
+// 16384 x 1024 x 4096: 389, 830; 200000 x 128 x 128: 103, 144; 414 x 1281 x 21: 29, 35).  bf16: one where there are elements enough on
+// all sides for the errors to come out at that; a gradient of few elements, or from few of dz, may have several times its share.
+// fp16: always two.  One piece of what lies below 2^-14 (a small dy, a saturated act') has 2^-25 as its error whatever its size, and
+// a sum over n or m carries that into results that are not small; the second piece takes it to 2^-36 (training step with gelu in us,
+// one and two: 16384 x 1024 x 4096: 622, 1033; 6912 x 512 x 2048: 144, 176; 200000 x 128 x 128: 181, 220).
 static int dz_pieces(int64_t m, int64_t n, int64_t k, int dtype, int act) {
-    return dtype == TFC_F32 || act == TFC_ACT_IDENTITY || std::min(m * n, std::min(m * k, n * k)) >= 1 << 14 ? 1 : 2;
+    if (dtype == TFC_F32 || act == TFC_ACT_IDENTITY) return 1;
+    return dtype == TFC_F16 || std::min(m * n, std::min(m * k, n * k)) < 1 << 14 ? 2 : 1;
 }
 
 // The general backward pass's workspace: [dz | what one of its parts needs at a time], in floats.
@@ -1082,7 +1088,7 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
     hipStream_t s = (hipStream_t)stream;
     if (m > 0 && tfc_dense_is_narrow(n, k)) return tfc_dense_narrow_bwd(d, workspace, s);
     const BwdSpace space = bwd_space(m, n, k, d->dtype, d->act);
-    const bool plain = d->act == TFC_ACT_IDENTITY;  // its constant goes into the products' own factor
+    const bool plain = d->act == TFC_ACT_IDENTITY;  // dz is dy
     const void* dz = plain ? d->dy : (const void*)workspace;
     float* rest = workspace + space.dz;
     const int64_t lo = dz_pieces(m, n, k, d->dtype, d->act) == 2 ? m * n : 0;
@@ -1092,7 +1098,7 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
         if (rc) return rc;
     }
     tfc_dense_desc g{};
-    g.alpha = plain ? d->alpha * d->act_cst : d->alpha;
+    g.alpha = d->alpha * d->act_cst * (plain || d->dtype == TFC_F32 ? 1.f : 1.f / TFC_DZ_SCALE);
     g.act_cst = 1.f, g.act = TFC_ACT_IDENTITY, g.dtype = d->dtype;
     if (d->dx) {  // dz W^T
         g.m = m, g.n = k, g.k = n;

@@ -32,7 +32,7 @@ struct Narrow {
     void* dx;
     float* part;  // [workgroups][k n + n], the weight's gradient in the weight's own order
     int pk, pn;   // its strides
-    float alpha, cst, factor;  // factor = alpha cst: dz stands without its constant, which is exact where 16 bits hold dy
+    float alpha, cst, factor;  // factor = alpha cst, for 16 bits / TFC_DZ_SCALE: what dz lacks in the images
     int act;
     int want_dw;
 };
@@ -191,7 +191,8 @@ __global__ __launch_bounds__(256, 2) void tfc_dense_narrow_bwd_kernel(const Narr
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            const float v[4] = {dz[4 * q], dz[4 * q + 1], dz[4 * q + 2], dz[4 * q + 3]};
+            float v[4] = {dz[4 * q], dz[4 * q + 1], dz[4 * q + 2], dz[4 * q + 3]};
+            if constexpr (P == 1) v[0] *= TFC_DZ_SCALE, v[1] *= TFC_DZ_SCALE, v[2] *= TFC_DZ_SCALE, v[3] *= TFC_DZ_SCALE;
             put4<T>(di, r32 + (lane & 31), c32 + 8 * q + half * 4, v);
         }
         __syncthreads();
@@ -290,7 +291,8 @@ int tfc_dense_narrow_bwd(const tfc_dense_bwd_desc* d, float* part, hipStream_t s
     g.wk = d->w_along_k ? 1 : (int)d->ldw, g.wn = d->w_along_k ? (int)d->ldw : 1;
     g.dx = d->dx, g.part = part;
     g.pk = d->w_along_k ? 1 : g.n, g.pn = d->w_along_k ? g.k : 1;
-    g.alpha = d->alpha, g.cst = d->act_cst, g.factor = d->alpha * d->act_cst, g.act = d->act, g.want_dw = d->dw != nullptr;
+    g.alpha = d->alpha, g.cst = d->act_cst, g.act = d->act, g.want_dw = d->dw != nullptr;
+    g.factor = d->alpha * d->act_cst * (d->dtype == TFC_F32 ? 1.f : 1.f / TFC_DZ_SCALE);
     const int64_t blocks = tfc_dense_narrow_partials(d->m);
     {
         TfcProfScope prof("tfc_dense_narrow_bwd", stream);

@@ -2142,8 +2142,8 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
     Sums are fp32 and the epilogue is applied to them before the one rounding to the result's type.  fp32 operands are cut into
     three bf16 pieces, which loses nothing, but an operand that is not finite may give NaN for an infinity.  Results are the same from run to
     run.  For the backward pass the pre-activation is kept (bf16: to 11 significant bits, fp16: to 16; layers of at most
-    64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces, and
-    rounded to x's type where x, the weight and y all have 2^14 elements or more.  Operand rows of 2^22 elements and more are refused.
+    64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces - bf16:
+    rounded to the type where x, the weight and y all have 2^14 elements or more.  Operand rows of 2^22 elements and more are refused.
 
     Differentiable to any order: the first-order backward is fused, a backward that is itself differentiated
     (`create_graph=True`) goes through torch's activations and this kernel's products."""
