@@ -2099,7 +2099,7 @@ class _DenseFn(torch.autograd.Function):
         if not any(need[:3]):
             return None, None, None, dr, None, None, None
         if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
-            return (*_differentiable_grads(lambda *t: _dense_composite(*t, *ctx.args), (x, w, b), need, g), dr, None, None, None)
+            return (*_dense_grads(g, x, w, b, *ctx.args, need), dr, None, None, None)
         return (*_dense_bwd_run(g.contiguous(), x, w, b, z, *ctx.args, need), dr, None, None, None)
 
 
@@ -2120,17 +2120,33 @@ class _ProductFn(torch.autograd.Function):
         return da, db, None
 
 
-def _torch_act(act: int, v):
-    F = torch.nn.functional
-    return {0: lambda t: t, 1: lambda t: F.softplus(t) - math.log(2.0), 2: F.silu, 3: torch.tanh, 4: torch.abs, 5: torch.sigmoid,
-            6: F.gelu}[act](v)
+def _slope(act: int, v):
+    """act'(v) out of torch operations, differentiable to any order."""
+    if act == _lib.DENSE_ACT["tanh"]:
+        t = torch.tanh(v)
+        return 1.0 - t * t
+    if act == _lib.DENSE_ACT["abs"]:
+        return torch.sign(v)
+    if act == _lib.DENSE_ACT["gelu"]:
+        return 0.5 * torch.erfc(v * -math.sqrt(0.5)) + v * torch.exp(-0.5 * v * v) * (1.0 / math.sqrt(2.0 * math.pi))
+    s = torch.sigmoid(v)
+    if act == _lib.DENSE_ACT["ssp"]:
+        return s
+    return s * (1.0 - s) if act == _lib.DENSE_ACT["sigmoid"] else s * (1.0 + v * (1.0 - s))  # (silu)
 
 
-def _dense_composite(x, w, b, act: int, alpha: float, cst: float):
-    v = _ProductFn.apply(x, w, alpha).float()
-    if b is not None:
-        v = v + b.float()
-    return (_torch_act(act, v) * cst).to(x.dtype)
+def _dense_grads(g, x, w, b, act: int, alpha: float, cst: float, need):
+    """(dx, dw, db) that can be differentiated again, None where not needed.  16 bits: z and dz are fp32 here, and so are the products with
+    them (exact on the operands); the identity has neither, its two products are those of the fused backward."""
+    dt, dz = x.dtype, g
+    if act != _lib.DENSE_ACT["identity"]:
+        x, w = x.float(), w.float()
+        z = _ProductFn.apply(x, w, alpha)
+        dz = _slope(act, z if b is None else z + b.float()) * g.float()
+    dx = _ProductFn.apply(dz, w.t(), alpha * cst).to(dt) if need[0] else None
+    dw = _ProductFn.apply(x.t(), dz, alpha * cst).to(dt) if need[1] else None
+    db = (dz.float().sum(0) * cst).to(dt) if need[2] else None
+    return dx, dw, db
 
 
 def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, act: str = "identity",
@@ -2146,7 +2162,7 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
     rounded to the type where x, the weight and y all have 2^14 elements or more.  Operand rows of 2^22 elements and more are refused.
 
     Differentiable to any order: the first-order backward is fused, a backward that is itself differentiated
-    (`create_graph=True`) goes through torch's activations and this kernel's products."""
+    (`create_graph=True`) is this kernel's products, in fp32 where there is an activation, and torch operations between them."""
     _floats(x, "x")
     _floats(weight, "weight", x)
     if act not in _lib.DENSE_ACT:

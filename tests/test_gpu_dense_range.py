@@ -104,3 +104,50 @@ def test_both_sides_of_64(device, dt):
             assert math.isfinite(size) and size > 0
             # each is off by its own rounding (h, or half the least step), 2^-12 or 2^-15 of act'' z dy and little else: 4 h of the largest
             assert ((a - e).abs() <= 2 * h * (a.abs() + e.abs()) + 4 * h * size / 8 + torch.finfo(dt).smallest_normal * 2 * h).all()
+
+
+@pytest.mark.parametrize("dt", [BF, HALF])
+@pytest.mark.parametrize("act", ["identity", "ssp", "silu", "tanh", "abs", "sigmoid", "gelu"])
+@pytest.mark.parametrize("m,k,n", [(300, 200, 150), (40, 64, 64), (1, 70, 9)])
+def test_differentiable_backward(device, dt, act, m, k, n):
+    """First-order gradients with create_graph=True: z, dz and the sums in fp32, one rounding at the end."""
+    from matten_amd import ops
+
+    r, x, w, b = _inputs(m, k, n, dt, device, 3)
+    dy, alpha, cst = r(m, n).to(dt), 0.8 / math.sqrt(k), -1.6
+    leaves = [t.requires_grad_(True) for t in (x, w, b)]
+    grads = torch.autograd.grad(ops.dense(*leaves, act=act, alpha=alpha, act_cst=cst), leaves, dy, create_graph=True)
+    assert all(g.requires_grad for g in (grads[:2] if act == "identity" else grads))
+    X, W, B, G = (t.detach().double() for t in (x, w, b, dy))
+    z = alpha * (X @ W) + B
+    ez = alpha * _sum_bound(X, W, k) + 8 * U * (z.abs() + B.abs())
+    _, da, dda = _act(act, z)
+    dz = da * G
+    edz = G.abs() * (dda * ez + 16 * U * (1 + z.abs())) + 4 * U * dz.abs() if act != "identity" else 0 * z
+    if act == "abs":  # the sign of a z within its error of zero is either
+        edz = torch.where(z.abs() <= ez, 2 * G.abs(), edz)
+    c = abs(alpha * cst)
+    _close("dx", grads[0], alpha * cst * (dz @ W.t()), c * (_sum_bound(dz.abs() + edz, W.t(), n) + edz @ W.t().abs() + 4 * U * (dz.abs() @ W.t().abs())))
+    _close("dw", grads[1], alpha * cst * (X.t() @ dz), c * (_sum_bound(X.t(), dz.abs() + edz, m) + X.t().abs() @ edz + 4 * U * (X.t().abs() @ dz.abs())))
+    _close("db", grads[2], cst * dz.sum(0), abs(cst) * (edz.sum(0) + (64 + m / 4) * U * dz.abs().sum(0)))
+
+
+@pytest.mark.parametrize("create_graph", [False, True])
+def test_pre_activations_beyond_fp16(device, create_graph):
+    """z of 800 000 under silu: finite gradients whichever backward pass forms them."""
+    from matten_amd import ops
+
+    r, x, w, b = _inputs(20, 80, 70, HALF, device, 4)
+    x, w = torch.full_like(x, 100.0), w.clone()
+    w[:, 0] = 100.0
+    dy = torch.full((20, 70), 2.0**-6, dtype=HALF, device=device)
+    leaves = [t.requires_grad_(True) for t in (x, w)]
+    grads = torch.autograd.grad(ops.dense(*leaves, act="silu"), leaves, dy, create_graph=create_graph)
+    X, W = x.detach().double(), w.detach().double()
+    z = X @ W
+    _, da, dda = _act("silu", z)
+    dz = da * dy.double()
+    # (act'' falls off as z exp(-z): at most 1/2, and below 2^-24 of act' beyond |z| = 25, however far z is off)
+    edz = dy.double() * (torch.where(z.abs() > 25, 2.0**-24, dda * (2.0**-15 * z.abs() + _sum_bound(X, W, 80))) + 64 * U) + 2.0**-22 * dz.abs() + 2.0**-35
+    _close("dx", grads[0], dz @ W.t(), _sum_bound(dz.abs() + edz, W.t(), 70) + edz @ W.t().abs())
+    _close("dw", grads[1], X.t() @ dz, _sum_bound(X.t(), dz.abs() + edz, 20) + X.t().abs() @ edz)
