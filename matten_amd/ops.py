@@ -1304,19 +1304,16 @@ def _radial_mlp_composite(x, ws, act_cst: float, act_id: Optional[int] = None):
     for i, w in enumerate(ws):
         h = _MatmulFn.apply(h, w, False, False, 1.0 / math.sqrt(w.shape[0]))
         if i < len(ws) - 1:
-            d = w.shape[1]
+            d = int(w.shape[1])  # (in a trace sizes are tensors)
             h = _GateFn.apply(h, GateSpec(d_in=d, d_out=d, segs=((0, 0, d, 1, -1, act_id, float(act_cst)),)))
     return h
 
 
 def radial_mlp_general(x, weights: Sequence[torch.Tensor], act_cst: float, act_id: int):
     """FullyConnectedNet with any of the gate kernel's activations (eigenn/nn/utils.py:182 `mlp_activation`), layer by
-    layer: the dense product with the activation in its epilogue."""
-    name = next(k for k, v in _lib.ACT.items() if v == act_id)
-    for i, w in enumerate(weights):
-        last = i == len(weights) - 1
-        x = dense(x, w, act="identity" if last else name, alpha=1.0 / math.sqrt(w.shape[0]), act_cst=1.0 if last else act_cst)
-    return x
+    layer: the fp32 product, then the activation as a one-segment gate.  (Not `dense`, whose fp32 products give NaN where an operand is
+    infinite, and whose second order - forces under a loss - has no kernels for the activations.)"""
+    return _radial_mlp_composite(x, list(weights), act_cst, act_id)
 
 
 _SELF_ORDERINGS: "dict[tuple, tuple]" = _tensor_cache()
