@@ -592,7 +592,8 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
  *   dw = alpha x^T dz, packed in the order of w ([k, n], or [n, k] where w_along_k), db = the column sums of dz [n]; each nullable.
  *   x [m, k] with row stride ldx.  z is what the forward call left, wanted where tfc_dense_keeps_z() says so (layers of at
  *   most 64 x 64 form it again, from x, w and bias: one kernel, bound by reading x and dy once).  dz goes into the products in
- *   fp32, for 16-bit types in two pieces (bf16: rounded to the type where m n, m k and n k are all 2^14 or more). */
+ *   fp32, for 16-bit types in two pieces (bf16 without exact_dz: rounded to the type where m n, m k and n k are all 2^14 or more,
+ *   which costs half of the products and makes the gradients' error sqrt 2 of their own rounding's). */
 #define TFC_ACT_GELU 6 /* x Phi(x) with the normal distribution function Phi (tfc_dense only) */
 typedef struct tfc_dense_desc {
     int64_t m, n, k;
@@ -625,12 +626,13 @@ typedef struct tfc_dense_bwd_desc {
     void* dw;
     void* db;
     float alpha, act_cst;
-    int32_t act, dtype, w_along_k;
+    int32_t act, dtype, w_along_k, exact_dz;
 } tfc_dense_bwd_desc;
 
 int tfc_dense_keeps_z(int64_t n, int64_t k, int32_t act);
 int64_t tfc_dense_z_bytes(int64_t m, int64_t n, int32_t dtype);
-int64_t tfc_dense_bwd_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act);
+int64_t tfc_dense_bwd_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act); /* exact_dz 0 */
+int64_t tfc_dense_bwd_desc_workspace_floats(const tfc_dense_bwd_desc* desc);
 int tfc_dense_bwd(const tfc_dense_bwd_desc* desc, float* workspace, int64_t workspace_floats, tfc_stream_t stream);
 
 /* One AdamW step over many parameter tensors of one dtype (the reference's trainer steps torch.optim one tensor at a time,

@@ -143,6 +143,7 @@ class DenseBwdDesc(C.Structure):
         ("act", C.c_int32),
         ("dtype", C.c_int32),
         ("w_along_k", C.c_int32),
+        ("exact_dz", C.c_int32),
     ]
 
 
@@ -240,6 +241,7 @@ SIGNATURES = {
     "tfc_dense_keeps_z": (C.c_int, [_I64, _I64, _I32]),
     "tfc_dense_z_bytes": (_I64, [_I64, _I64, _I32]),
     "tfc_dense_bwd_workspace_floats": (_I64, [_I64, _I64, _I64, _I32, _I32]),
+    "tfc_dense_bwd_desc_workspace_floats": (_I64, [C.POINTER(DenseBwdDesc)]),
     "tfc_dense_bwd": (C.c_int, [C.POINTER(DenseBwdDesc), _P, _I64, _P]),
     "tfc_grad_sumsq_partials": (_I64, [C.POINTER(AdamwTensor), _I32]),
     "tfc_grad_sumsq": (C.c_int, [C.POINTER(AdamwTensor), _I32, _I32, _P, _P]),

@@ -1047,29 +1047,38 @@ extern "C" int64_t tfc_dense_z_bytes(int64_t m, int64_t n, int32_t dtype) {
 // fp16: always two.  One piece of what lies below 2^-14 (a small dy, a saturated act') has 2^-25 as its error whatever its size, and
 // a sum over n or m carries that into results that are not small; the second piece takes it to 2^-36 (training step with gelu in us,
 // one and two: 16384 x 1024 x 4096: 622, 1033; 6912 x 512 x 2048: 144, 176; 200000 x 128 x 128: 181, 220).
-static int dz_pieces(int64_t m, int64_t n, int64_t k, int dtype, int act) {
+// exact: the caller's choice of two.
+static int dz_pieces(int64_t m, int64_t n, int64_t k, int dtype, int act, bool exact) {
     if (dtype == TFC_F32 || act == TFC_ACT_IDENTITY) return 1;
-    return dtype == TFC_F16 || std::min(m * n, std::min(m * k, n * k)) < 1 << 14 ? 2 : 1;
+    return exact || dtype == TFC_F16 || std::min(m * n, std::min(m * k, n * k)) < 1 << 14 ? 2 : 1;
 }
 
 // The general backward pass's workspace: [dz | what one of its parts needs at a time], in floats.
 struct BwdSpace {
     int64_t dz, rest;
 };
-static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int dtype, int act) {
+static BwdSpace bwd_space(int64_t m, int64_t n, int64_t k, int dtype, int act, bool exact) {
     BwdSpace w{};
-    if (act != TFC_ACT_IDENTITY) w.dz = (m * n * dz_pieces(m, n, k, dtype, act) * (int64_t)tfc_dtype_size(dtype) + 15) / 16 * 4;
+    if (act != TFC_ACT_IDENTITY) w.dz = (m * n * dz_pieces(m, n, k, dtype, act, exact) * (int64_t)tfc_dtype_size(dtype) + 15) / 16 * 4;
     w.rest = std::max(m > 0 && n > 0 ? dz_plan(m, n, dtype).slabs * n : 0,
                       std::max(product_floats(m, k, n, dtype),
                                std::max(product_floats(k, n, m, dtype), product_floats(n, k, m, dtype))));
     return w;
 }
 
-extern "C" int64_t tfc_dense_bwd_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act) {
+static int64_t bwd_floats(int64_t m, int64_t n, int64_t k, int dtype, int act, bool exact) {
     if (m < 0 || n < 0 || k < 0 || !tfc_dtype_ok(dtype)) return 0;
     if (m > 0 && tfc_dense_is_narrow(n, k)) return tfc_dense_narrow_partials(m) * (k * n + n);
-    const BwdSpace w = bwd_space(m, n, k, dtype, act);
+    const BwdSpace w = bwd_space(m, n, k, dtype, act, exact);
     return w.dz + w.rest;
+}
+
+extern "C" int64_t tfc_dense_bwd_workspace_floats(int64_t m, int64_t n, int64_t k, int32_t dtype, int32_t act) {
+    return bwd_floats(m, n, k, dtype, act, false);
+}
+
+extern "C" int64_t tfc_dense_bwd_desc_workspace_floats(const tfc_dense_bwd_desc* d) {
+    return d ? bwd_floats(d->m, d->n, d->k, d->dtype, d->act, d->exact_dz != 0) : 0;
 }
 
 extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int64_t workspace_floats, tfc_stream_t stream) {
@@ -1083,15 +1092,16 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
     TFC_REQUIRE(m == 0 || n == 0 || (d->dy && (k == 0 || (d->x && d->w))), TFC_EINVAL, "tfc_dense_bwd: null pointer");
     TFC_REQUIRE(m == 0 || n == 0 || d->z || !tfc_dense_keeps_z(n, k, d->act), TFC_EINVAL, "tfc_dense_bwd: activation %d needs z",
                 (int)d->act);
-    TFC_REQUIRE(workspace_floats >= tfc_dense_bwd_workspace_floats(m, n, k, d->dtype, d->act) && (workspace || workspace_floats == 0),
-                TFC_EINVAL, "tfc_dense_bwd: workspace too small");
+    TFC_REQUIRE(workspace_floats >= tfc_dense_bwd_desc_workspace_floats(d) && (workspace || workspace_floats == 0), TFC_EINVAL,
+                "tfc_dense_bwd: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     if (m > 0 && tfc_dense_is_narrow(n, k)) return tfc_dense_narrow_bwd(d, workspace, s);
-    const BwdSpace space = bwd_space(m, n, k, d->dtype, d->act);
+    const bool exact = d->exact_dz != 0;
+    const BwdSpace space = bwd_space(m, n, k, d->dtype, d->act, exact);
     const bool plain = d->act == TFC_ACT_IDENTITY;  // dz is dy
     const void* dz = plain ? d->dy : (const void*)workspace;
     float* rest = workspace + space.dz;
-    const int64_t lo = dz_pieces(m, n, k, d->dtype, d->act) == 2 ? m * n : 0;
+    const int64_t lo = dz_pieces(m, n, k, d->dtype, d->act, exact) == 2 ? m * n : 0;
     if (n > 0 && ((!plain && (d->dx || d->dw)) || d->db)) {
         const int rc = dense_dz_pass(d->dy, d->z, m, n, d->dtype, d->act, d->act_cst, plain || !(d->dx || d->dw) ? nullptr : workspace,
                                      d->dx || d->dw ? lo : 0, d->db, rest, s);

@@ -2057,7 +2057,7 @@ def _dense_run(a, b, bias=None, residual=None, act: int = 0, alpha: float = 1.0,
     return c, z
 
 
-def _dense_bwd_run(g, x, w, b, z, act: int, alpha: float, cst: float, need):
+def _dense_bwd_run(g, x, w, b, z, act: int, alpha: float, cst: float, need, exact: bool):
     """(dx, dw, db) of a contiguous incoming gradient, None where not needed (tfc_dense_bwd); dw in the weight's own order."""
     m, k = x.shape
     n = w.shape[1]
@@ -2070,9 +2070,9 @@ def _dense_bwd_run(g, x, w, b, z, act: int, alpha: float, cst: float, need):
     L = _lib.lib()
     dt = _dtype_codes[g.dtype]
     d = _lib.DenseBwdDesc(m, n, k, x.data_ptr(), ldx, w.data_ptr(), ldw, _at(b), _at(z), g.data_ptr(), _at(dx), _at(dw), _at(db), alpha,
-                          cst, act, dt, not along_n)
+                          cst, act, dt, not along_n, exact)
     with _on(g.device):
-        floats = L.tfc_dense_bwd_workspace_floats(m, n, k, dt, act)
+        floats = L.tfc_dense_bwd_desc_workspace_floats(C.byref(d))
         ws = torch.empty(floats, dtype=torch.float32, device=g.device) if floats else None
         _lib.check(L.tfc_dense_bwd(C.byref(d), _at(ws), floats, _stream_of(g.device)))
     return dx, (dw if along_n or dw is None else dw.t()), db
@@ -2082,10 +2082,10 @@ class _DenseFn(torch.autograd.Function):
     """x [m, k], w [k, n]; the pre-activation is kept where the backward kernels want it."""
 
     @staticmethod
-    def forward(ctx, x, w, b, r, act: int, alpha: float, cst: float):
+    def forward(ctx, x, w, b, r, act: int, alpha: float, cst: float, exact: bool):
         y, z = _dense_run(x, w, b, r, act, alpha, cst, keep_z=bool(_lib.lib().tfc_dense_keeps_z(w.shape[1], w.shape[0], act)))
         ctx.save_for_backward(x, w, b, z)
-        ctx.args = (act, alpha, cst)
+        ctx.args, ctx.exact = (act, alpha, cst), exact
         return y
 
     @staticmethod
@@ -2094,10 +2094,10 @@ class _DenseFn(torch.autograd.Function):
         need = ctx.needs_input_grad
         dr = g if need[3] else None
         if not any(need[:3]):
-            return None, None, None, dr, None, None, None
+            return None, None, None, dr, None, None, None, None
         if torch.is_grad_enabled():  # create_graph=True: out of ops that autograd can differentiate again
-            return (*_dense_grads(g, x, w, b, *ctx.args, need), dr, None, None, None)
-        return (*_dense_bwd_run(g.contiguous(), x, w, b, z, *ctx.args, need), dr, None, None, None)
+            return (*_dense_grads(g, x, w, b, *ctx.args, need), dr, None, None, None, None)
+        return (*_dense_bwd_run(g.contiguous(), x, w, b, z, *ctx.args, need, ctx.exact), dr, None, None, None, None)
 
 
 class _ProductFn(torch.autograd.Function):
@@ -2147,7 +2147,7 @@ def _dense_grads(g, x, w, b, act: int, alpha: float, cst: float, need):
 
 
 def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None, act: str = "identity",
-          alpha: float = 1.0, act_cst: float = 1.0):
+          alpha: float = 1.0, act_cst: float = 1.0, exact_grad: bool = False):
     """y = act_cst * act(alpha * x @ weight + bias) + residual in one product (tfc_dense); x [..., k], weight [k, n] (this
     package's order; the transposed view of an [n, k] weight is taken as it lies), bias [n], residual [..., n], all fp32, bf16 or
     fp16.  `act`: identity, ssp, silu, tanh, abs, sigmoid or gelu.
@@ -2155,8 +2155,9 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
     Sums are fp32 and the epilogue is applied to them before the one rounding to the result's type.  fp32 operands are cut into
     three bf16 pieces, which loses nothing, but an operand that is not finite may give NaN for an infinity.  Results are the same from run to
     run.  For the backward pass the pre-activation is kept (bf16: to 11 significant bits, fp16: to 16; layers of at most
-    64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces - bf16:
-    rounded to the type where x, the weight and y all have 2^14 elements or more.  Operand rows of 2^22 elements and more are refused.
+    64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces.  bf16 where x, the
+    weight and y all have 2^14 elements or more: rounded to the type, which makes the gradients' error sqrt 2 of what their own
+    rounding is, unless `exact_grad` (twice the products).  Operand rows of 2^22 elements and more are refused.
 
     Differentiable to any order: the first-order backward is fused, a backward that is itself differentiated
     (`create_graph=True`) is this kernel's products, in fp32 where there is an activation, and torch operations between them."""
@@ -2186,7 +2187,7 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
         residual = _tracked(residual if flat else residual.reshape(rows.shape[0], n))
     args = _lib.DENSE_ACT[act], float(alpha), float(act_cst)
     if _watched(x, weight, bias, residual):
-        y = _DenseFn.apply(rows, weight, bias, residual, *args)
+        y = _DenseFn.apply(rows, weight, bias, residual, *args, bool(exact_grad))
     else:
         y = _dense_run(rows, weight, bias, residual, *args)[0]
     return y if flat else y.reshape(shape)

@@ -17,11 +17,11 @@ SIZES = [(256, 128, 128), (256, 64, 64), (256, 64, 65), (3, 200, 130), (700, 330
 BF, HALF = torch.bfloat16, torch.float16
 
 
-def _check(x, w, b, dy, act, alpha, cst, bias=True):
+def _check(x, w, b, dy, act, alpha, cst, bias=True, exact=False):
     from matten_amd import ops
 
     leaves = [t.requires_grad_(True) for t in ((x, w, b) if bias else (x, w))]
-    grads = torch.autograd.grad(ops.dense(x, w, b, act=act, alpha=alpha, act_cst=cst), leaves, dy)
+    grads = torch.autograd.grad(ops.dense(x, w, b, act=act, alpha=alpha, act_cst=cst, exact_grad=exact), leaves, dy)
     (m, k), n = x.shape, w.shape[1]
     h = torch.finfo(x.dtype).eps / 2
     X, W, G = x.detach().double(), w.detach().double(), dy.double()
@@ -31,7 +31,7 @@ def _check(x, w, b, dy, act, alpha, cst, bias=True):
     _, da, dda = _act(act, z)
     dz = da * G
     edz = G.abs() * (dda * ez + 16 * U * (1 + z.abs()) * torch.maximum(da.abs(), dda)) + 4 * U * dz.abs()
-    one = x.dtype == BF and min(m * k, k * n, m * n) >= 2**14 and max(k, n) > 64
+    one = x.dtype == BF and min(m * k, k * n, m * n) >= 2**14 and max(k, n) > 64 and not exact
     edb = edz
     edz = edz + (h if one else h * h) * (dz.abs() + edz) + (2.0**-35 if x.dtype == HALF else 0)
     c = abs(alpha * cst)
@@ -151,3 +151,23 @@ def test_pre_activations_beyond_fp16(device, create_graph):
     edz = dy.double() * (torch.where(z.abs() > 25, 2.0**-24, dda * (2.0**-15 * z.abs() + _sum_bound(X, W, 80))) + 64 * U) + 2.0**-22 * dz.abs() + 2.0**-35
     _close("dx", grads[0], dz @ W.t(), _sum_bound(dz.abs() + edz, W.t(), 70) + edz @ W.t().abs())
     _close("dw", grads[1], X.t() @ dz, _sum_bound(X.t(), dz.abs() + edz, 20) + X.t().abs() @ edz)
+
+
+@pytest.mark.parametrize("dt", [torch.float32, BF, HALF])
+@pytest.mark.parametrize("m,k,n", [(256, 128, 128), (700, 330, 150), (4096, 512, 640), (64, 64, 64)])
+def test_exact_grad(device, dt, m, k, n):
+    """In bf16 the gradients of a large layer are then as exact as those of a small one (h^2 of dz in the bound instead of h); elsewhere
+    nothing changes."""
+    from matten_amd import ops
+
+    r, x, w, b = _inputs(m, k, n, dt, device, 5)
+    dy = r(m, n).to(dt)
+    if dt != torch.float32:
+        _check(x, w, b, dy, "silu", 1 / math.sqrt(k), 1.3, exact=True)
+
+    def grads(**kw):
+        leaves = [t.detach().requires_grad_(True) for t in (x, w, b)]
+        return torch.autograd.grad(ops.dense(*leaves, act="silu", alpha=1 / math.sqrt(k), **kw), leaves, dy)
+
+    same = [torch.equal(p, q) for p, q in zip(grads(), grads(exact_grad=True))]
+    assert same == [False, False, True] if dt == BF and k > 64 else same == [True, True, True]
