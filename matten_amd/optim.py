@@ -1,9 +1,10 @@
 """AdamW over all parameter tensors of a model at once (tfc_adamw_step), with moments in 32 or in 8 bits and the gradients
 optionally limited to a largest global norm, in the same launches.
 
-A drop-in for the `class_path: torch.optim.Adam` / `AdamW` of the reference's configs (its trainer steps whatever optimizer the
-yaml names, eigenn/model/model.py:410-426): a `torch.optim.Optimizer` with param groups, schedulers, closures and
-`state_dict`.  Everything a step needs lives on the device - the step counts too - so that a step can be part of a captured
+Takes the place of torch.optim.AdamW in the `class_path` of a config (the reference's trainer steps whatever optimizer its yaml
+names, eigenn/model/model.py:410-426), and of torch.optim.Adam, which the reference's own configs name, where `weight_decay: 0` is
+written out: Adam's default is no decay and its decay is part of the gradient, here it is 0.01 and apart from it.  A
+`torch.optim.Optimizer` with param groups, schedulers, closures and `state_dict`.  Everything a step needs lives on the device - the step counts too - so that a step can be part of a captured
 graph (matten_amd.graphs.GraphedStep)."""
 from __future__ import annotations
 
@@ -126,6 +127,8 @@ class AdamW(torch.optim.Optimizer):
             raise ValueError(f"AdamW: betas must lie in [0, 1), got {g['betas']}")
         if g.get("amsgrad") or g.get("maximize"):  # (a loaded state dict's)
             raise ValueError("AdamW: `amsgrad` and `maximize` do not exist here")
+        if g.get("decoupled_weight_decay") is False and g["weight_decay"] != 0:
+            raise ValueError("AdamW: torch.optim.Adam's weight decay, a part of the gradient, does not exist here")
         if not 0.0 <= g["eps"] < math.inf or not 0.0 <= g["weight_decay"] < math.inf:
             raise ValueError(f"AdamW: eps and weight_decay must be finite and not negative, got {g['eps']}, {g['weight_decay']}")
 
@@ -155,8 +158,8 @@ class AdamW(torch.optim.Optimizer):
                 raise ValueError(f"AdamW: state entry `{k}` must be a contiguous {dt} tensor of {n} elements on {p.device}; got {got}")
 
     def load_state_dict(self, state_dict):
-        """Takes copies.  The moments must have this optimizer's width and the parameters' sizes; those of torch.optim.AdamW fit
-        32 bits where the parameters are fp32."""
+        """Takes copies.  The moments must have this optimizer's width and the parameters' sizes; those of torch.optim.AdamW, and of
+        torch.optim.Adam without weight decay, fit 32 bits where the parameters are fp32."""
         for g in state_dict["param_groups"]:
             self._check_group(g)
         names = _STATE[self.state_bits]

@@ -76,3 +76,28 @@ def test_codes_bracket_what_they_stand_for():
     top = x.abs().double()
     spacing = torch.maximum(a * 2.0**-3, torch.ldexp(torch.ones(4, dtype=torch.float64), lo[1].int() - 127 - 9).repeat_interleave(256)[:1000])
     assert (b - a <= spacing * (1 + 1e-12)).all() and (top - a < spacing).all()
+
+
+def test_state_of_torch_adam():
+    """Its weight decay is another update rule: a state dict that carries one is refused and leaves the optimizer as it was, at a later
+    step too; one without is taken."""
+    from matten_amd import optim
+
+    p = _param(5)
+    p.grad = torch.ones(5)
+    for torch_opt, decay, fits in ((torch.optim.Adam, 0.1, False), (torch.optim.Adam, 0.0, True), (torch.optim.AdamW, 0.1, True)):
+        source = torch_opt([p], lr=0.5, weight_decay=decay)
+        source.step()
+        q = _param(5)
+        opt = optim.AdamW([q])
+        if fits:
+            opt.load_state_dict(source.state_dict())
+            assert opt.param_groups[0]["lr"] == 0.5 and torch.equal(opt.state[q]["exp_avg"], source.state[p]["exp_avg"])
+        else:
+            with pytest.raises(ValueError, match="weight decay"):
+                opt.load_state_dict(source.state_dict())
+            assert opt.param_groups[0]["lr"] == 1e-3 and not opt.state
+        if fits and decay == 0:
+            opt.param_groups[0]["weight_decay"] = 0.1
+            with pytest.raises(ValueError, match="weight decay"):
+                opt.step()
