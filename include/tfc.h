@@ -587,7 +587,7 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
  *   b [k, n]: b_along_k: element (kk, j) at j ldb + kk, else at kk ldb + j.  (a along its rows with b along k: not built.)
  *   c: row stride ldc; residual (nullable) [m, n] with row stride ldr; bias (nullable) [n]; z (nullable), of
  *   tfc_dense_z_bytes(): receives alpha a b + bias for tfc_dense_bwd, in a form of its own.  Workspace: tfc_dense_workspace_floats() (0: none).  k = 0: the epilogue of zeros.
- * Operand rows are shorter than 2^22 elements.
+ * Operand rows are shorter than 2^22 elements (dy's too where dx or dw is wanted and m > 1).
  * tfc_dense_bwd: from dy [m, n] packed, with dz = act_cst act'(alpha x w + bias) dy:  dx = alpha dz w^T [m, k] packed,
  *   dw = alpha x^T dz, packed in the order of w ([k, n], or [n, k] where w_along_k), db = the column sums of dz [n]; each nullable.
  *   x [m, k] with row stride ldx.  z is what the forward call left, wanted where tfc_dense_keeps_z() says so (layers of at

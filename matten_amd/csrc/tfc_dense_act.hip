@@ -985,6 +985,9 @@ extern "C" int64_t tfc_dense_workspace_floats(const tfc_dense_desc* d) {
     return splits > 1 ? splits * d->m * d->n : 0;
 }
 
+// A thread's offset in a tile has 32 bits: 256 rows, or a step of 64, of the longest row.
+constexpr int64_t TFC_LD_MAX = 1 << 22;
+
 // lo_a, lo_b: bytes from an operand's first pieces to its second ones (0: there are none).
 static int dense_product(const tfc_dense_desc* d, int64_t lo_a, int64_t lo_b, float* workspace, int64_t workspace_floats,
                          tfc_stream_t stream) {
@@ -999,8 +1002,7 @@ static int dense_product(const tfc_dense_desc* d, int64_t lo_a, int64_t lo_b, fl
     TFC_REQUIRE(d->lda >= 0 && d->ldb >= 0 && d->ldc >= d->n && (!d->residual || d->ldr >= 0), TFC_EINVAL, "tfc_dense: bad stride");
     const bool few = few_rows(*d) && !lo_b;
     const Plan p = d->k && !few ? plan(d->m, d->n, d->k, d->dtype, !lo_a && !lo_b && deep_operands(*d)) : Plan{64, 64, 1, 1, 1, 0};
-    // (a thread's offset in a tile has 32 bits: 256 rows, or a step of 64, of the longest row)
-    TFC_REQUIRE(d->lda < 1 << 22 && d->ldb < 1 << 22, TFC_EUNSUPPORTED, "tfc_dense: operand rows of 2^22 elements or more");
+    TFC_REQUIRE(d->lda < TFC_LD_MAX && d->ldb < TFC_LD_MAX, TFC_EUNSUPPORTED, "tfc_dense: operand rows of 2^22 elements or more");
     TFC_REQUIRE(p.tiles_m * p.tiles_n < (int64_t)1 << 31, TFC_EUNSUPPORTED, "tfc_dense: %lld x %lld has too many tiles",
                 (long long)d->m, (long long)d->n);
     TFC_REQUIRE(p.splits == 1 || (workspace && workspace_floats >= p.splits * d->m * d->n), TFC_EINVAL,
@@ -1096,6 +1098,9 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
                 "tfc_dense_bwd: workspace too small");
     hipStream_t s = (hipStream_t)stream;
     if (m > 0 && tfc_dense_is_narrow(n, k)) return tfc_dense_narrow_bwd(d, workspace, s);
+    const int64_t ldz = m > 1 ? n : 0;  // (one row: nothing strides)
+    TFC_REQUIRE((!d->dx && !d->dw) || (ldz < TFC_LD_MAX && (!d->dx || d->ldw < TFC_LD_MAX) && (!d->dw || d->ldx < TFC_LD_MAX)), TFC_EUNSUPPORTED,
+                "tfc_dense_bwd: operand rows of 2^22 elements or more");  // (before anything is launched)
     const bool exact = d->exact_dz != 0;
     const BwdSpace space = bwd_space(m, n, k, d->dtype, d->act, exact);
     const bool plain = d->act == TFC_ACT_IDENTITY;  // dz is dy
@@ -1112,7 +1117,7 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
     g.act_cst = 1.f, g.act = TFC_ACT_IDENTITY, g.dtype = d->dtype;
     if (d->dx) {  // dz W^T
         g.m = m, g.n = k, g.k = n;
-        g.a = dz, g.lda = n, g.a_along_k = 1;
+        g.a = dz, g.lda = ldz, g.a_along_k = 1;
         g.b = d->w, g.ldb = d->ldw, g.b_along_k = !d->w_along_k;
         g.c = d->dx, g.ldc = k;
         const int rc = dense_product(&g, 2 * lo, 0, rest, space.rest, stream);
@@ -1122,10 +1127,10 @@ extern "C" int tfc_dense_bwd(const tfc_dense_bwd_desc* d, float* workspace, int6
         g.k = m, g.a_along_k = g.b_along_k = 0;
         if (d->w_along_k) {
             g.m = n, g.n = k;
-            g.a = dz, g.lda = n, g.b = d->x, g.ldb = d->ldx;
+            g.a = dz, g.lda = ldz, g.b = d->x, g.ldb = d->ldx;
         } else {
             g.m = k, g.n = n;
-            g.a = d->x, g.lda = d->ldx, g.b = dz, g.ldb = n;
+            g.a = d->x, g.lda = d->ldx, g.b = dz, g.ldb = ldz;
         }
         g.c = d->dw, g.ldc = g.n;
         return dense_product(&g, d->w_along_k ? 2 * lo : 0, d->w_along_k ? 0 : 2 * lo, rest, space.rest, stream);

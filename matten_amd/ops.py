@@ -2157,7 +2157,8 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
     run.  For the backward pass the pre-activation is kept (bf16: to 11 significant bits, fp16: to 16; layers of at most
     64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces.  bf16 where x, the
     weight and y all have 2^14 elements or more: rounded to the type, which makes the gradients' error sqrt 2 of what their own
-    rounding is, unless `exact_grad` (twice the products).  Operand rows of 2^22 elements and more are refused.
+    rounding is, unless `exact_grad` (twice the products).  Operand rows of 2^22 elements and more are refused, and so are
+    such rows of the result where x or weight wants a gradient.
 
     Differentiable to any order: the first-order backward is fused, a backward that is itself differentiated
     (`create_graph=True`) is this kernel's products, in fp32 where there is an activation, and torch operations between them."""
@@ -2185,6 +2186,8 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
         if residual.shape != shape:
             raise ValueError(f"dense: `residual` must have shape {shape}, got {tuple(residual.shape)}")
         residual = _tracked(residual if flat else residual.reshape(rows.shape[0], n))
+    if n >= 1 << 22 and rows.shape[0] > 1 and _watched(x, weight):  # (not first in the backward pass)
+        raise ValueError(f"dense: {n} columns: gradients need a result with rows of less than 2^22 elements")
     args = _lib.DENSE_ACT[act], float(alpha), float(act_cst)
     if _watched(x, weight, bias, residual):
         y = _DenseFn.apply(rows, weight, bias, residual, *args, bool(exact_grad))

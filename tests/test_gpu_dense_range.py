@@ -171,3 +171,22 @@ def test_exact_grad(device, dt, m, k, n):
 
     same = [torch.equal(p, q) for p, q in zip(grads(), grads(exact_grad=True))]
     assert same == [False, False, True] if dt == BF and k > 64 else same == [True, True, True]
+
+
+def test_one_row_of_2_to_22_columns(device):
+    """A single row has no stride: its gradients exist at any width."""
+    from matten_amd import ops
+
+    n = (1 << 22) + 5
+    r = torch.randn(n, 3, device=device)
+    x, w = torch.randn(1, 3, device=device, requires_grad=True), r.t().requires_grad_(True)
+    dy = torch.zeros(1, n, device=device)
+    dy[0, ::4099] = torch.randn(dy[0, ::4099].numel(), device=device)  # (1024 terms that are not zero: 6 roundings each, 64 for the joins)
+    dx, dw = torch.autograd.grad(ops.dense(x, w, act="tanh", alpha=0.3), [x, w], dy)
+    X, W = x.detach().double(), w.detach().double()
+    z = 0.3 * (X @ W)
+    dz = (1 - torch.tanh(z) ** 2) * dy.double()
+    edz = dy.double().abs() * (0.3 * _sum_bound(X, W, 3) + 16 * U * (1 + z.abs())) + 4 * U * dz.abs()
+    size = 0.3 * dz.abs() @ W.t().abs()
+    _close("dx", dx, 0.3 * dz @ W.t(), (6 * 1024 + 67) * U * size + 0.3 * edz @ W.t().abs())
+    _close("dw", dw, 0.3 * X.t() @ dz, 0.3 * X.t().abs() @ edz + 73 * U * 0.3 * (X.t() @ dz).abs())
