@@ -12,7 +12,8 @@ Rules for the captured function: inputs and outputs live in tensors that keep th
 values into them between replays), no host synchronisation inside (`.item()`, data-dependent shapes).  A backward pass inside
 starts from gradients that are None, and a leaf other than a parameter that collects a gradient is made inside: autograd
 accumulates into a gradient that is there on the stream where an earlier graph of the same leaf was recorded, and while that
-graph lives (the warm-up's may) this breaks the capture and ends the process.  An optimizer step may be part of the function
+graph lives (the warm-up's may) this would break the capture and end the process: GraphedStep looks for it in the last warm-up
+call (of two or more) and raises before the capture.  An optimizer step may be part of the function
 (matten_amd.optim.AdamW); the warm-up calls step it too.
 
 What may change between replays depends on `rebuild_topology`:
@@ -32,9 +33,39 @@ What may change between replays depends on `rebuild_topology`:
 """
 from __future__ import annotations
 
-from typing import Callable, Optional, Sequence
+import gc
+import weakref
+from typing import Callable, List, Optional, Sequence
 
 import torch
+from torch.autograd.graph import get_gradient_edge
+
+
+class _Accumulated:
+    """Leaves whose gradient a call added to the one that was there (`with _Accumulated() as a: fn()`)."""
+
+    @staticmethod
+    def _leaves():
+        return [t for t in gc.get_objects() if issubclass(type(t), torch.Tensor) and t.requires_grad and t.is_leaf and t.is_cuda]
+
+    def __enter__(self):
+        # (weak: the call may drop the gradients, and their memory is then free as it would be without this)
+        self._before = [(weakref.ref(t), weakref.ref(t.grad), t.grad._version) for t in self._leaves() if t.grad is not None]
+        self.leaves: List[torch.Tensor] = []
+        return self
+
+    def __exit__(self, *exc):
+        for leaf, grad, version in self._before:
+            t, g = leaf(), grad()
+            if t is not None and g is not None and t.grad is g and g._version != version:
+                self.leaves.append(t)
+
+    def held(self) -> "List[torch.Tensor]":
+        """Those among them that a graph still refers to: the node that accumulates is then the one of that graph, and on its stream.
+        (A node that nothing else holds goes with the first edge asked for, and its mark with it.)"""
+        for t in self.leaves:
+            get_gradient_edge(t).node.metadata[_Accumulated] = True
+        return [t for t in self.leaves if get_gradient_edge(t).node.metadata.pop(_Accumulated, False)]
 
 
 class GraphedStep:
@@ -57,8 +88,18 @@ class GraphedStep:
             quiet(False)
         try:
             with torch.cuda.stream(s):  # torch asks for the warm-up on a non-default stream
-                for _ in range(warmup):
+                for _ in range(warmup - 1):
                     fn()
+                if warmup > 0:
+                    with _Accumulated() as accumulated:
+                        fn()
+                    held = accumulated.held() if warmup > 1 else []
+                    if held:
+                        raise RuntimeError(
+                            f"GraphedStep: the captured function accumulates into existing gradients of {len(held)} leaves (the first of "
+                            f"shape {tuple(held[0].shape)}) that an earlier graph still refers to.  Set them to None inside the function "
+                            "(zero_grad()), or let go of what holds that graph (a loss that was not detached, say)."
+                        )
             cur.wait_stream(s)
             torch.cuda.synchronize()
             if self.rebuild_topology:

@@ -43,3 +43,27 @@ def test_forward_mode_is_refused(device, name):
         with pytest.raises((RuntimeError, NotImplementedError)):
             f(forward_ad.make_dual(x, torch.ones_like(x)))
         assert torch.equal(f(x), f(x.clone()))
+
+
+def test_accumulation_under_a_living_graph_is_seen(device):
+    """What GraphedStep asks before it captures, in eager calls on a stream of their own."""
+    from matten_amd.graphs import _Accumulated
+
+    layer = torch.nn.Linear(5, 3).to(device)
+    x = torch.randn(7, 5, device=device)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        kept = layer(x).sum()
+        kept.backward()
+        for keep, want in ((True, 2), (False, 0)):
+            if not keep:
+                kept = None
+            with _Accumulated() as a:
+                layer(x).sum().backward()
+            assert len(a.leaves) == 2 and len(a.held()) == want
+        with _Accumulated() as a:
+            layer.zero_grad()
+            layer(x).sum().backward()
+        assert not a.leaves
+    torch.cuda.current_stream().wait_stream(side)
