@@ -581,7 +581,7 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
                        tfc_stream_t stream);
 
 /* Matrix product with its epilogue: c[m, n] = act_cst act(alpha a b + bias) + residual, one dtype throughout, sums in fp32
- * (fp32 operands as three bf16 pieces each, exactly; an operand that is not finite gives NaN).  The reference's scalar layers
+ * (fp32 operands as three bf16 pieces each, exactly; an operand that is not finite, or a product beyond 2^143, gives NaN).  The reference's scalar layers
  * are torch.nn.Linear + activation (eigenn/nn/utils.py).
  *   a [m, k]: a_along_k: element (i, kk) at i lda + kk, else at kk lda + i;
  *   b [k, n]: b_along_k: element (kk, j) at j ldb + kk, else at kk ldb + j.  (a along its rows with b along k: not built.)

@@ -16,7 +16,8 @@ typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef short shortx4 __attribute__((ext_vector_type(4)));
 
-// FAST (16-bit results): exp and 1/x as single instructions, a few 2^-22 of the result off where its half step is 2^-9 or 2^-12.
+// FAST (16-bit results): exp as the power of 2 of x log2(e), 1/x as a single instruction.  exp is off by what its argument's rounding makes of
+// it, |x| 2^-24 of the result, 2^-17 at most over the range in which it is not 0 or inf, and 1/x by 2^-23; half a step of the result is 2^-9 or 2^-12.
 template <bool FAST>
 __device__ __forceinline__ float exp_(float x) {
     return FAST ? __expf(x) : expf(x);

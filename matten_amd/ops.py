@@ -2153,7 +2153,7 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
     fp16.  `act`: identity, ssp, silu, tanh, abs, sigmoid or gelu.
 
     Sums are fp32 and the epilogue is applied to them before the one rounding to the result's type.  fp32 operands are cut into
-    three bf16 pieces, which loses nothing, but an operand that is not finite may give NaN for an infinity.  Results are the same from run to
+    three bf16 pieces, which loses nothing, but an operand that is not finite, or a product beyond 2^143, may give NaN for an infinity.  Results are the same from run to
     run.  For the backward pass the pre-activation is kept (bf16: to 11 significant bits, fp16: to 16; layers of at most
     64 x 64 form it again); for these types the gradient at it goes into the two products that need it in two pieces.  bf16 where x, the
     weight and y all have 2^14 elements or more: rounded to the type, which makes the gradients' error sqrt 2 of what their own
