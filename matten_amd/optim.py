@@ -52,7 +52,7 @@ class _Table:
                 row.m, row.m_scale, row.v, row.v_scale = (st[k].data_ptr() for k in names)
 
     def holds(self, state) -> bool:
-        """Whether parameters and state still lie where the descriptors say, every parameter with a gradient."""
+        """Whether parameters and state still lie where the descriptors say, in the type they say, every parameter with a gradient."""
         entries = []
         for p, st in zip(self.params, self.states):
             if p.grad is None or state.get(p) is not st:
@@ -60,7 +60,7 @@ class _Table:
             entries += st.values()
         try:
             return (list(map(_address, (*self.params, *entries))) == self.at and list(map(_numel, self.params)) == self.sizes
-                    and all(map(_packed, self.params)))
+                    and set(map(_type, self.params)) == {self.dtype} and all(map(_packed, self.params)))
         except TypeError:  # (not a tensor: for _check_state to name)
             return False
 

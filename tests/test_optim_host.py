@@ -101,3 +101,19 @@ def test_state_of_torch_adam():
             opt.param_groups[0]["weight_decay"] = 0.1
             with pytest.raises(ValueError, match="weight decay"):
                 opt.step()
+
+
+def test_a_parameter_of_another_type_at_the_same_address():
+    """Memory that one type of 16 bits gave back may be handed to the other: the table of the last step is not the parameter's any more."""
+    from matten_amd import optim
+
+    p = _param(7, dtype=torch.bfloat16)
+    p.grad = torch.zeros_like(p)
+    state = {p: {"step": torch.zeros((), dtype=torch.int32), "exp_avg": torch.zeros(7), "exp_avg_sq": torch.zeros(7)}}
+    table = optim._Table({}, [p], [state[p]], [0], 32)
+    assert table.holds(state)
+    at = p.data_ptr()
+    p.grad = None
+    p.data = p.data.view(torch.float16)
+    p.grad = torch.zeros_like(p)
+    assert p.data_ptr() == at and not table.holds(state)
