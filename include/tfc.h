@@ -593,7 +593,7 @@ int tfc_layer_norm_bwd(const void* dy, const void* x, const void* w, const float
  *   x [m, k] with row stride ldx.  z is what the forward call left, wanted where tfc_dense_keeps_z() says so (layers of at
  *   most 64 x 64 form it again, from x, w and bias: one kernel, bound by reading x and dy once).  dz goes into the products in
  *   fp32, for 16-bit types in two pieces (bf16 without exact_dz: rounded to the type where m n, m k and n k are all 2^14 or more,
- *   which costs half of the products and makes the gradients' error sqrt 2 of their own rounding's). */
+ *   half as many products, and gradients whose error is sqrt 2 of their own rounding's). */
 #define TFC_ACT_GELU 6 /* x Phi(x) with the normal distribution function Phi (tfc_dense only) */
 typedef struct tfc_dense_desc {
     int64_t m, n, k;
