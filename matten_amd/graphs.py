@@ -90,18 +90,19 @@ class GraphedStep:
             with torch.cuda.stream(s):  # torch asks for the warm-up on a non-default stream
                 for _ in range(warmup - 1):
                     fn()
+                held: List[torch.Tensor] = []
                 if warmup > 0:
                     with _Accumulated() as accumulated:
                         fn()
                     held = accumulated.held() if warmup > 1 else []
-                    if held:
-                        raise RuntimeError(
-                            f"GraphedStep: the captured function accumulates into existing gradients of {len(held)} leaves (the first of "
-                            f"shape {tuple(held[0].shape)}) that an earlier graph still refers to.  Set them to None inside the function "
-                            "(zero_grad()), or let go of what holds that graph (a loss that was not detached, say)."
-                        )
             cur.wait_stream(s)
             torch.cuda.synchronize()
+            if held:
+                raise RuntimeError(
+                    f"GraphedStep: the captured function accumulates into existing gradients of {len(held)} leaves (the first of shape "
+                    f"{tuple(held[0].shape)}) that an earlier graph still refers to.  Set them to None inside the function (zero_grad()), or "
+                    "let go of what holds that graph (a loss that was not detached, say)."
+                )
             if self.rebuild_topology:
                 # every topology cache misses inside the capture: its kernels become part of the graph
                 ops.clear_caches()

@@ -7,8 +7,10 @@ import torch
 
 
 class _Stream:
+    waits = 0
+
     def wait_stream(self, other):
-        pass
+        _Stream.waits += 1
 
 
 @pytest.fixture
@@ -51,9 +53,10 @@ def _backward(leaves, keep=None):
 def test_accumulation_under_a_living_graph_is_refused(step):
     leaves, make = step
     held = (leaves[0] ** 2).sum()  # a loss that someone kept
+    _Stream.waits = 0
     with pytest.raises(RuntimeError, match="1 leaves .*shape \\(3,\\)"):
         make(lambda: _backward(leaves[:2]))
-    assert make.captured == 0
+    assert make.captured == 0 and _Stream.waits == 2  # (the warm-up's stream for the caller's work before, and that for the warm-up)
     del held
     make(lambda: _backward(leaves[:2]))
     assert make.captured == 1
