@@ -52,7 +52,7 @@ class _Table:
                 row.m, row.m_scale, row.v, row.v_scale = (st[k].data_ptr() for k in names)
 
     def holds(self, state) -> bool:
-        """Whether parameters and state still lie where the descriptors say, in the type they say, every parameter with a gradient."""
+        """Whether parameters and state still lie where the descriptors say, every parameter with a gradient."""
         entries = []
         for p, st in zip(self.params, self.states):
             if p.grad is None or state.get(p) is not st:
@@ -60,7 +60,7 @@ class _Table:
             entries += st.values()
         try:
             return (list(map(_address, (*self.params, *entries))) == self.at and list(map(_numel, self.params)) == self.sizes
-                    and set(map(_type, self.params)) == {self.dtype} and all(map(_packed, self.params)))
+                    and all(map(_packed, self.params)))
         except TypeError:  # (not a tensor: for _check_state to name)
             return False
 
@@ -237,13 +237,11 @@ class AdamW(torch.optim.Optimizer):
             self._check_state(p)
         return _Table(group, params, [self.state[p] for p in params], indexes, self.state_bits)
 
-    @torch.no_grad()
-    def step(self, closure=None):
-        loss = None
-        if closure is not None:
-            with torch.enable_grad():
-                loss = closure()
-        tables = self._gather()
+    @staticmethod
+    def _point_at_gradients(tables) -> Optional[list]:
+        """Checks the gradients and puts their addresses into the tables.  Returns what has to live as long as these are used, or None
+        where a table is out of date: the parameters' type has changed at the same addresses (memory that one type of 16 bits gave back
+        and the other was handed; looked for only here, where it shows, since every step would pay for it)."""
         copies = []  # gradients that are not contiguous
         for t in tables:
             dtype, at = t.dtype, t.device.index
@@ -253,6 +251,8 @@ class AdamW(torch.optim.Optimizer):
             grads = [p.grad for p in t.params]
             if set(map(_type, grads)) != {dtype} or set(map(_layout, grads)) != {torch.strided} or set(map(_device, grads)) != {at} \
                     or list(map(_numel, grads)) != t.sizes:
+                if any(p.dtype != dtype for p in t.params):
+                    return None
                 p, g = next((p, g) for p, g, n in zip(t.params, grads, t.sizes)
                             if g.dtype != dtype or g.layout != torch.strided or g.get_device() != at or g.numel() != n)
                 raise RuntimeError(f"AdamW: a gradient must be a dense {dtype} tensor of shape {tuple(p.shape)} on {t.device}; got "
@@ -262,6 +262,20 @@ class AdamW(torch.optim.Optimizer):
                 copies += grads
             for row, address in zip(t.each, map(_address, grads)):
                 row.g = address
+        return copies
+
+    @torch.no_grad()
+    def step(self, closure=None):
+        loss = None
+        if closure is not None:
+            with torch.enable_grad():
+                loss = closure()
+        tables = self._gather()
+        copies = self._point_at_gradients(tables)
+        if copies is None:
+            self._tables = None
+            tables = self._gather()
+            copies = self._point_at_gradients(tables)  # noqa: F841 (kept until the launches are queued)
         L = _lib.lib()
         partials, n_partials = None, 0
         self.grad_norm = None

@@ -67,3 +67,26 @@ def test_accumulation_under_a_living_graph_is_seen(device):
             layer(x).sum().backward()
         assert not a.leaves
     torch.cuda.current_stream().wait_stream(side)
+
+
+def test_adamw_steps_a_parameter_that_came_back_in_another_type(device):
+    """bf16 memory handed to fp16 between two steps: the second step is one of fp16, with the moments of before."""
+    from matten_amd import optim
+
+    p = torch.nn.Parameter(torch.randn(300, device=device).to(torch.bfloat16))
+    opt = optim.AdamW([p], lr=0.1)
+    p.grad = torch.randn_like(p)
+    opt.step()
+    values = torch.randn(300, device=device).half()
+    moments = {k: v.clone() for k, v in opt.state[p].items()}
+    at, p.grad = p.data_ptr(), None
+    p.data = p.data.view(torch.float16)
+    p.data.copy_(values)
+    assert p.data_ptr() == at
+    p.grad = torch.randn_like(p)
+    q = torch.nn.Parameter(values.clone())
+    fresh = optim.AdamW([q], lr=0.1)
+    fresh.state[q].update(moments)
+    q.grad = p.grad.clone()
+    opt.step(), fresh.step()
+    assert p.dtype == torch.float16 and torch.equal(p, q) and all(torch.equal(opt.state[p][k], fresh.state[q][k]) for k in moments)

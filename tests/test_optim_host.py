@@ -109,11 +109,16 @@ def test_a_parameter_of_another_type_at_the_same_address():
 
     p = _param(7, dtype=torch.bfloat16)
     p.grad = torch.zeros_like(p)
-    state = {p: {"step": torch.zeros((), dtype=torch.int32), "exp_avg": torch.zeros(7), "exp_avg_sq": torch.zeros(7)}}
-    table = optim._Table({}, [p], [state[p]], [0], 32)
-    assert table.holds(state)
+    state = {"step": torch.zeros((), dtype=torch.int32), "exp_avg": torch.zeros(7), "exp_avg_sq": torch.zeros(7)}
+    table = lambda: optim._Table({"lr": 1e-3}, [p], [state], [0], 32)  # noqa: E731
+    old, point = table(), optim.AdamW._point_at_gradients
+    old.device = torch.device("cpu", -1)  # (what a host tensor's get_device says)
+    assert point([old]) == []
     at = p.data_ptr()
     p.grad = None
     p.data = p.data.view(torch.float16)
     p.grad = torch.zeros_like(p)
-    assert p.data_ptr() == at and not table.holds(state)
+    assert p.data_ptr() == at and old.holds({p: state}) and point([old]) is None
+    new = table()
+    new.device = old.device
+    assert point([new]) == [] and new.each[0].g == p.grad.data_ptr()
