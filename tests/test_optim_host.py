@@ -1,4 +1,6 @@
 """CPU: what optim.AdamW refuses before it touches a device, and the plain step the GPU tests compare with."""
+from types import SimpleNamespace
+
 import pytest
 import torch
 
@@ -112,7 +114,7 @@ def test_a_parameter_of_another_type_at_the_same_address():
     state = {"step": torch.zeros((), dtype=torch.int32), "exp_avg": torch.zeros(7), "exp_avg_sq": torch.zeros(7)}
     table = lambda: optim._Table({"lr": 1e-3}, [p], [state], [0], 32)  # noqa: E731
     old, point = table(), optim.AdamW._point_at_gradients
-    old.device = torch.device("cpu", -1)  # (what a host tensor's get_device says)
+    old.device = SimpleNamespace(index=-1)  # (what a host tensor's get_device says)
     assert point([old]) == []
     at = p.data_ptr()
     p.grad = None
