@@ -1925,17 +1925,21 @@ def _stream_of(device: torch.device) -> int:
     return torch._C._cuda_getCurrentRawStream(device.index)
 
 
+def _wants_grad(*tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
 def _watched(*tensors) -> bool:
     """Whether the call has to be an autograd.Function: one of the tensors wants a gradient, or a trace or forward-mode
     differentiation is under way.  The launch behind a bare `torch.empty` is visible to neither: a trace would keep the
     uninitialised result, a dual tensor lose its tangent without a word (as a Function it is refused)."""
     if torch._C._get_tracing_state() is not None or forward_ad._current_level >= 0:
         return True
-    if torch.is_grad_enabled():
-        for t in tensors:
-            if t is not None and t.requires_grad:
-                return True
-    return False
+    return _wants_grad(*tensors)
 
 
 def _layer_norm_run(x, w, b, eps: float, keep: bool):
@@ -2186,7 +2190,7 @@ def dense(x, weight, bias: Optional[torch.Tensor] = None, residual: Optional[tor
         if residual.shape != shape:
             raise ValueError(f"dense: `residual` must have shape {shape}, got {tuple(residual.shape)}")
         residual = _tracked(residual if flat else residual.reshape(rows.shape[0], n))
-    if n >= 1 << 22 and rows.shape[0] > 1 and _watched(x, weight):  # (not first in the backward pass)
+    if n >= 1 << 22 and rows.shape[0] > 1 and _wants_grad(x, weight):  # (not first in the backward pass)
         raise ValueError(f"dense: {n} columns: gradients need a result with rows of less than 2^22 elements")
     args = _lib.DENSE_ACT[act], float(alpha), float(act_cst)
     if _watched(x, weight, bias, residual):

@@ -54,5 +54,7 @@ def test_dense_refuses_wide_results_with_gradients(monkeypatch):
         assert ops.dense(x[:1], w).shape == (1, 1 << 22)
         with torch.no_grad():
             assert ops.dense(x, w).shape == (3, 1 << 22)
+            with torch.autograd.forward_ad.dual_level():  # (an autograd.Function then, and still no gradient)
+                assert ops.dense(x, w).shape == (3, 1 << 22)
         leaf.requires_grad_(False)
         calls.clear()
